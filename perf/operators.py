@@ -160,8 +160,9 @@ def _empty(*shape, dtype=torch.float32):
     return torch.empty(shape, device="cuda", dtype=dtype)
 
 
-def _ldq(k):
-    return (k + 15) // 16 * 16
+def _q8(t, k):
+    """Room for t quantised rows of k, in whole tiles."""
+    return _empty((t + 15) // 16 * 16, (k + 127) // 128 * 128, dtype=torch.int8)
 
 
 def prepare(case, seed):
@@ -173,13 +174,13 @@ def prepare(case, seed):
         s.lins = [[s.linear(g, "%s.%d.%d" % (s.prefix, i, p), n, k) for p in range(c["parts"])] for i in range(c["layers"])]
         s.x = [_randn(g, t, k, dtype=TYPES[c["x_type"]]) for _ in s.lins]
         s.y = [[_empty(t, n // 2 if c["glu"] else n, dtype=y) for _ in parts] for parts in s.lins]
-        s.q, s.s = _empty(t, _ldq(k), dtype=torch.int8), _empty(t)
+        s.q, s.s = _q8(t, k), _empty(t)
     elif c["kind"] == "mlp":
         h, f = c["hidden"], c["n_ff"]
         s.lins = [[s.linear(g, "%s.%d.gate_up" % (s.prefix, i), 2 * f, h), s.linear(g, "%s.%d.down" % (s.prefix, i), h, f)] for i in range(c["layers"])]
         s.x, s.ab = [_randn(g, t, h) * 4 for _ in s.lins], [_randn(g, t, h) for _ in s.lins]
         s.nw = [1 + 0.1 * _randn(g, h) for _ in s.lins]
-        s.q, s.s, s.a = _empty(t, _ldq(h), dtype=torch.int8), _empty(t), _empty(t, f, dtype=torch.float16)
+        s.q, s.s, s.a = _q8(t, h), _empty(t), _empty(t, f, dtype=torch.float16)
         s.y = [_empty(t, h, dtype=torch.float16) for _ in s.lins]
     else:
         v = c["vocab"]
