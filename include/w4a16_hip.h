@@ -501,6 +501,57 @@ int w4a16_chain_graph_create(w4a16_ctx* ctx, const char* prefix, size_t layer0, 
 int w4a16_bench_chain(w4a16_ctx* ctx, const char* prefix, size_t n_layers, uint64_t x_dev, size_t t, uint64_t y_dev,
                       size_t warmup, size_t reps, int use_graph, int fused, float* ms_events, double* ms_wall);
 
+/* ------------------------------------------------------------------------------------------------------------
+ * W8A8 linears: int8 weights w [n][k] with one scale per output channel, activations quantised to int8 with one scale
+ * per row.  The reference keeps its language-model heads this way (int8 weights, assets/head.cu); its activations stay
+ * floats there.
+ *     y[m][c] = (sum_k q[m][k] w[c][k]) * s[m] * ws[c]
+ * The sum is exact (32-bit whole numbers; k <= 131071), the two products are rounded to f32 in this order and the result
+ * once more to y's type.
+ * A row x is quantised as s = fl32(max |x| / 127), q = the whole number nearest to x / s (halves to the even one), exactly;
+ * a row whose s would fall below 2^-126 counts as zeros (s = 0), a row that holds infinity or NaN has s = NaN (and so has
+ * every output of it) and q = 0.
+ * Every call is ordered on the launch stream, may be captured, and does not synchronise.
+ * ---------------------------------------------------------------------------------------------------------- */
+enum { W4A16_F32 = 0, W4A16_F16 = 1, W4A16_BF16 = 2, W4A16_Q8 = 3 }; /* element types; Q8: quantised rows, see below */
+
+/* Registers w int8 [n][k] (row-major, any n and k) and its scales [n] (s_type: f32, f16 or bf16) under `name`, in a name
+ * space of its own.  A name registered before gets the new weights; graphs captured until then are stale
+ * (W4A16_ERR_STALE_GRAPH).  Only the re-laid-out copy stays on the device. */
+int w4a16_upload_lin_w8a8(w4a16_ctx* ctx, const char* name, const void* q, size_t qlen_bytes, const void* s, size_t slen_bytes, size_t n,
+                          size_t k, int s_type);
+int w4a16_lin_w8a8_info(w4a16_ctx* ctx, const char* name, size_t* n, size_t* k);
+
+/* Bytes of a buffer for t quantised rows of k (0 where no such rows exist).  The rows lie in tiles: with R = 1 (t == 1), 4 (t <= 4)
+ * or 16, element (m, j) is byte ((m / R * K + j / 16) * R + m % R) * 16 + j % 16, K = 8 * ceil(k / 128).  Bytes of no
+ * element are left as they are, and never matter. */
+size_t w4a16_q8_bytes(size_t t, size_t k);
+/* x (f32, f16 or bf16, rows ldx elements apart, 0 = k) -> q (w4a16_q8_bytes(t, k) bytes, 16-byte aligned) and s f32 [t]. */
+int w4a16_quant_rows(w4a16_ctx* ctx, uint64_t x_dev, int x_type, size_t ldx, size_t t, size_t k, uint64_t q_dev, uint64_t s_dev);
+/* w4a16_norm_resid with its f32 result quantised as by w4a16_quant_rows instead of stored, in one launch; the same bits as the two.
+ * x <- x + ab. */
+int w4a16_norm_resid_q8(w4a16_ctx* ctx, uint64_t x_dev, uint64_t nw_dev, uint64_t ab_dev, uint64_t q_dev, uint64_t s_dev, size_t t,
+                        size_t w_off, size_t hidden);
+
+/* y [t][n] (f32, f16 or bf16).  x: rows of floats (x_type, ldx as above, xs_dev = 0), quantised into a buffer of the context on the
+ * way; or x_type = W4A16_Q8: x_dev and xs_dev are the q and s of t rows of k, which several linears may read (ldx = 0). */
+int w4a16_lin_forward_w8a8(w4a16_ctx* ctx, const char* name, uint64_t x_dev, int x_type, size_t ldx, uint64_t xs_dev, size_t t,
+                           uint64_t y_dev, int y_type);
+/* A fused gate|up linear (rows 0..n/2 gate, n/2..n up; n a multiple of 32) with its activation: y [t][n/2] = act(gate) * up on the f32
+ * values of w4a16_lin_forward_w8a8, rounded once to y's type.  act: W4A16_ACT_SILU or W4A16_ACT_GELU_TANH. */
+int w4a16_lin_forward_w8a8_glu(w4a16_ctx* ctx, const char* name, uint64_t x_dev, int x_type, size_t ldx, uint64_t xs_dev, size_t t,
+                               uint64_t y_dev, int y_type, int act);
+
+/* Scores rows of logits z [t][n_vocab] (f32, f16 or bf16, rows ld elements apart, 0 = n_vocab); results of no interest are 0.
+ *   targets int32 [t], logp f32 [t]: log softmax(z)[target]; 0 for a negative target (none is asked for), NaN for one >= n_vocab;
+ *   entropy f32 [t]: -sum p log p, natural logarithm;
+ *   top_idx int32 [t][top_k], top_logp f32 [t][top_k]: the top_k (up to 32) most likely tokens, best first, of equal logits the lower
+ *     token first, NaN ahead of everything, and their log probabilities.
+ * -infinity rules a token out: log probability -infinity, no part in the entropy.  A row of nothing else has entropy 0 and gives every
+ * token -infinity.  A row that holds NaN or +infinity has NaN for logp, entropy and top_logp. */
+int w4a16_token_logprobs(w4a16_ctx* ctx, uint64_t logits_dev, int logits_type, size_t ld, size_t t, size_t n_vocab, uint64_t targets_dev,
+                         uint64_t logp_dev, uint64_t entropy_dev, size_t top_k, uint64_t top_idx_dev, uint64_t top_logp_dev);
+
 #ifdef __cplusplus
 }
 #endif

@@ -112,6 +112,15 @@ static const char* const kMoeSyms[] = {W4_MOE_FAMILY("w4a16_moe_g32_f16"),
                                        "w4a16_moe_topk_sum_f16",
                                        nullptr};
 
+static const char* const kQuantSyms[] = {"w4a16_quant_rows_f32", "w4a16_quant_rows_f16", "w4a16_quant_rows_bf16", "w4a16_norm_resid_q8", "w4a16_tile_w8",
+                                         nullptr};
+// row blocks per workgroup and token tiles; gated builds (kernels/w8a8.hip)
+#define W8_TT(P, S) P "_t1" S, P "_t2" S, P "_t3" S, P "_t4" S
+static const char* const kW8a8Syms[] = {W8_TT("w4a16_w8a8_skinny_r1", ""), W8_TT("w4a16_w8a8_skinny_r2", ""), W8_TT("w4a16_w8a8_skinny_r4", ""),
+                                        W8_TT("w4a16_w8a8_skinny_r2", "_glu"), W8_TT("w4a16_w8a8_skinny_r4", "_glu"),
+                                        "w4a16_w8a8_tiled_m128", "w4a16_w8a8_tiled_m128_glu", nullptr};
+static const char* const kScoreSyms[] = {"w4a16_token_logprobs_f32", "w4a16_token_logprobs_f16", "w4a16_token_logprobs_bf16", nullptr};
+
 struct W4Asset {
     const char* name;
     const char* const* syms;
@@ -126,6 +135,9 @@ static const W4Asset kAssets[] = {
     {"moe", kMoeSyms},
     {"glue", kGlueSyms},
     {"util", kUtilSyms},
+    {"quant", kQuantSyms},
+    {"w8a8", kW8a8Syms},
+    {"score", kScoreSyms},
 };
 static const size_t kAssetCount = sizeof kAssets / sizeof kAssets[0];
 

@@ -29,6 +29,12 @@ struct W4Lin {
     std::vector<size_t> part_n;  // a fused linear: the rows of each part, in order (empty for a linear uploaded as one)
 };
 
+// One registered W8A8 linear: int8 weights in tiles (kernels/q8_common.hpp), f32 scales padded to whole row blocks.
+struct W8Lin {
+    uint64_t q = 0, s = 0;
+    size_t n = 0, k = 0;
+};
+
 // The experts of one MoE layer: two arenas in the tiled layout, experts at a fixed stride
 // (reference: moe_m13 / moe_s13 / moe_m2 / moe_s2, w4a16_dec/upload.rs:1116-1235).
 struct W4Experts {
@@ -83,6 +89,11 @@ struct w4a16_ctx {
     size_t allocated = 0;
     std::map<std::string, W4Lin, std::less<>> lins;
     std::map<std::string, W4Experts, std::less<>> experts;
+    std::map<std::string, W8Lin, std::less<>> w8lins;
+    uint64_t q8 = 0, q8_scales = 0;  // quantised rows of a W8A8 linear that was given rows of floats
+    size_t q8_cap = 0, q8_scales_cap = 0;
+    uint64_t score_ws = 0, score_tickets = 0;  // records of the segments of a row of logits, one ticket per row
+    size_t score_ws_cap = 0, score_tickets_cap = 0;
     W4MoeScratch moe;
     W4ChainScratch chain;
     // prefill launch plans: (t, n, k, group, pinned tile, pinned slices, 1 = k kept whole | 2 = gated) -> {tile rows, k slices,
@@ -127,6 +138,10 @@ constexpr int kW4PfBn = 256;                // PF_BN (prefill.hip): block tile c
 constexpr int kW4PfKs = 128;                // PF_KS (prefill.hip): k per LDS stage
 constexpr int kW4PfMoeIdsAt = 36864;        // PF_MOE_IDS_AT (prefill.hip): LDS bytes ahead of the grouped kernels' slot ids
 constexpr int kW4PfThreads = 256;           // PF_THREADS (prefill.hip)
+constexpr int kW4Q8MaxK = 131071;           // Q8_MAX_K (q8_common.hpp)
+constexpr int kW4ScoreStage = 1024;         // SCORE_STAGE (score.hip): elements of a wave's stage
+constexpr int kW4ScoreMaxTop = 32;          // SCORE_MAX_TOP
+constexpr int kW4ScoreRecord = 272;         // SCORE_RECORD
 
 int w4_fail(int code, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
 int w4_hip(hipError_t e, const char* api);

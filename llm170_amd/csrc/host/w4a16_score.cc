@@ -1,0 +1,46 @@
+// Scoring of logits (kernels/score.hip): log probabilities of given tokens, entropy, most likely tokens.
+#include <algorithm>
+
+#include "w4a16_internal.h"
+
+// Workgroups per row: one where the rows fill the chip; with fewer rows a row is cut into segments of at least 4096 elements (one
+// stage of a workgroup's four waves), about four workgroups per CU.
+static size_t score_segments(size_t t, size_t vocab, size_t cus) {
+    const size_t most = (vocab + kW4ScoreStage * 4 - 1) / (kW4ScoreStage * 4), want = (4 * cus + t - 1) / t;
+    return std::max<size_t>(1, std::min(std::min(most, want), (size_t)256));
+}
+
+extern "C" int w4a16_token_logprobs(w4a16_ctx* ctx, uint64_t logits_dev, int logits_type, size_t ld, size_t t, size_t n_vocab,
+                                    uint64_t targets_dev, uint64_t logp_dev, uint64_t entropy_dev, size_t top_k, uint64_t top_idx_dev,
+                                    uint64_t top_logp_dev) {
+    if (!ctx || !logits_dev) return w4_fail(W4A16_ERR_ARG, "token_logprobs: null operand");
+    if (logits_type != W4A16_F32 && logits_type != W4A16_F16 && logits_type != W4A16_BF16)
+        return w4_fail(W4A16_ERR_ARG, "token_logprobs: logits type %d (0 = f32, 1 = f16, 2 = bf16)", logits_type);
+    if (t == 0 || t > 0x7fffff00u || n_vocab == 0 || n_vocab > 0x7fffff00u)
+        return w4_fail(W4A16_ERR_SHAPE, "token_logprobs: t=%zu n_vocab=%zu outside 1..2^31-256", t, n_vocab);
+    if (ld == 0) ld = n_vocab;
+    if (ld < n_vocab) return w4_fail(W4A16_ERR_SHAPE, "token_logprobs: ld=%zu below n_vocab=%zu", ld, n_vocab);
+    if (top_k > kW4ScoreMaxTop || top_k > n_vocab)
+        return w4_fail(W4A16_ERR_SHAPE, "token_logprobs: top_k=%zu above %d or n_vocab=%zu", top_k, kW4ScoreMaxTop, n_vocab);
+    if ((logp_dev != 0) != (targets_dev != 0)) return w4_fail(W4A16_ERR_ARG, "token_logprobs: targets and logp come together");
+    if (top_k ? !top_idx_dev && !top_logp_dev : top_idx_dev || top_logp_dev)
+        return w4_fail(W4A16_ERR_ARG, "token_logprobs: top_k=%zu and its results come together", top_k);
+    if (!logp_dev && !entropy_dev && !top_k) return w4_fail(W4A16_ERR_ARG, "token_logprobs: no result asked for");
+    if (logits_dev % (logits_type == W4A16_F32 ? 4 : 2) || (targets_dev | logp_dev | entropy_dev | top_idx_dev | top_logp_dev) % 4)
+        return w4_fail(W4A16_ERR_ARG, "token_logprobs: operands must be aligned to their elements");
+    W4_TRY(w4_hip(hipSetDevice(ctx->device), "hipSetDevice"));
+    const size_t want = score_segments(t, n_vocab, (size_t)std::max(ctx->cu_count, 1)), stage = kW4ScoreStage * 4;
+    const size_t seg_len = ((n_vocab + want - 1) / want + stage - 1) / stage * stage, segs = (n_vocab + seg_len - 1) / seg_len;
+    if (segs > 1) {
+        W4_TRY(w4_ensure(ctx, &ctx->score_ws, &ctx->score_ws_cap, t * segs * kW4ScoreRecord));
+        if (t * 4 > ctx->score_tickets_cap) {
+            W4_TRY(w4_ensure(ctx, &ctx->score_tickets, &ctx->score_tickets_cap, std::max<size_t>(t * 4, 8192)));
+            W4_TRY(w4a16_memset0(ctx, ctx->score_tickets, ctx->score_tickets_cap));
+        }
+    }
+    uint64_t ws = ctx->score_ws, tickets = ctx->score_tickets;
+    int v = (int)n_vocab, top = (int)top_k, sg = (int)segs, sl = (int)std::min<size_t>(seg_len, 0x7fffffff);
+    void* params[] = {&logits_dev, &ld, &v, &targets_dev, &logp_dev, &entropy_dev, &top, &top_idx_dev, &top_logp_dev, &sg, &sl, &ws, &tickets};
+    const char* sym = logits_type == W4A16_F32 ? "w4a16_token_logprobs_f32" : logits_type == W4A16_F16 ? "w4a16_token_logprobs_f16" : "w4a16_token_logprobs_bf16";
+    return w4_launch(ctx, sym, (unsigned)(t * segs), 1, 256, 0, params);
+}

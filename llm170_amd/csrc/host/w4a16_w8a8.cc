@@ -1,0 +1,230 @@
+// W8A8 linears: registration, quantisation of activation rows, regime dispatch (kernels/quant.hip, kernels/w8a8.hip).
+#include <algorithm>
+#include <cmath>
+#include <cstdio>
+#include <cstring>
+
+#include "w4a16_internal.h"
+
+static inline unsigned ceil_div(size_t a, size_t b) { return (unsigned)((a + b - 1) / b); }
+
+// k tiles of a row block: whole pairs of 64 k (q8_common.hpp)
+static size_t k_tiles(size_t k) { return (k + 127) / 128 * 2; }
+// rows of an activation tile
+static size_t tile_rows(size_t t) { return t == 1 ? 1 : t <= 4 ? 4 : 16; }
+
+static size_t type_bytes(int type) { return type == W4A16_F32 ? 4 : 2; }
+static bool float_type(int type) { return type == W4A16_F32 || type == W4A16_F16 || type == W4A16_BF16; }
+static const char* type_name(int type) { return type == W4A16_F32 ? "f32" : type == W4A16_F16 ? "f16" : "bf16"; }
+
+static int check_rows(const char* what, size_t t, size_t k) {
+    if (t == 0 || t > 0x7fffff00u || k == 0 || k > kW4Q8MaxK)
+        return w4_fail(W4A16_ERR_SHAPE, "%s: t=%zu k=%zu outside 1..2^31-256 and 1..%d", what, t, k, kW4Q8MaxK);
+    return 0;
+}
+
+extern "C" size_t w4a16_q8_bytes(size_t t, size_t k) {
+    if (t == 0 || t > 0x7fffff00u || k == 0 || k > kW4Q8MaxK) return 0;
+    const size_t r = tile_rows(t);
+    return (t + r - 1) / r * r * k_tiles(k) * 64;
+}
+
+static int quant_rows(w4a16_ctx* ctx, uint64_t x, int x_type, size_t ldx, size_t t, size_t k, uint64_t q, uint64_t s) {
+    char sym[64];
+    snprintf(sym, sizeof sym, "w4a16_quant_rows_%s", type_name(x_type));
+    const size_t chunks = (k + 15) / 16;
+    const int r = (int)tile_rows(t);
+    // as many threads as a row has chunks, up to four waves; few rows take up to sixteen
+    const unsigned block = (unsigned)std::min<size_t>((chunks + 63) / 64 * 64, t <= 64 ? 1024 : 256);
+    const unsigned grid = r == 16 ? ceil_div(t, 128) * 128 : (unsigned)t;
+    int ki = (int)k, kt = (int)k_tiles(k), ri = r, ti = (int)t, bi = (int)block;
+    void* params[] = {&x, &ldx, &ki, &kt, &ri, &q, &s, &ti, &bi};
+    return w4_launch(ctx, sym, grid, 1, block, 0, params);
+}
+
+extern "C" int w4a16_quant_rows(w4a16_ctx* ctx, uint64_t x_dev, int x_type, size_t ldx, size_t t, size_t k, uint64_t q_dev, uint64_t s_dev) {
+    if (!ctx || !x_dev || !q_dev || !s_dev) return w4_fail(W4A16_ERR_ARG, "quant_rows: null operand");
+    if (!float_type(x_type)) return w4_fail(W4A16_ERR_ARG, "quant_rows: x type %d (0 = f32, 1 = f16, 2 = bf16)", x_type);
+    W4_TRY(check_rows("quant_rows", t, k));
+    if (ldx == 0) ldx = k;
+    if (ldx < k) return w4_fail(W4A16_ERR_SHAPE, "quant_rows: ldx=%zu below k=%zu", ldx, k);
+    if (x_dev % type_bytes(x_type) || s_dev % 4 || q_dev % 16)
+        return w4_fail(W4A16_ERR_ARG, "quant_rows: x and s must be aligned to their elements, q to 16 bytes");
+    W4_TRY(w4_hip(hipSetDevice(ctx->device), "hipSetDevice"));
+    return quant_rows(ctx, x_dev, x_type, ldx, t, k, q_dev, s_dev);
+}
+
+extern "C" int w4a16_norm_resid_q8(w4a16_ctx* ctx, uint64_t x_dev, uint64_t nw_dev, uint64_t ab_dev, uint64_t q_dev, uint64_t s_dev, size_t t,
+                                   size_t w_off, size_t hidden) {
+    if (!ctx || !x_dev || !nw_dev || !ab_dev || !q_dev || !s_dev) return w4_fail(W4A16_ERR_ARG, "norm_resid_q8: null operand");
+    if (hidden == 0 || hidden > 8192) return w4_fail(W4A16_ERR_SHAPE, "norm_resid_q8: hidden=%zu outside 1..8192", hidden);
+    if (w_off > 0x7fffffffu - hidden) return w4_fail(W4A16_ERR_SHAPE, "norm_resid_q8: w_off=%zu too large", w_off);
+    W4_TRY(check_rows("norm_resid_q8", t, hidden));
+    if (x_dev % 4 || nw_dev % 4 || ab_dev % 4 || s_dev % 4 || q_dev % 16)
+        return w4_fail(W4A16_ERR_ARG, "norm_resid_q8: f32 operands must be aligned to 4 bytes, q to 16");
+    W4_TRY(w4_hip(hipSetDevice(ctx->device), "hipSetDevice"));
+    int wo = (int)w_off, h = (int)hidden, kt = (int)k_tiles(hidden), r = (int)tile_rows(t);
+    void* params[] = {&x_dev, &nw_dev, &ab_dev, &q_dev, &s_dev, &wo, &h, &kt, &r};
+    return w4_launch(ctx, "w4a16_norm_resid_q8", (unsigned)t, 1, 1024, 0, params);
+}
+
+// ------------------------------------------------------------------------------------------------ registration
+static void free_w8(w4a16_ctx* ctx, W8Lin& L) {
+    (void)w4a16_free(ctx, L.q);
+    (void)w4a16_free(ctx, L.s);
+    L = W8Lin();
+}
+
+static float w4_f16_to_f32(uint16_t h) {
+    const float sign = h & 0x8000u ? -1.0f : 1.0f;
+    const int exp = (h >> 10) & 0x1f, frac = h & 0x3ff;
+    if (exp == 0x1f) return frac ? NAN : sign * INFINITY;
+    return sign * (exp ? std::ldexp((float)(1024 + frac), exp - 25) : std::ldexp((float)frac, -24));
+}
+
+static float scale_at(const void* s, int type, size_t i) {
+    uint32_t b = 0;
+    if (type == W4A16_F32) {
+        memcpy(&b, static_cast<const char*>(s) + i * 4, 4);
+    } else {
+        uint16_t h;
+        memcpy(&h, static_cast<const char*>(s) + i * 2, 2);
+        if (type == W4A16_F16) return w4_f16_to_f32(h);
+        b = (uint32_t)h << 16;
+    }
+    float v;
+    memcpy(&v, &b, 4);
+    return v;
+}
+
+extern "C" int w4a16_upload_lin_w8a8(w4a16_ctx* ctx, const char* name, const void* q, size_t qlen_bytes, const void* s, size_t slen_bytes, size_t n,
+                                     size_t k, int s_type) {
+    if (!ctx || !name || !q || !s) return w4_fail(W4A16_ERR_ARG, "upload_lin_w8a8: null argument");
+    if (!float_type(s_type)) return w4_fail(W4A16_ERR_ARG, "upload_lin_w8a8 %s: scale type %d (0 = f32, 1 = f16, 2 = bf16)", name, s_type);
+    if (n == 0 || n > 0x7fffff00u || k == 0 || k > kW4Q8MaxK || qlen_bytes != n * k || slen_bytes != n * type_bytes(s_type))
+        return w4_fail(W4A16_ERR_SHAPE, "upload_lin_w8a8 %s: q=%zu s=%zu bytes for n=%zu k=%zu (k up to %d)", name, qlen_bytes, slen_bytes, n, k,
+                       kW4Q8MaxK);
+    W4_TRY(w4_hip(hipSetDevice(ctx->device), "hipSetDevice"));
+    W8Lin L;
+    L.n = n;
+    L.k = k;
+    const size_t row_blocks = (n + 15) / 16, kt = k_tiles(k), chunks = row_blocks * kt * 64;
+    std::vector<float> scales(row_blocks * 16, 0.0f);
+    for (size_t i = 0; i < n; i++) scales[i] = scale_at(s, s_type, i);
+    uint64_t raw = 0;
+    int rc = w4a16_alloc(ctx, chunks * 16, &L.q);
+    if (!rc) rc = w4a16_alloc(ctx, scales.size() * 4, &L.s);
+    if (!rc) rc = w4a16_alloc(ctx, qlen_bytes, &raw);
+    if (!rc) rc = w4a16_h2d(ctx, raw, q, qlen_bytes);
+    if (!rc) rc = w4a16_h2d(ctx, L.s, scales.data(), scales.size() * 4);
+    if (!rc) {
+        size_t ns = n, cs = chunks;
+        int ki = (int)k, kti = (int)kt;
+        void* params[] = {&raw, &L.q, &ns, &ki, &kti, &cs};
+        rc = w4_launch(ctx, "w4a16_tile_w8", std::min<unsigned>(ceil_div(chunks, 256), 65536), 1, 256, 0, params);
+    }
+    if (!rc) rc = w4a16_sync(ctx);
+    const std::string keep = rc ? w4_err_save() : std::string();
+    (void)w4a16_free(ctx, raw);
+    if (rc) {
+        free_w8(ctx, L);
+        w4_err_restore(keep);
+        return rc;
+    }
+    auto it = ctx->w8lins.find(std::string_view(name));
+    if (it != ctx->w8lins.end()) {
+        free_w8(ctx, it->second);
+        ctx->scratch_gen++;  // graphs captured so far hold the old weights' address
+        it->second = L;
+    } else {
+        ctx->w8lins.emplace(name, L);
+    }
+    return 0;
+}
+
+static int find_w8(w4a16_ctx* ctx, const char* name, const W8Lin** out) {
+    if (!ctx || !name) return w4_fail(W4A16_ERR_ARG, "lin_w8a8: null argument");
+    auto it = ctx->w8lins.find(std::string_view(name));
+    if (it == ctx->w8lins.end()) return w4_fail(W4A16_ERR_NOT_FOUND, "lin_w8a8 %s: not registered", name);
+    *out = &it->second;
+    return 0;
+}
+
+extern "C" int w4a16_lin_w8a8_info(w4a16_ctx* ctx, const char* name, size_t* n, size_t* k) {
+    const W8Lin* L = nullptr;
+    W4_TRY(find_w8(ctx, name, &L));
+    if (n) *n = L->n;
+    if (k) *k = L->k;
+    return 0;
+}
+
+// ------------------------------------------------------------------------------------------------ forward
+static int launch_skinny(w4a16_ctx* ctx, const W8Lin& L, uint64_t q, uint64_t s, size_t t, uint64_t y, int y_type, int act) {
+    const bool glu = act >= 0;
+    const int tt = (int)((t + 15) / 16);
+    const size_t kt = k_tiles(L.k), blocks16 = (L.n + 15) / 16;
+    int rb = blocks16 >= 1024 ? (tt == 1 ? 2 : 4) : glu ? 2 : 1;
+    const size_t blocks = (blocks16 + rb - 1) / rb;
+    const size_t waves_max = std::min<size_t>(std::min<size_t>(rb == 1 ? 16 : 8, 64 / (size_t)(rb * tt)), std::max<size_t>(kt / 2, 1));
+    const size_t waves = std::max<size_t>(1, std::min(waves_max, std::max<size_t>(4, 4096 / blocks)));
+    char sym[64];
+    snprintf(sym, sizeof sym, "w4a16_w8a8_skinny_r%d_t%d%s", rb, tt, glu ? "_glu" : "");
+    uint64_t wt = L.q, ws = L.s;
+    int ni = (int)L.n, kti = (int)kt, ti = (int)t, r = (int)tile_rows(t), wi = (int)waves;
+    void* params[] = {&wt, &ws, &q, &s, &y, &ni, &kti, &ti, &r, &y_type, &act, &wi};
+    const unsigned grid = glu ? ceil_div(blocks16 / 2, rb / 2) : (unsigned)blocks;
+    return w4_launch(ctx, sym, grid, 1, (unsigned)waves * 64, waves > 1 ? (unsigned)(waves * rb * tt * 1024) : 0u, params);
+}
+
+static int launch_tiled(w4a16_ctx* ctx, const W8Lin& L, uint64_t q, uint64_t s, size_t t, uint64_t y, int y_type, int act) {
+    const bool glu = act >= 0;
+    const size_t bm = 128, tiles = (t + bm - 1) / bm * ((glu ? L.n / 2 + 127 : L.n + 255) / (glu ? 128 : 256));
+    if (tiles > 0x7ffffff0u) return w4_fail(W4A16_ERR_SHAPE, "lin_w8a8: t=%zu n=%zu exceed the grid", t, L.n);
+    uint64_t wt = L.q, ws = L.s;
+    int ni = (int)L.n, kti = (int)k_tiles(L.k), ti = (int)t;
+    void* params[] = {&wt, &ws, &q, &s, &y, &ni, &kti, &ti, &y_type, &act};
+    return w4_launch(ctx, glu ? "w4a16_w8a8_tiled_m128_glu" : "w4a16_w8a8_tiled_m128", (unsigned)((tiles + 7) / 8 * 8), 1, 256,
+                     (unsigned)(2 * bm * 128), params);
+}
+
+static int forward_w8a8(w4a16_ctx* ctx, const char* api, const char* name, uint64_t x, int x_type, size_t ldx, uint64_t xs, size_t t, uint64_t y,
+                        int y_type, int act) {
+    const W8Lin* L = nullptr;
+    W4_TRY(find_w8(ctx, name, &L));
+    if (!x || !y) return w4_fail(W4A16_ERR_ARG, "%s %s: null operand", api, name);
+    if (x_type != W4A16_Q8 && !float_type(x_type))
+        return w4_fail(W4A16_ERR_ARG, "%s %s: x type %d (0 = f32, 1 = f16, 2 = bf16, 3 = quantised rows)", api, name, x_type);
+    if (!float_type(y_type)) return w4_fail(W4A16_ERR_ARG, "%s %s: y type %d (0 = f32, 1 = f16, 2 = bf16)", api, name, y_type);
+    W4_TRY(check_rows(api, t, L->k));
+    if (x_type == W4A16_Q8 ? !xs || ldx != 0 : xs != 0)
+        return w4_fail(W4A16_ERR_ARG, "%s %s: quantised rows come with their scales and without a row stride, others without scales", api, name);
+    if (act >= 0 && L->n % 32 != 0)
+        return w4_fail(W4A16_ERR_SHAPE, "%s %s: n=%zu must be a multiple of 32 (gate and values of whole row blocks)", api, name, L->n);
+    if (x_type != W4A16_Q8) {
+        if (ldx == 0) ldx = L->k;
+        if (ldx < L->k) return w4_fail(W4A16_ERR_SHAPE, "%s %s: ldx=%zu below k=%zu", api, name, ldx, L->k);
+    }
+    if (y % type_bytes(y_type) || x % (x_type == W4A16_Q8 ? 16 : type_bytes(x_type)) || xs % 4)
+        return w4_fail(W4A16_ERR_ARG, "%s %s: operands must be aligned to their elements, quantised rows to 16 bytes", api, name);
+    W4_TRY(w4_hip(hipSetDevice(ctx->device), "hipSetDevice"));
+    if (x_type != W4A16_Q8) {
+        W4_TRY(w4_ensure(ctx, &ctx->q8, &ctx->q8_cap, w4a16_q8_bytes(t, L->k)));
+        W4_TRY(w4_ensure(ctx, &ctx->q8_scales, &ctx->q8_scales_cap, std::max<size_t>(t * 4, 256)));
+        W4_TRY(quant_rows(ctx, x, x_type, ldx, t, L->k, ctx->q8, ctx->q8_scales));
+        x = ctx->q8;
+        xs = ctx->q8_scales;
+    }
+    return t <= 64 ? launch_skinny(ctx, *L, x, xs, t, y, y_type, act) : launch_tiled(ctx, *L, x, xs, t, y, y_type, act);
+}
+
+extern "C" int w4a16_lin_forward_w8a8(w4a16_ctx* ctx, const char* name, uint64_t x_dev, int x_type, size_t ldx, uint64_t xs_dev, size_t t,
+                                      uint64_t y_dev, int y_type) {
+    return forward_w8a8(ctx, "lin_forward_w8a8", name, x_dev, x_type, ldx, xs_dev, t, y_dev, y_type, -1);
+}
+
+extern "C" int w4a16_lin_forward_w8a8_glu(w4a16_ctx* ctx, const char* name, uint64_t x_dev, int x_type, size_t ldx, uint64_t xs_dev, size_t t,
+                                          uint64_t y_dev, int y_type, int act) {
+    if (act != W4A16_ACT_SILU && act != W4A16_ACT_GELU_TANH)
+        return w4_fail(W4A16_ERR_ARG, "lin_forward_w8a8_glu %s: activation %d (0 = silu, 1 = gelu, tanh form)", name ? name : "", act);
+    return forward_w8a8(ctx, "lin_forward_w8a8_glu", name, x_dev, x_type, ldx, xs_dev, t, y_dev, y_type, act);
+}

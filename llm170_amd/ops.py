@@ -436,6 +436,44 @@ class W4a16Dec:
                                               warmup, reps, C.byref(ms), C.byref(wall)))
         return ms.value, wall.value
 
+    # ---- W8A8 linears: int8 weights with a scale per output channel, activations quantised per row
+    def upload_lin_w8a8(self, name, q, s, n, k):
+        """q int8 [n][k]; s [n]: float32, float16, or uint16 (bf16 bits)."""
+        q, s = np.ascontiguousarray(q), np.ascontiguousarray(s)
+        types = {"float32": ffi.F32, "float16": ffi.F16, "uint16": ffi.BF16}
+        if q.dtype != np.int8 or s.dtype.name not in types:
+            raise W4a16Error(ffi.ERR_ARG, "upload_lin_w8a8 %s: q %s, s %s (int8, and float32, float16 or uint16)" % (name, q.dtype, s.dtype))
+        ffi.check(self.cc.lib.w4a16_upload_lin_w8a8(self.cc.h, name.encode(), _ptr(q), q.nbytes, _ptr(s), s.nbytes, n, k, types[s.dtype.name]))
+
+    def lin_w8a8_spec(self, name):
+        n, k = C.c_size_t(), C.c_size_t()
+        ffi.check(self.cc.lib.w4a16_lin_w8a8_info(self.cc.h, name.encode(), C.byref(n), C.byref(k)))
+        return {"n": n.value, "k": k.value}
+
+    def quant_rows(self, x_dev, q_dev, s_dev, t, k, x_type=ffi.F16, ldx=0):
+        """q <- x in steps of s = max|row| / 127, in tiles (q8_bytes(t, k) bytes; unpack_q8 reads them back)."""
+        ffi.check(self.cc.lib.w4a16_quant_rows(self.cc.h, x_dev, x_type, ldx, t, k, q_dev, s_dev))
+
+    def norm_resid_q8(self, x_dev, nw_dev, ab_dev, q_dev, s_dev, t, hidden, w_off=0):
+        """norm_resid and quant_rows of its result in one launch: x <- x + ab; q, s <- the normalised rows."""
+        ffi.check(self.cc.lib.w4a16_norm_resid_q8(self.cc.h, x_dev, nw_dev, ab_dev, q_dev, s_dev, t, w_off, hidden))
+
+    def lin_forward_w8a8(self, name, x_dev, dst_dev, t, x_type=ffi.F16, ldx=0, xs_dev=0, y_type=ffi.F32):
+        """y [t][n]; x in rows of floats, quantised on the way, or x_type Q8: what quant_rows or norm_resid_q8 wrote for t rows."""
+        ffi.check(self.cc.lib.w4a16_lin_forward_w8a8(self.cc.h, name.encode(), x_dev, x_type, ldx, xs_dev, t, dst_dev, y_type))
+
+    def lin_forward_w8a8_glu(self, name, x_dev, dst_dev, t, x_type=ffi.F16, ldx=0, xs_dev=0, y_type=ffi.F16, gelu=False):
+        """act(gate) * up of a fused gate|up linear (rows 0..n/2 gate), y [t][n/2]."""
+        ffi.check(self.cc.lib.w4a16_lin_forward_w8a8_glu(self.cc.h, name.encode(), x_dev, x_type, ldx, xs_dev, t, dst_dev, y_type,
+                                                         ACT_GELU_TANH if gelu else ACT_SILU))
+
+    # ---- scoring of logits
+    def token_logprobs(self, logits_dev, t, n_vocab, logits_type=ffi.F32, ld=0, targets_dev=0, logp_dev=0, entropy_dev=0, top_k=0,
+                       top_idx_dev=0, top_logp_dev=0):
+        """Per row: the log probability of a given token (int32 target, negative: none), the entropy, the top_k most likely tokens."""
+        ffi.check(self.cc.lib.w4a16_token_logprobs(self.cc.h, logits_dev, logits_type, ld, t, n_vocab, targets_dev, logp_dev, entropy_dev,
+                                                   top_k, top_idx_dev, top_logp_dev))
+
     # ---- layer chain
     CHAIN_ROLES = ("attn_qkv", "attn_output", "ffn_gate_up", "ffn_down")
 
@@ -496,6 +534,18 @@ class W4a16Dec:
         ffi.check(self.cc.lib.w4a16_bench_chain(self.cc.h, prefix.encode(), n_layers, x_dev, t, y_dev, warmup, reps,
                                                 int(use_graph), int(fused), C.byref(ms), C.byref(wall)))
         return ms.value, wall.value
+
+
+def q8_bytes(t, k):
+    """Bytes of t quantised rows of k (0: no such rows)."""
+    return ffi.load().w4a16_q8_bytes(t, k)
+
+
+def unpack_q8(q, t, k):
+    """Rows int8 [t][k] from what quant_rows or norm_resid_q8 wrote (q: q8_bytes(t, k) bytes, on the host)."""
+    r = 1 if t == 1 else 4 if t <= 4 else 16
+    tiles = np.ascontiguousarray(q).reshape(-1).view(np.int8).reshape(-(-t // r), -(-k // 128) * 8, r, 16)
+    return tiles.transpose(0, 2, 1, 3).reshape(-(-t // r) * r, -1)[:t, :k].copy()
 
 
 def moe_topk(logits, top_k):
