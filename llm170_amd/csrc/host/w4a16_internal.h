@@ -139,7 +139,7 @@ constexpr int kW4PfKs = 128;                // PF_KS (prefill.hip): k per LDS st
 constexpr int kW4PfMoeIdsAt = 36864;        // PF_MOE_IDS_AT (prefill.hip): LDS bytes ahead of the grouped kernels' slot ids
 constexpr int kW4PfThreads = 256;           // PF_THREADS (prefill.hip)
 constexpr int kW4Q8MaxK = 131071;           // Q8_MAX_K (q8_common.hpp)
-constexpr int kW4ScoreStage = 1024;         // SCORE_STAGE (score.hip): elements of a wave's stage
+constexpr int kW4ScoreStageBytes = 4096;    // SCORE_STAGE_BYTES (score.hip): of a wave's stage, four waves to a workgroup
 constexpr int kW4ScoreMaxTop = 32;          // SCORE_MAX_TOP
 constexpr int kW4ScoreRecord = 272;         // SCORE_RECORD
 

@@ -3,11 +3,14 @@
 
 #include "w4a16_internal.h"
 
-// Workgroups per row: one where the rows fill the chip; with fewer rows a row is cut into segments of at least 4096 elements (one
-// stage of a workgroup's four waves), about four workgroups per CU.
-static size_t score_segments(size_t t, size_t vocab, size_t cus) {
-    const size_t most = (vocab + kW4ScoreStage * 4 - 1) / (kW4ScoreStage * 4), want = (4 * cus + t - 1) / t;
-    return std::max<size_t>(1, std::min(std::min(most, want), (size_t)256));
+// Workgroups per row.  One from 1024 rows on; with fewer a row is cut into segments of whole stages of a workgroup's four waves: about
+// 1024 workgroups, but no more than 16 per row, or as many as make 256 workgroups, up to 32 (the records of more cost more than the
+// shorter segments save).  us in 1 / 4 / 8 / 16 / 32 segments: 1 x 131072 bf16, 20 best, 35.5 / 21.4 / 16.9 / 14.6 / 14.7; 16 x
+// 131072 f32 49.1 / 25.7 / 20.0 / 18.2 / 21.1; 64 x 131072 bf16 41.4 / 23.9 / 20.9 / 20.7 / -; 256 x 131072 f16 39.2 / 31.6 / 36.8 / 49.0;
+// 600 x 100003 f16, 5 best, 41.5 / 50.3 / 48.2 / 64.7; 1000 x 32000 bf16 28.5 / 54.0.
+static size_t score_segments(size_t t, size_t vocab, size_t cus, size_t stage) {
+    const size_t most = (vocab + stage - 1) / stage, few = std::max(cus / t, std::min<size_t>(4 * cus / t, 16));
+    return std::max<size_t>(1, std::min({most, few, (size_t)32}));
 }
 
 extern "C" int w4a16_token_logprobs(w4a16_ctx* ctx, uint64_t logits_dev, int logits_type, size_t ld, size_t t, size_t n_vocab,
@@ -29,7 +32,8 @@ extern "C" int w4a16_token_logprobs(w4a16_ctx* ctx, uint64_t logits_dev, int log
     if (logits_dev % (logits_type == W4A16_F32 ? 4 : 2) || (targets_dev | logp_dev | entropy_dev | top_idx_dev | top_logp_dev) % 4)
         return w4_fail(W4A16_ERR_ARG, "token_logprobs: operands must be aligned to their elements");
     W4_TRY(w4_hip(hipSetDevice(ctx->device), "hipSetDevice"));
-    const size_t want = score_segments(t, n_vocab, (size_t)std::max(ctx->cu_count, 1)), stage = kW4ScoreStage * 4;
+    const size_t stage = kW4ScoreStageBytes * 4 / (logits_type == W4A16_F32 ? 4 : 2);
+    const size_t want = score_segments(t, n_vocab, (size_t)std::max(ctx->cu_count, 1), stage);
     const size_t seg_len = ((n_vocab + want - 1) / want + stage - 1) / stage * stage, segs = (n_vocab + seg_len - 1) / seg_len;
     if (segs > 1) {
         W4_TRY(w4_ensure(ctx, &ctx->score_ws, &ctx->score_ws_cap, t * segs * kW4ScoreRecord));
