@@ -112,7 +112,8 @@ static const char* const kMoeSyms[] = {W4_MOE_FAMILY("w4a16_moe_g32_f16"),
                                        "w4a16_moe_topk_sum_f16",
                                        nullptr};
 
-static const char* const kQuantSyms[] = {"w4a16_quant_rows_f32", "w4a16_quant_rows_f16", "w4a16_quant_rows_bf16", "w4a16_norm_resid_q8", "w4a16_tile_w8",
+static const char* const kQuantSyms[] = {"w4a16_quant_rows_f32", "w4a16_quant_rows_f16", "w4a16_quant_rows_bf16", "w4a16_quant_few_f32",
+                                         "w4a16_quant_few_f16", "w4a16_quant_few_bf16", "w4a16_norm_resid_q8", "w4a16_tile_w8",
                                          nullptr};
 // row blocks per workgroup and token tiles; gated builds (kernels/w8a8.hip)
 #define W8_TT(P, S) P "_t1" S, P "_t2" S, P "_t3" S, P "_t4" S

@@ -92,6 +92,8 @@ struct w4a16_ctx {
     std::map<std::string, W8Lin, std::less<>> w8lins;
     uint64_t q8 = 0, q8_scales = 0;  // quantised rows of a W8A8 linear that was given rows of floats
     size_t q8_cap = 0, q8_scales_cap = 0;
+    uint64_t w8_part = 0, w8_tickets = 0;  // sums of the k slices of a W8A8 launch, one ticket per workgroup of a slice
+    size_t w8_part_cap = 0, w8_tickets_cap = 0;
     uint64_t score_ws = 0, score_tickets = 0;  // records of the segments of a row of logits, one ticket per row
     size_t score_ws_cap = 0, score_tickets_cap = 0;
     W4MoeScratch moe;

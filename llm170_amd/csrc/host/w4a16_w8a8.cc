@@ -31,15 +31,15 @@ extern "C" size_t w4a16_q8_bytes(size_t t, size_t k) {
 
 static int quant_rows(w4a16_ctx* ctx, uint64_t x, int x_type, size_t ldx, size_t t, size_t k, uint64_t q, uint64_t s) {
     char sym[64];
-    snprintf(sym, sizeof sym, "w4a16_quant_rows_%s", type_name(x_type));
-    const size_t chunks = (k + 15) / 16;
+    // Few rows: a thread per four columns; else one per sixteen
+    const bool few = t <= 16;
+    snprintf(sym, sizeof sym, "w4a16_quant_%s_%s", few ? "few" : "rows", type_name(x_type));
     const int r = (int)tile_rows(t);
-    // as many threads as a row has chunks, up to four waves; few rows take up to sixteen
-    const unsigned block = (unsigned)std::min<size_t>((chunks + 63) / 64 * 64, t <= 64 ? 1024 : 256);
-    const unsigned grid = r == 16 ? ceil_div(t, 128) * 128 : (unsigned)t;
+    const unsigned block = (unsigned)std::min<size_t>(few ? (k + 255) / 256 * 64 : (k + 1023) / 1024 * 64, 1024);
+    const unsigned grid = few ? (unsigned)t : ceil_div(t, 128) * 128;
     int ki = (int)k, kt = (int)k_tiles(k), ri = r, ti = (int)t, bi = (int)block;
     void* params[] = {&x, &ldx, &ki, &kt, &ri, &q, &s, &ti, &bi};
-    return w4_launch(ctx, sym, grid, 1, block, 0, params);
+    return w4_launch(ctx, sym, grid, few ? ceil_div(k, block * 4) : 1, block, 0, params);
 }
 
 extern "C" int w4a16_quant_rows(w4a16_ctx* ctx, uint64_t x_dev, int x_type, size_t ldx, size_t t, size_t k, uint64_t q_dev, uint64_t s_dev) {
@@ -159,21 +159,61 @@ extern "C" int w4a16_lin_w8a8_info(w4a16_ctx* ctx, const char* name, size_t* n, 
 }
 
 // ------------------------------------------------------------------------------------------------ forward
-static int launch_skinny(w4a16_ctx* ctx, const W8Lin& L, uint64_t q, uint64_t s, size_t t, uint64_t y, int y_type, int act) {
+// Launch of the kernel for up to 64 rows: row blocks per workgroup, waves, k slices; a function of the shape alone.
+struct SkinnyPlan {
+    int rb = 1, waves = 8, nks = 1;
+    double price = 0.0;
+};
+
+static SkinnyPlan plan_skinny(size_t n, size_t k, size_t t, size_t cus, bool glu) {
+    const size_t kt = k_tiles(k), blocks16 = (n + 15) / 16;
+    const int tt = (int)((t + 15) / 16);
+    SkinnyPlan best;
+    best.price = 1e30;
+    for (int rb = 4; rb >= (glu ? 2 : 1); rb /= 2) {
+        for (int nks = 1; nks <= 8; nks++) {
+            const size_t blocks = (blocks16 + rb - 1) / rb, grid = blocks * nks;
+            if (nks > 1 && ((size_t)nks * 8 > kt || grid > 4 * cus)) break;
+            const double run = (double)kt / nks;
+            // Price in us, fitted to 3000 launches of 19 shapes (n 512 .. 65536, k 1024 .. 17408) at 1 .. 64 rows, cold weights: what it
+            // picks is 1.7 % slower in the mean than the best of them.  A CU takes 50 KiB per us of weights and half of the activations'
+            // (from the L2); workgroups over those that all CUs have cost nearly a whole one; slices cost a hand-over and their sums' way
+            // through memory.  5120 x 17408 at t = 16: one row block, whole k 23.9 us, four and three slices 17.7; 7168 x 5120 at t = 64:
+            // 17.5, two row blocks 12.7.
+            const size_t full = grid / cus, rest = grid % cus;
+            const double rounds = (double)full + (rest == 0 ? 0.0 : full == 0 ? 1.0 : 0.94 + 0.06 * (double)rest / (double)cus);
+            const double load = run * (rb + 0.48 * (t <= 4 ? 0.25 : tt));
+            SkinnyPlan p;
+            p.rb = rb;
+            p.nks = nks;
+            // four waves where a CU has several workgroups and eight would have few k tiles each or hold many sums, or k is short
+            p.waves = (grid > cus && (run <= 40 || rb * tt >= 16)) || run <= 16 ? 4 : 8;
+            p.waves = (int)std::min<size_t>(p.waves, kt);
+            p.price = std::max(rounds * load / 49.6, (double)(blocks16 * kt) / 9079.0) + (nks > 1 ? 2.07 + 0.24e-6 * nks * n * t * 8 : 0.0);
+            if (p.price < best.price) best = p;
+        }
+    }
+    return best;
+}
+
+static int launch_skinny(w4a16_ctx* ctx, const W8Lin& L, const SkinnyPlan& P, uint64_t q, uint64_t s, size_t t, uint64_t y, int y_type, int act) {
     const bool glu = act >= 0;
     const int tt = (int)((t + 15) / 16);
     const size_t kt = k_tiles(L.k), blocks16 = (L.n + 15) / 16;
-    int rb = blocks16 >= 1024 ? (tt == 1 ? 2 : 4) : glu ? 2 : 1;
-    const size_t blocks = (blocks16 + rb - 1) / rb;
-    const size_t waves_max = std::min<size_t>(std::min<size_t>(rb == 1 ? 16 : 8, 64 / (size_t)(rb * tt)), std::max<size_t>(kt / 2, 1));
-    const size_t waves = std::max<size_t>(1, std::min(waves_max, std::max<size_t>(4, 4096 / blocks)));
     char sym[64];
-    snprintf(sym, sizeof sym, "w4a16_w8a8_skinny_r%d_t%d%s", rb, tt, glu ? "_glu" : "");
-    uint64_t wt = L.q, ws = L.s;
-    int ni = (int)L.n, kti = (int)kt, ti = (int)t, r = (int)tile_rows(t), wi = (int)waves;
-    void* params[] = {&wt, &ws, &q, &s, &y, &ni, &kti, &ti, &r, &y_type, &act, &wi};
-    const unsigned grid = glu ? ceil_div(blocks16 / 2, rb / 2) : (unsigned)blocks;
-    return w4_launch(ctx, sym, grid, 1, (unsigned)waves * 64, waves > 1 ? (unsigned)(waves * rb * tt * 1024) : 0u, params);
+    snprintf(sym, sizeof sym, "w4a16_w8a8_skinny_r%d_t%d%s", P.rb, tt, glu ? "_glu" : "");
+    const unsigned grid = glu ? ceil_div(blocks16 / 2, P.rb / 2) : ceil_div(blocks16, P.rb);
+    if (P.nks > 1) {
+        W4_TRY(w4_ensure(ctx, &ctx->w8_part, &ctx->w8_part_cap, (size_t)grid * P.nks * P.rb * tt * 1024));
+        if ((size_t)grid * 4 > ctx->w8_tickets_cap) {
+            W4_TRY(w4_ensure(ctx, &ctx->w8_tickets, &ctx->w8_tickets_cap, std::max<size_t>((size_t)grid * 4, 16384)));
+            W4_TRY(w4a16_memset0(ctx, ctx->w8_tickets, ctx->w8_tickets_cap));
+        }
+    }
+    uint64_t wt = L.q, ws = L.s, part = ctx->w8_part, tickets = ctx->w8_tickets;
+    int ni = (int)L.n, kti = (int)kt, ti = (int)t, r = (int)tile_rows(t), wi = P.waves, ksi = P.nks;
+    void* params[] = {&wt, &ws, &q, &s, &y, &ni, &kti, &ti, &r, &y_type, &act, &wi, &ksi, &part, &tickets};
+    return w4_launch(ctx, sym, grid, (unsigned)P.nks, (unsigned)P.waves * 64, 0, params);
 }
 
 static int launch_tiled(w4a16_ctx* ctx, const W8Lin& L, uint64_t q, uint64_t s, size_t t, uint64_t y, int y_type, int act) {
@@ -214,7 +254,8 @@ static int forward_w8a8(w4a16_ctx* ctx, const char* api, const char* name, uint6
         x = ctx->q8;
         xs = ctx->q8_scales;
     }
-    return t <= 64 ? launch_skinny(ctx, *L, x, xs, t, y, y_type, act) : launch_tiled(ctx, *L, x, xs, t, y, y_type, act);
+    if (t <= 64) return launch_skinny(ctx, *L, plan_skinny(L->n, L->k, t, (size_t)std::max(ctx->cu_count, 1), act >= 0), x, xs, t, y, y_type, act);
+    return launch_tiled(ctx, *L, x, xs, t, y, y_type, act);
 }
 
 extern "C" int w4a16_lin_forward_w8a8(w4a16_ctx* ctx, const char* name, uint64_t x_dev, int x_type, size_t ldx, uint64_t xs_dev, size_t t,

@@ -105,6 +105,46 @@ __device__ __forceinline__ int q8_round(float x, float s, float r) {
 
 __device__ __forceinline__ float q8_recip(float s) { return s > 0.f ? 1.0f / s : 0.f; }  // NaN > 0 is false
 
+// N values of a row quantised, byte e of the result is value e's (two's complement).  x * r + 128 is off by less than 2^-15: r and the sum
+// are rounded once each, |x * r| <= 127.  Only where it lies within 1/20000 of a half (for sixteen values a lane one wave in ten) q8_round is asked.
+template <int N>
+__device__ __forceinline__ void q8_pack(const float (&w)[N], float step, float r, unsigned (&out)[N / 4]) {
+    float far = 0.f, q[N];
+#pragma unroll
+    for (int e = 0; e < N; e++) {
+        const float p = __builtin_fmaf(w[e], r, 128.0f);
+        q[e] = __builtin_rintf(p);
+        far = __builtin_fmaxf(far, __builtin_fabsf(p - q[e]));
+    }
+#pragma unroll
+    for (int i = 0; i < N / 4; i++) {
+        unsigned b = 0;
+#pragma unroll
+        for (int e = 0; e < 4; e++) b = __builtin_amdgcn_cvt_pk_u8_f32(q[4 * i + e], e, b);
+        out[i] = r == 0.f ? 0u : b ^ 0x80808080u;  // r = 0: nothing but zeros
+    }
+    if (__any(far > 0.49995f)) {
+#pragma unroll
+        for (int i = 0; i < N / 4; i++) {
+            unsigned b = 0;
+#pragma unroll
+            for (int e = 0; e < 4; e++) b |= ((unsigned)q8_round(w[4 * i + e], step, r) & 0xffu) << (8 * e);
+            out[i] = b;
+        }
+    }
+}
+
+// Largest of one value per lane: rows of 16 by shifts, then across the rows, to lane 63
+__device__ __forceinline__ unsigned q8_wave_max(unsigned v) {
+    v = max(v, (unsigned)__builtin_amdgcn_update_dpp((int)v, (int)v, 0x111, 0xf, 0xf, false));
+    v = max(v, (unsigned)__builtin_amdgcn_update_dpp((int)v, (int)v, 0x112, 0xf, 0xf, false));
+    v = max(v, (unsigned)__builtin_amdgcn_update_dpp((int)v, (int)v, 0x114, 0xf, 0xf, false));
+    v = max(v, (unsigned)__builtin_amdgcn_update_dpp((int)v, (int)v, 0x118, 0xf, 0xf, false));
+    v = max(v, (unsigned)__builtin_amdgcn_update_dpp((int)v, (int)v, 0x142, 0xa, 0xf, false));
+    v = max(v, (unsigned)__builtin_amdgcn_update_dpp((int)v, (int)v, 0x143, 0xc, 0xf, false));
+    return (unsigned)__builtin_amdgcn_readlane((int)v, 63);
+}
+
 // Byte offset of chunk (row, 16 k from kc * 16) in a buffer of quantised rows with kt k tiles, tiles of R rows
 __device__ __forceinline__ size_t q8_chunk_at(int row, int kc, int kt, int R) {
     return ((((size_t)(row / R) * kt + (kc >> 2)) * 4 + (kc & 3)) * R + row % R) * 16;

@@ -72,15 +72,6 @@ __device__ __forceinline__ float score_wave_max(float v) {  // NaN where a lane 
     v = __builtin_elementwise_maximum(v, score_dpp<0x143, 0xc>(v, v));
     return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
 }
-__device__ __forceinline__ unsigned score_wave_max_u32(unsigned v) {
-    v = max(v, (unsigned)__builtin_amdgcn_update_dpp((int)v, (int)v, 0x111, 0xf, 0xf, false));
-    v = max(v, (unsigned)__builtin_amdgcn_update_dpp((int)v, (int)v, 0x112, 0xf, 0xf, false));
-    v = max(v, (unsigned)__builtin_amdgcn_update_dpp((int)v, (int)v, 0x114, 0xf, 0xf, false));
-    v = max(v, (unsigned)__builtin_amdgcn_update_dpp((int)v, (int)v, 0x118, 0xf, 0xf, false));
-    v = max(v, (unsigned)__builtin_amdgcn_update_dpp((int)v, (int)v, 0x142, 0xa, 0xf, false));
-    v = max(v, (unsigned)__builtin_amdgcn_update_dpp((int)v, (int)v, 0x143, 0xc, 0xf, false));
-    return (unsigned)__builtin_amdgcn_readlane((int)v, 63);
-}
 __device__ __forceinline__ ScoreStats score_wave_join(ScoreStats a) {
     ScoreStats o;
     o.m = score_wave_max(a.m);
@@ -149,7 +140,7 @@ struct ScoreTop {
 // An image that `want` lanes at least, and not many more, reach with theirs: between the largest and the smallest by halves.
 __device__ __forceinline__ unsigned score_reach(float best, int want) {
     const unsigned o = score_order(best);
-    unsigned hi = score_wave_max_u32(o), lo = ~score_wave_max_u32(~o);
+    unsigned hi = q8_wave_max(o), lo = ~q8_wave_max(~o);
     if (__popcll(__ballot(o >= hi)) >= want) return hi;
 #pragma unroll 1
     while (hi - lo > 1) {

@@ -36,14 +36,20 @@ __device__ __forceinline__ void w8_store4(void* __restrict__ y, size_t at, int l
 }
 
 // ------------------------------------------------------------------------------------------------ up to 64 rows
-// The weight stream bounds these launches.  A workgroup's waves take consecutive runs of k of the same RB row blocks (16 outputs
-// each); the weights arrive as whole tiles straight in registers, DEPTH of them in flight per row block, meet TT tiles of 16
-// activation rows (from the L2), and the waves' sums are added through LDS: whole numbers, so in any order the same.
+// The weight stream bounds these launches.  A workgroup's waves take consecutive runs of a k slice of the same RB row blocks (16
+// outputs each); the weights arrive as whole tiles straight in registers, DEPTH of them in flight per row block, meet TT tiles of 16
+// activation rows (from the L2), and the waves' sums are added in LDS: whole numbers, so in any order the same.  Where there are too
+// few row blocks for the chip, slices of k go to several workgroups (gridDim.y of them): each leaves its sums in the workspace and
+// draws a ticket of its row blocks, the last one adds them.
+typedef unsigned long long w8_pair_t;
+
 template <int RB, int TT, bool GLU>
 __device__ __forceinline__ void skinny_body(const char* __restrict__ wt, const float* __restrict__ ws, const char* __restrict__ xq,
-                                            const float* __restrict__ xs, void* __restrict__ y, int n, int kt, int t, int R, int y_type, int act, int W) {
-    extern __shared__ char lds[];
-    constexpr int DEPTH = RB * TT == 1 ? 8 : RB + TT <= 4 ? 4 : RB + TT <= 6 ? 3 : 2;
+                                            const float* __restrict__ xs, void* __restrict__ y, int n, int kt, int t, int R, int y_type, int act, int W,
+                                            int nks, w8_pair_t* __restrict__ part, int* __restrict__ tickets) {
+    constexpr int DEPTH = RB * TT == 1 ? 8 : RB + TT <= 4 ? 4 : RB + TT <= 6 ? 3 : 2, TILES = RB * TT;
+    __shared__ int sums[TILES][4][64];
+    __shared__ int last_one;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int row_blocks = (n + 15) >> 4, half_rb = GLU ? row_blocks >> 1 : 0;
     // row block of slot i: gated, slots 2j and 2j + 1 are a gate's and its values'
@@ -62,7 +68,8 @@ __device__ __forceinline__ void skinny_body(const char* __restrict__ wt, const f
     const char* const xp = xq + ((size_t)kg * R + tok % R) * 16;
     const size_t x_tile = (size_t)R * 64, x_block = x_tile * kt;
 
-    const int lo = (int)((long long)kt * wave / W), hi = (int)((long long)kt * (wave + 1) / W);
+    const int runs = nks * W, run = blockIdx.y * W + wave;
+    const int lo = (int)((long long)kt * run / runs), hi = (int)((long long)kt * (run + 1) / runs);
     i4_t acc[RB][TT];
 #pragma unroll
     for (int i = 0; i < RB; i++)
@@ -70,15 +77,18 @@ __device__ __forceinline__ void skinny_body(const char* __restrict__ wt, const f
         for (int j = 0; j < TT; j++) acc[i][j] = (i4_t){0, 0, 0, 0};
     i4_t wv[DEPTH][RB], xv[DEPTH][TT];
     auto load = [&](int d, int k) {
-        const int kc = min(k, kt - 1);  // in bounds; loads past the run are not used
 #pragma unroll
-        for (int i = 0; i < RB; i++) wv[d][i] = __builtin_nontemporal_load(reinterpret_cast<const i4_t*>(wp[i] + (size_t)kc * 1024));
+        for (int i = 0; i < RB; i++) wv[d][i] = __builtin_nontemporal_load(reinterpret_cast<const i4_t*>(wp[i] + (size_t)k * 1024));
 #pragma unroll
-        for (int j = 0; j < TT; j++) xv[d][j] = *reinterpret_cast<const i4_t*>(xp + j * x_block + kc * x_tile);
+        for (int j = 0; j < TT; j++) xv[d][j] = *reinterpret_cast<const i4_t*>(xp + j * x_block + k * x_tile);
     };
 #pragma unroll
     for (int d = 0; d < DEPTH; d++)
         if (lo + d < hi) load(d, lo + d);
+    if (W > 1) {
+        for (int i = threadIdx.x; i < TILES * 256; i += W * 64) (&sums[0][0][0])[i] = 0;
+        __syncthreads();
+    }
     for (int k = lo; k < hi; k += DEPTH) {
 #pragma unroll
         for (int d = 0; d < DEPTH; d++) {
@@ -91,30 +101,63 @@ __device__ __forceinline__ void skinny_body(const char* __restrict__ wt, const f
             }
         }
     }
-    // [wave][slot][token tile] partial tiles; a wave finishes every W-th unit (gated: a gate and its values)
-    i4_t* const part = reinterpret_cast<i4_t*>(lds);
     if (W > 1) {
 #pragma unroll
         for (int i = 0; i < RB; i++)
 #pragma unroll
-            for (int j = 0; j < TT; j++) part[((wave * RB + i) * TT + j) * 64 + lane] = acc[i][j];
+            for (int j = 0; j < TT; j++)
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    __hip_atomic_fetch_add(&sums[i * TT + j][e][lane], acc[i][j][e], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
         __syncthreads();
     }
+    // A wave finishes every W-th tile (gated: a gate and its values)
+    auto total = [&](int tile) {
+        i4_t v;
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[e] = sums[tile][e][lane];
+        return v;
+    };
     constexpr int U = GLU ? RB / 2 : RB;
+    const size_t slice = (size_t)gridDim.x * (TILES * 128);  // pairs of sums per k slice
+    w8_pair_t* const mine = part + (size_t)blockIdx.x * (TILES * 128) + lane;
+    if (nks > 1) {
+        // Device-scope stores, complete before the ticket is drawn; device-scope loads behind the barrier that follows the ticket's return.
+        // Neither is served from a cache that is not coherent.
+#pragma unroll
+        for (int u = 0; u < TILES; u++) {
+            if (u % W != wave || (u % TT) * 16 + tok >= t) continue;
+            const i4_t v = W > 1 ? total(u) : acc[u / TT][u % TT];
+            w8_pair_t* const p = mine + blockIdx.y * slice + u * 128;
+            __hip_atomic_store(p, (w8_pair_t)(unsigned)v[1] << 32 | (unsigned)v[0], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            __hip_atomic_store(p + 64, (w8_pair_t)(unsigned)v[3] << 32 | (unsigned)v[2], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        if (threadIdx.x == 0) last_one = __hip_atomic_fetch_add(tickets + blockIdx.x, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == nks - 1;
+        __syncthreads();
+        if (!last_one) return;
+        if (threadIdx.x == 0) __hip_atomic_store(tickets + blockIdx.x, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);  // for the next launch
+    }
 #pragma unroll
     for (int u = 0; u < U * TT; u++) {
         if (u % W != wave) continue;  // uniform for the wave
         const int i = GLU ? u / TT * 2 : u / TT, j = u % TT;
-        auto total = [&](int i_) {
-            if (W == 1) return acc[i_][j];
-            i4_t v = part[(i_ * TT + j) * 64 + lane];
-            for (int w = 1; w < W; w++) v += part[((w * RB + i_) * TT + j) * 64 + lane];
+        const int b = block_of(i), m = j * 16 + tok, c = b * 16 + kg * 4;
+        if (b > last || m >= t) continue;
+        auto sum_of = [&](int i_) {
+            if (nks == 1) return W > 1 ? total(i_ * TT + j) : acc[i_][j];
+            i4_t v = {0, 0, 0, 0};
+            const w8_pair_t* p = mine + (i_ * TT + j) * 128;
+#pragma unroll 4
+            for (int s = 0; s < nks; s++, p += slice) {
+                const w8_pair_t a = __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                const w8_pair_t d = __hip_atomic_load(p + 64, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                v += (i4_t){(int)a, (int)(a >> 32), (int)d, (int)(d >> 32)};
+            }
             return v;
         };
-        const int b = block_of(i);
-        const i4_t sum = total(i), sum_up = GLU ? total(i + 1) : sum;
-        const int m = j * 16 + tok, c = b * 16 + kg * 4;
-        if (b > last || m >= t) continue;
+        const i4_t sum = sum_of(i), sum_up = GLU ? sum_of(i + 1) : sum;
         const float sx = xs[m];
         float v[4];
 #pragma unroll
@@ -129,29 +172,20 @@ __device__ __forceinline__ void skinny_body(const char* __restrict__ wt, const f
 
 #define W8_SKINNY(NAME, RB, TT, GLU, THREADS)                                                                                     \
     extern "C" __global__ __launch_bounds__(THREADS) void NAME(const char* wt, const float* ws, const char* xq, const float* xs, void* y, int n, \
-                                                               int kt, int t, int R, int y_type, int act, int waves) {            \
-        skinny_body<RB, TT, GLU>(wt, ws, xq, xs, y, n, kt, t, R, y_type, act, waves);                                                    \
+                                                               int kt, int t, int R, int y_type, int act, int waves, int nks, w8_pair_t* part,   \
+                                                               int* tickets) {                                                    \
+        skinny_body<RB, TT, GLU>(wt, ws, xq, xs, y, n, kt, t, R, y_type, act, waves, nks, part, tickets);                         \
     }
-W8_SKINNY(w4a16_w8a8_skinny_r1_t1, 1, 1, false, 1024)
-W8_SKINNY(w4a16_w8a8_skinny_r2_t1, 2, 1, false, 512)
-W8_SKINNY(w4a16_w8a8_skinny_r1_t2, 1, 2, false, 1024)
-W8_SKINNY(w4a16_w8a8_skinny_r2_t2, 2, 2, false, 512)
-W8_SKINNY(w4a16_w8a8_skinny_r1_t3, 1, 3, false, 1024)
-W8_SKINNY(w4a16_w8a8_skinny_r2_t3, 2, 3, false, 512)
-W8_SKINNY(w4a16_w8a8_skinny_r1_t4, 1, 4, false, 1024)
-W8_SKINNY(w4a16_w8a8_skinny_r2_t4, 2, 4, false, 512)
-W8_SKINNY(w4a16_w8a8_skinny_r4_t1, 4, 1, false, 512)
-W8_SKINNY(w4a16_w8a8_skinny_r4_t2, 4, 2, false, 512)
-W8_SKINNY(w4a16_w8a8_skinny_r4_t3, 4, 3, false, 512)
-W8_SKINNY(w4a16_w8a8_skinny_r4_t4, 4, 4, false, 512)
-W8_SKINNY(w4a16_w8a8_skinny_r2_t1_glu, 2, 1, true, 512)
-W8_SKINNY(w4a16_w8a8_skinny_r2_t2_glu, 2, 2, true, 512)
-W8_SKINNY(w4a16_w8a8_skinny_r2_t3_glu, 2, 3, true, 512)
-W8_SKINNY(w4a16_w8a8_skinny_r2_t4_glu, 2, 4, true, 512)
-W8_SKINNY(w4a16_w8a8_skinny_r4_t1_glu, 4, 1, true, 512)
-W8_SKINNY(w4a16_w8a8_skinny_r4_t2_glu, 4, 2, true, 512)
-W8_SKINNY(w4a16_w8a8_skinny_r4_t3_glu, 4, 3, true, 512)
-W8_SKINNY(w4a16_w8a8_skinny_r4_t4_glu, 4, 4, true, 512)
+#define W8_SKINNY_T(NAME, RB, GLU, SUFFIX)                \
+    W8_SKINNY(NAME##_t1##SUFFIX, RB, 1, GLU, 512)         \
+    W8_SKINNY(NAME##_t2##SUFFIX, RB, 2, GLU, 512)         \
+    W8_SKINNY(NAME##_t3##SUFFIX, RB, 3, GLU, 512)         \
+    W8_SKINNY(NAME##_t4##SUFFIX, RB, 4, GLU, 512)
+W8_SKINNY_T(w4a16_w8a8_skinny_r1, 1, false, )
+W8_SKINNY_T(w4a16_w8a8_skinny_r2, 2, false, )
+W8_SKINNY_T(w4a16_w8a8_skinny_r4, 4, false, )
+W8_SKINNY_T(w4a16_w8a8_skinny_r2, 2, true, _glu)
+W8_SKINNY_T(w4a16_w8a8_skinny_r4, 4, true, _glu)
 
 // ------------------------------------------------------------------------------------------------ tiles, any number of rows
 // Block tile 32 MI rows x 256 columns, four waves along n, wave tile 32 MI x 64 on v_mfma_i32_32x32x32_i8.  Activations go
