@@ -196,6 +196,15 @@ static SkinnyPlan plan_skinny(size_t n, size_t k, size_t t, size_t cus, bool glu
     return best;
 }
 
+static int split_workspace(w4a16_ctx* ctx, size_t part_bytes, size_t tickets) {
+    W4_TRY(w4_ensure(ctx, &ctx->w8_part, &ctx->w8_part_cap, part_bytes));
+    if (tickets * 4 > ctx->w8_tickets_cap) {
+        W4_TRY(w4_ensure(ctx, &ctx->w8_tickets, &ctx->w8_tickets_cap, std::max<size_t>(tickets * 4, 16384)));
+        W4_TRY(w4a16_memset0(ctx, ctx->w8_tickets, ctx->w8_tickets_cap));
+    }
+    return 0;
+}
+
 static int launch_skinny(w4a16_ctx* ctx, const W8Lin& L, const SkinnyPlan& P, uint64_t q, uint64_t s, size_t t, uint64_t y, int y_type, int act) {
     const bool glu = act >= 0;
     const int tt = (int)((t + 15) / 16);
@@ -203,28 +212,57 @@ static int launch_skinny(w4a16_ctx* ctx, const W8Lin& L, const SkinnyPlan& P, ui
     char sym[64];
     snprintf(sym, sizeof sym, "w4a16_w8a8_skinny_r%d_t%d%s", P.rb, tt, glu ? "_glu" : "");
     const unsigned grid = glu ? ceil_div(blocks16 / 2, P.rb / 2) : ceil_div(blocks16, P.rb);
-    if (P.nks > 1) {
-        W4_TRY(w4_ensure(ctx, &ctx->w8_part, &ctx->w8_part_cap, (size_t)grid * P.nks * P.rb * tt * 1024));
-        if ((size_t)grid * 4 > ctx->w8_tickets_cap) {
-            W4_TRY(w4_ensure(ctx, &ctx->w8_tickets, &ctx->w8_tickets_cap, std::max<size_t>((size_t)grid * 4, 16384)));
-            W4_TRY(w4a16_memset0(ctx, ctx->w8_tickets, ctx->w8_tickets_cap));
-        }
-    }
+    if (P.nks > 1) W4_TRY(split_workspace(ctx, (size_t)grid * P.nks * P.rb * tt * 1024, grid));
     uint64_t wt = L.q, ws = L.s, part = ctx->w8_part, tickets = ctx->w8_tickets;
     int ni = (int)L.n, kti = (int)kt, ti = (int)t, r = (int)tile_rows(t), wi = P.waves, ksi = P.nks;
     void* params[] = {&wt, &ws, &q, &s, &y, &ni, &kti, &ti, &r, &y_type, &act, &wi, &ksi, &part, &tickets};
     return w4_launch(ctx, sym, grid, (unsigned)P.nks, (unsigned)P.waves * 64, 0, params);
 }
 
-static int launch_tiled(w4a16_ctx* ctx, const W8Lin& L, uint64_t q, uint64_t s, size_t t, uint64_t y, int y_type, int act) {
+// Launch of the tiled kernel: 64 or 128 rows per tile, k slices; a function of the shape alone.
+struct TiledPlan {
+    int bm = 64, nks = 1;
+    double price = 0.0;
+};
+
+static TiledPlan plan_tiled(size_t n, size_t k, size_t t, size_t cus, bool glu) {
+    const size_t kt = k_tiles(k), tiles_n = glu ? (n / 2 + 127) / 128 : (n + 255) / 256;
+    TiledPlan best;
+    best.price = 1e30;
+    for (int bm = 64; bm <= 128; bm *= 2) {
+        for (int nks = 1; nks <= 8; nks++) {
+            const size_t grid = (t + bm - 1) / bm * tiles_n * nks;
+            if (nks > 1 && ((size_t)nks * 8 > kt || grid > 2 * cus)) break;
+            // Price in us, fitted to 300 launches of 7 shapes (n 1000 .. 34816, k 2048 .. 17408) at 65 .. 4096 rows, cold weights: what it
+            // picks is 0.6 % slower in the mean than the best of them.  A k tile takes a workgroup 0.27 us (64 rows) or 0.44 us (128) alone
+            // on its CU, twice that where the CU has two of them; a round over that costs between its share and a whole one; slices cost
+            // their sums' way through memory.  5120 x 17408 at t = 300: 128 rows, whole k 113 us, four slices 53; t = 100: 64 rows, whole k
+            // 73 us, six slices 34; 22016 x 4096 gated at t = 1000: 64 rows 127 us, 128 rows 109.
+            const double alone = bm == 64 ? 0.27 : 0.44, pair = bm == 64 ? 0.54 : 0.83;
+            const double load = (double)grid / (double)cus, rounds = load / 2.0;
+            const double per_k = load <= 1.0 ? alone : rounds <= 1.0 ? pair : pair * (0.6 * std::ceil(rounds) + 0.4 * rounds);
+            TiledPlan p;
+            p.bm = bm;
+            p.nks = nks;
+            p.price = (double)((kt + nks - 1) / nks) * per_k + (nks > 1 ? (1.2 * nks + 10.0 * load) * bm / 128.0 : 0.0);
+            if (p.price < best.price) best = p;
+        }
+    }
+    return best;
+}
+
+static int launch_tiled(w4a16_ctx* ctx, const W8Lin& L, const TiledPlan& P, uint64_t q, uint64_t s, size_t t, uint64_t y, int y_type, int act) {
     const bool glu = act >= 0;
-    const size_t bm = 128, tiles = (t + bm - 1) / bm * ((glu ? L.n / 2 + 127 : L.n + 255) / (glu ? 128 : 256));
-    if (tiles > 0x7ffffff0u) return w4_fail(W4A16_ERR_SHAPE, "lin_w8a8: t=%zu n=%zu exceed the grid", t, L.n);
-    uint64_t wt = L.q, ws = L.s;
-    int ni = (int)L.n, kti = (int)k_tiles(L.k), ti = (int)t;
-    void* params[] = {&wt, &ws, &q, &s, &y, &ni, &kti, &ti, &y_type, &act};
-    return w4_launch(ctx, glu ? "w4a16_w8a8_tiled_m128_glu" : "w4a16_w8a8_tiled_m128", (unsigned)((tiles + 7) / 8 * 8), 1, 256,
-                     (unsigned)(2 * bm * 128), params);
+    const size_t tiles = (t + P.bm - 1) / P.bm * (glu ? (L.n / 2 + 127) / 128 : (L.n + 255) / 256), nks = (size_t)P.nks;
+    if (tiles * nks > 0x7ffffff0u) return w4_fail(W4A16_ERR_SHAPE, "lin_w8a8: t=%zu n=%zu exceed the grid", t, L.n);
+    if (nks > 1) W4_TRY(split_workspace(ctx, tiles * nks * P.bm * 1024, tiles));
+    uint64_t wt = L.q, ws = L.s, part = ctx->w8_part, tickets = ctx->w8_tickets;
+    // 1024 rows of tiles share their weights in the L2: 34816 x 5120 gated at t = 4096 666 us, 512 rows 679, 256 rows 727
+    int ni = (int)L.n, kti = (int)k_tiles(L.k), ti = (int)t, ki = P.nks, band = 1024 / P.bm;
+    char sym[64];
+    snprintf(sym, sizeof sym, "w4a16_w8a8_tiled_m%d%s", P.bm, glu ? "_glu" : "");
+    void* params[] = {&wt, &ws, &q, &s, &y, &ni, &kti, &ti, &y_type, &act, &ki, &band, &part, &tickets};
+    return w4_launch(ctx, sym, (unsigned)((tiles * nks + 7) / 8 * 8), 1, 256, 0, params);
 }
 
 static int forward_w8a8(w4a16_ctx* ctx, const char* api, const char* name, uint64_t x, int x_type, size_t ldx, uint64_t xs, size_t t, uint64_t y,
@@ -254,8 +292,9 @@ static int forward_w8a8(w4a16_ctx* ctx, const char* api, const char* name, uint6
         x = ctx->q8;
         xs = ctx->q8_scales;
     }
-    if (t <= 64) return launch_skinny(ctx, *L, plan_skinny(L->n, L->k, t, (size_t)std::max(ctx->cu_count, 1), act >= 0), x, xs, t, y, y_type, act);
-    return launch_tiled(ctx, *L, x, xs, t, y, y_type, act);
+    const size_t cus = (size_t)std::max(ctx->cu_count, 1);
+    if (t <= 64) return launch_skinny(ctx, *L, plan_skinny(L->n, L->k, t, cus, act >= 0), x, xs, t, y, y_type, act);
+    return launch_tiled(ctx, *L, plan_tiled(L->n, L->k, t, cus, act >= 0), x, xs, t, y, y_type, act);
 }
 
 extern "C" int w4a16_lin_forward_w8a8(w4a16_ctx* ctx, const char* name, uint64_t x_dev, int x_type, size_t ldx, uint64_t xs_dev, size_t t,

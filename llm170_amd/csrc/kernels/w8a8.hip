@@ -188,128 +188,174 @@ W8_SKINNY_T(w4a16_w8a8_skinny_r2, 2, true, _glu)
 W8_SKINNY_T(w4a16_w8a8_skinny_r4, 4, true, _glu)
 
 // ------------------------------------------------------------------------------------------------ tiles, any number of rows
-// Block tile 32 MI rows x 256 columns, four waves along n, wave tile 32 MI x 64 on v_mfma_i32_32x32x32_i8.  Activations go
-// through LDS by DMA, 128 k a stage, two stages; weights straight into registers, a stage ahead.
-#define W8_KS 128
-template <int MI, bool GLU>
+// Block tile BM = 64 or 128 rows x 256 columns, four waves along n, wave tile BM x 64 on v_mfma_i32_16x16x64_i8 (the 32 x 32 x 32 form
+// keeps up 3.3 POP/s on random bytes, this one 4.1).  Weights go straight into registers, activations through registers into LDS, a k tile
+// of 64 at a time, both asked for AHEAD k tiles ahead: a line's first reader of an XCD waits up to 2 us for it.  Nothing waits for the
+// newest loads: a k tile's barrier orders LDS alone, and with three LDS buffers the next tile's first blocks are read ahead of it.  (LDS
+// DMA, whose barriers have to wait for every load of the wave, kept 128 k in flight and let them run dry: 34816 x 5120 gated t = 4096
+// 672 us, this 650, 2.25 POP/s of int8.)  There the matrix units are busy half the time, at 2.0 GHz; with every load hitting the L1
+// 500 us: the L1's 24 KiB per k tile, the four waves' common step and the L2 share the rest.
+// nks > 1: slices of k go to several workgroups, which hand their sums over as those of the kernels above do.
+__device__ __forceinline__ void w8_lds_done() { __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local"); }  // global loads stay in flight
+__device__ __forceinline__ void w8_lds_barrier() {  // behind w8_lds_done
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
+template <int BM, int AHEAD, int XRING, bool GLU>
 __device__ __forceinline__ void tiled_body(const char* __restrict__ wt, const float* __restrict__ ws, const char* __restrict__ xq,
-                                           const float* __restrict__ xs, void* __restrict__ y, int n, int kt, int t, int y_type, int act) {
-    extern __shared__ char lds[];
-    constexpr int BM = 32 * MI, STAGE = BM * W8_KS, NA = STAGE / 4096;  // DMA loads per wave and stage
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int nl = lane & 31, kh = lane >> 5;
+                                           const float* __restrict__ xs, void* __restrict__ y, int n, int kt, int t, int y_type, int act, int nks,
+                                           int band, w8_pair_t* __restrict__ part, int* __restrict__ tickets) {
+    constexpr int J = BM / 16, XL = J / 4, WAVES = 4, PERIOD = XRING == AHEAD ? AHEAD * (AHEAD + 1) : AHEAD + 1;
+    static_assert(BM % 64 == 0 && PERIOD % 3 == 0 && (XRING == AHEAD || XRING == AHEAD + 1), "rings and the three buffers fit the period");
+    __shared__ __attribute__((aligned(1024))) char lds[3][BM * 64];  // a k tile of activations: [row block] of 1 KiB
+    __shared__ int last_one;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wn = wave;
+    const int tok = lane & 15, kg = lane >> 4;
     const int out_n = GLU ? n >> 1 : n, half_rb = GLU ? n >> 5 : 0, row_blocks = (n + 15) >> 4;
     constexpr int BN = GLU ? 128 : 256;
-    // Block tiles: every XCD takes a consecutive eighth of them, bands of eight tile rows, in a band m fastest
+    // Block tiles: every XCD takes a consecutive eighth of them (and of their slices), bands of `band` tile rows, in a band m fastest
     const int tiles_m = (t + BM - 1) / BM, tiles_n = (out_n + BN - 1) / BN;
-    const unsigned work = (unsigned)tiles_m * (unsigned)tiles_n, xcd = blockIdx.x & 7;
+    const unsigned work = (unsigned)tiles_m * (unsigned)tiles_n * (unsigned)nks, xcd = blockIdx.x & 7;
     const unsigned at = (unsigned)((unsigned long long)work * xcd / 8) + (blockIdx.x >> 3);
     if (at >= (unsigned)((unsigned long long)work * (xcd + 1) / 8)) return;
-    const unsigned band = at / (8u * tiles_n), in_band = at - band * 8u * tiles_n;
-    const unsigned rows = min(8u, (unsigned)tiles_m - band * 8u);
-    const int tn = (int)(in_band / rows), tm = (int)(band * 8u + in_band - tn * rows);
+    const unsigned tile = at / (unsigned)nks, slice = at - tile * (unsigned)nks;
+    const unsigned per_band = (unsigned)band * tiles_n, b_at = tile / per_band, in_band = tile - b_at * per_band;
+    const unsigned rows = min((unsigned)band, (unsigned)tiles_m - b_at * band);
+    const int tn = (int)(in_band / rows), tm = (int)(b_at * band + in_band - tn * rows);
     const int m0 = tm * BM, n0 = tn * BN;
 
     const int x_blocks = (t + 15) >> 4;
     const __amdgpu_buffer_rsrc_t xr = w4_make_rsrc(xq + (size_t)(m0 >> 4) * kt * 1024, (unsigned)min(x_blocks - (m0 >> 4), BM / 16) * (unsigned)kt * 1024u);
     // first row block of the wave's columns and what is left of the matrix behind it
-    const int wrb = (n0 >> 4) + wave * (GLU ? 2 : 4), w_end = GLU ? half_rb : row_blocks;
+    const int wrb = (n0 >> 4) + wn * (GLU ? 2 : 4), w_end = GLU ? half_rb : row_blocks;
     auto w_rsrc = [&](int first, int count) {
-        return w4_make_rsrc(wt + (size_t)(count > 0 ? first : 0) * kt * 1024, (unsigned)max(count, 0) * (unsigned)kt * 1024u);
+        first = __builtin_amdgcn_readfirstlane(count > 0 ? first : 0);  // uniform, and known to be
+        count = __builtin_amdgcn_readfirstlane(max(count, 0));
+        return w4_make_rsrc(wt + (size_t)(unsigned)first * (unsigned)kt * 1024, (unsigned)count * (unsigned)kt * 1024u);
     };
     const __amdgpu_buffer_rsrc_t wr0 = w_rsrc(wrb, min(w_end - wrb, GLU ? 2 : 4)),
                                  wr1 = GLU ? w_rsrc(half_rb + wrb, min(w_end - wrb, 2)) : wr0;
-    typedef __attribute__((address_space(3))) char lds_char_t;
-    lds_char_t* const lds_base = (lds_char_t*)lds;
-    // stage in LDS: [row block][two k tiles] of 1 KiB
-    unsigned xa[NA];
+    // row block slot i of the wave: gated, slots 0 and 1 are the gate's, 2 and 3 its values'
+    unsigned wo[4], xo[XL];
 #pragma unroll
-    for (int i = 0; i < NA; i++) {
-        const int tile = i * 4 + wave;
-        xa[i] = (unsigned)(tile >> 1) * (unsigned)kt * 1024u + (tile & 1) * 1024u + lane * 16u;
-    }
-    auto load_x = [&](int s, int buf) {
+    for (int i = 0; i < 4; i++) wo[i] = (unsigned)(GLU ? i & 1 : i) * (unsigned)kt * 1024u + lane * 16u;
 #pragma unroll
-        for (int i = 0; i < NA; i++)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(xr, (__attribute__((address_space(3))) void*)(lds_base + buf * STAGE + (i * 4 + wave) * 1024), 16,
-                                                     xa[i], s * 2048, 0, 0);
+    for (int i = 0; i < XL; i++) xo[i] = (unsigned)(wave + 4 * i) * (unsigned)kt * 1024u + lane * 16u;
+    const int from = (int)((long long)kt * slice / nks), to = (int)((long long)kt * (slice + 1) / nks);
+    i4_t w[AHEAD + 1][4], x[XRING][XL], a[4];  // k tiles i .. i + AHEAD of the weights, i + 2 .. i + AHEAD + 1 of the activations
+    auto load_w = [&](i4_t (&d)[4], int k) {
+        const int at = min(k, to - 1) * 1024;  // behind the end the last tile again, not used
+#pragma unroll
+        for (int i = 0; i < 4; i++) d[i] = __builtin_bit_cast(i4_t, __builtin_amdgcn_raw_buffer_load_b128(GLU && i >= 2 ? wr1 : wr0, wo[i], at, 0));
     };
-    unsigned wo[2];
+    auto load_x = [&](i4_t (&d)[XL], int k) {
+        const int at = min(k, to - 1) * 1024;
 #pragma unroll
-    for (int ni = 0; ni < 2; ni++)
-        wo[ni] = (unsigned)((GLU ? 0 : ni * 2) + (nl >> 4)) * (unsigned)kt * 1024u + kh * 256u + (nl & 15) * 16u;
-    i4_t b[2][2][4];
-    auto load_w = [&](i4_t (&d)[2][4], int s) {
-#pragma unroll
-        for (int ni = 0; ni < 2; ni++)
-#pragma unroll
-            for (int q = 0; q < 4; q++)
-                d[ni][q] = __builtin_bit_cast(i4_t, __builtin_amdgcn_raw_buffer_load_b128(ni ? wr1 : wr0, wo[ni] + q * 512, s * 2048, 0));
+        for (int i = 0; i < XL; i++) d[i] = __builtin_bit_cast(i4_t, __builtin_amdgcn_raw_buffer_load_b128(xr, xo[i], at, 0));
     };
-    i16_t acc[MI][2];
+    auto put_x = [&](const i4_t (&s)[XL], int buf) {
 #pragma unroll
-    for (int mi = 0; mi < MI; mi++)
+        for (int i = 0; i < XL; i++) *reinterpret_cast<i4_t*>(lds[buf] + (wave + 4 * i) * 1024 + lane * 16) = s[i];
+    };
+    auto get_x = [&](int buf, int j) { return *reinterpret_cast<const i4_t*>(lds[buf] + j * 1024 + lane * 16); };
+    i4_t acc[J][4];
 #pragma unroll
-        for (int ni = 0; ni < 2; ni++)
+    for (int j = 0; j < J; j++)
 #pragma unroll
-            for (int e = 0; e < 16; e++) acc[mi][ni][e] = 0;
-    const char* const frag = lds + ((nl >> 4) * 2048 + kh * 256 + (nl & 15) * 16);
-    auto products = [&](const i4_t (&w)[2][4], int buf) {
+        for (int i = 0; i < 4; i++) acc[j][i] = (i4_t){0, 0, 0, 0};
+    if (from < to) {
+        i4_t first[XL];
+        load_x(first, from);
 #pragma unroll
-        for (int q = 0; q < 4; q++) {
-            i4_t a[MI];
-#pragma unroll
-            for (int mi = 0; mi < MI; mi++) a[mi] = *reinterpret_cast<const i4_t*>(frag + buf * STAGE + mi * 4096 + q * 512);
-#pragma unroll
-            for (int ni = 0; ni < 2; ni++)
-#pragma unroll
-                for (int mi = 0; mi < MI; mi++) acc[mi][ni] = __builtin_amdgcn_mfma_i32_32x32x32_i8(w[ni][q], a[mi], acc[mi][ni], 0, 0, 0);
+        for (int u = 0; u < AHEAD; u++) {
+            load_x(x[(u + 1) % XRING], from + u + 1);
+            load_w(w[u], from + u);
+            __builtin_amdgcn_sched_barrier(0);  // in the order of the loop, whose waits count them
         }
-    };
-    const int stages = kt >> 1;
-    load_x(0, 0);
-    load_w(b[0], 0);
-    w4_dma_barrier();
-    for (int s = 0; s < stages; s += 2) {
+        put_x(first, 0);
+        put_x(x[1], 1);
+        w8_lds_done();
+        w8_lds_barrier();
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-            if (s + h < stages) {
-                if (s + h + 1 < stages) {
-                    load_x(s + h + 1, h ^ 1);  // the buffer that stage s + h - 1 was read from: every wave is past its barrier
-                    load_w(b[h ^ 1], s + h + 1);
+        for (int j = 0; j < 4; j++) a[j] = get_x(0, j);
+        // Leaving from the middle, not skipping steps: the compiler's waits count the loads of every way that leads to a step
+        for (int k = from;; k += PERIOD) {
+#pragma unroll
+            for (int u = 0; u < PERIOD; u++) {
+                // k tile k + u from lds[u % 3], its first blocks in a; x holds tiles k + u + 2 .. k + u + AHEAD
+                load_x(x[(u + AHEAD + 1) % XRING], k + u + AHEAD + 1);
+                load_w(w[(u + AHEAD) % (AHEAD + 1)], k + u + AHEAD);
+#pragma unroll
+                for (int j = 0; j < J; j++) {
+                    __builtin_amdgcn_sched_barrier(0);
+                    if (j == J / 2 - (J == 4 ? 2 : 1)) put_x(x[(u + 2) % XRING], (u + 2) % 3);  // read last a tile ago, which the barrier since then ends
+#pragma unroll
+                    for (int i = 0; i < 4; i++) acc[j][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[u % (AHEAD + 1)][i], a[j & 3], acc[j][i], 0, 0, 0);
+                    __builtin_amdgcn_sched_barrier(0);
+                    if (j == J - 4) w8_lds_done();
+                    a[j & 3] = j < J - 4 ? get_x(u % 3, j + 4) : get_x((u + 1) % 3, j + 4 - J);  // written a tile ago: there behind the last barrier
                 }
-                products(b[h], h);
-                w4_dma_barrier();
+                w8_lds_barrier();
+                if (k + u + 1 >= to) goto summed;
             }
         }
     }
-    // D register e of lane (nl, kh): output column 8 (e / 4) + 4 kh + e % 4, row nl
+summed:
+    if (nks > 1) {
+        // [tile][slice][wave][block of 16 x 16][64 lanes] of 16 bytes, at device scope: past this XCD's L2
+        constexpr int DEVICE = 16;  // sc1
+        constexpr unsigned MINE = J * 4 * 1024;
+        char* const base = reinterpret_cast<char*>(part) + (size_t)tile * nks * WAVES * MINE;
+        const __amdgpu_buffer_rsrc_t pr = w4_make_rsrc(base, (unsigned)nks * WAVES * MINE);
 #pragma unroll
-    for (int mi = 0; mi < MI; mi++) {
-        const int m = m0 + mi * 32 + nl;
+        for (int j = 0; j < J; j++)
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4_t, acc[j][i]), pr, lane * 16, ((int)slice * WAVES + wave) * (int)MINE + (j * 4 + i) * 1024, DEVICE);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        if (threadIdx.x == 0) last_one = __hip_atomic_fetch_add(tickets + tile, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == nks - 1;
+        __syncthreads();
+        if (!last_one) return;
+        if (threadIdx.x == 0) __hip_atomic_store(tickets + tile, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);  // for the next launch
+        for (int o = 0; o < nks; o++) {
+            if (o == (int)slice) continue;
+#pragma unroll
+            for (int j = 0; j < J; j++)
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    acc[j][i] += __builtin_bit_cast(i4_t, __builtin_amdgcn_raw_buffer_load_b128(pr, lane * 16, (o * WAVES + wave) * (int)MINE + (j * 4 + i) * 1024, DEVICE));
+        }
+    }
+    // D register e of lane (tok, kg): output column 4 kg + e of its row block, row tok
+#pragma unroll
+    for (int j = 0; j < J; j++) {
+        const int m = m0 + j * 16 + tok;
         if (m >= t) continue;
         const float sx = xs[m];
 #pragma unroll
-        for (int ni = 0; ni < (GLU ? 1 : 2); ni++)
+        for (int i = 0; i < (GLU ? 2 : 4); i++) {
+            const int c = (wrb + i) * 16 + kg * 4;
+            if (c >= out_n) continue;
+            float v[4];
 #pragma unroll
-            for (int g = 0; g < 4; g++) {
-                const int c = n0 + wave * (GLU ? 32 : 64) + ni * 32 + g * 8 + kh * 4;
-                if (c >= out_n) continue;
-                float v[4];
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    v[e] = (float)acc[mi][ni][g * 4 + e] * sx * ws[c + e];
-                    if (GLU) v[e] = w4_act_mul(v[e], (float)acc[mi][1][g * 4 + e] * sx * ws[out_n + c + e], act);
-                }
-                w8_store4(y, (size_t)m * out_n + c, out_n - c, v, y_type);
+            for (int e = 0; e < 4; e++) {
+                v[e] = (float)acc[j][i][e] * sx * ws[c + e];
+                if (GLU) v[e] = w4_act_mul(v[e], (float)acc[j][i + 2][e] * sx * ws[out_n + c + e], act);
             }
+            w8_store4(y, (size_t)m * out_n + c, out_n - c, v, y_type);
+        }
     }
 }
 
-#define W8_TILED(NAME, MI, GLU)                                                                                                   \
+#define W8_TILED(NAME, BM, AHEAD, XRING, GLU)                                                                                     \
     extern "C" __global__ __launch_bounds__(256, 2) void NAME(const char* wt, const float* ws, const char* xq, const float* xs, void* y, int n, \
-                                                           int kt, int t, int y_type, int act) {                                  \
-        tiled_body<MI, GLU>(wt, ws, xq, xs, y, n, kt, t, y_type, act);                                                            \
+                                                              int kt, int t, int y_type, int act, int nks, int band, w8_pair_t* part,  \
+                                                              int* tickets) {                                                     \
+        tiled_body<BM, AHEAD, XRING, GLU>(wt, ws, xq, xs, y, n, kt, t, y_type, act, nks, band, part, tickets);                    \
     }
-W8_TILED(w4a16_w8a8_tiled_m128, 4, false)
-W8_TILED(w4a16_w8a8_tiled_m128_glu, 4, true)
+W8_TILED(w4a16_w8a8_tiled_m128, 128, 3, 3, false)
+W8_TILED(w4a16_w8a8_tiled_m128_glu, 128, 3, 3, true)
+W8_TILED(w4a16_w8a8_tiled_m64, 64, 5, 6, false)
+W8_TILED(w4a16_w8a8_tiled_m64_glu, 64, 5, 6, true)

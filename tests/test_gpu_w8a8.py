@@ -147,7 +147,9 @@ def test_norm_resid_q8_of_infinity(dec):
 
 SHAPES = [(1, 16, 64), (1, 1, 1), (1, 4096, 4096), (1, 16500, 640), (2, 33, 130), (3, 100, 77), (4, 512, 2048), (5, 48, 63), (7, 17, 4000), (16, 512, 17408),
           (16, 16400, 256), (17, 40, 300), (31, 1000, 1024), (33, 16401, 192), (37, 5003, 2051), (48, 64, 65), (49, 256, 512), (64, 16416, 320), (64, 700, 1500),
-          (65, 256, 128), (65, 1, 1), (100, 513, 1000), (128, 256, 384), (129, 300, 64), (300, 520, 2051), (1000, 257, 129), (513, 4100, 640), (2049, 1030, 256)]
+          (65, 256, 128), (65, 1, 1), (100, 513, 1000), (128, 256, 384), (129, 300, 64), (300, 520, 2051), (1000, 257, 129), (513, 4100, 640), (2049, 1030, 256),
+          # k in two to eight slices, under both tile heights, and the higher tile alone
+          (65, 256, 1000), (70, 300, 2048), (129, 1000, 2048), (66, 300, 17408), (100, 700, 12000), (257, 5, 8000), (200, 10000, 8000), (400, 10000, 128)]
 
 
 @pytest.mark.parametrize("t,n,k", SHAPES)
@@ -234,7 +236,7 @@ def test_rows_with_no_number_stay_alone(dec, t):
 
 @pytest.mark.parametrize("gelu", [False, True])
 @pytest.mark.parametrize("t,n,k", [(1, 32, 64), (1, 34816, 256), (2, 96, 200), (4, 22016, 128), (16, 1056, 777), (17, 64, 64), (33, 33000 // 32 * 32, 128), (48, 320, 100),
-                                   (64, 2080, 640), (65, 32, 64), (70, 544, 333), (257, 1088, 512)])
+                                   (64, 2080, 640), (65, 32, 64), (70, 544, 333), (257, 1088, 512), (70, 800, 9000), (140, 2080, 4100), (450, 9984, 128)])
 def test_gated_is_the_linear_and_its_activation(dec, t, n, k, gelu):
     say("glu", t, n, k, gelu)
     w, sb, sv = ref.weights(n + k, n, k)
@@ -378,6 +380,56 @@ def test_captured_ffn_replays_the_eager_bits(dec):
                 dec.lin_forward_w8a8("ffn.down", a, small, 1, x_type=ffi.F16, y_type=ffi.F32)  # another call through the same scratch
                 cc.sync()
             graph.destroy()
+
+
+@pytest.mark.parametrize("t,n,k,gelu", [(16, 1024, 8000, None), (60, 640, 4096, False), (70, 512, 4096, None), (130, 2048, 8192, True), (200, 10000, 8000, None)])
+def test_captured_slices_of_k_replay_the_eager_bits(dec, t, n, k, gelu):
+    """Slices hand their sums over through scratch and tickets that every call of the context shares: graphs and eager calls in turn."""
+    cc = dec.cc
+    w, sb, sv = ref.weights(n + k, n, k)
+    dec.upload_lin_w8a8("big", w, sb, n, k)
+    w2, sb2, sv2 = ref.weights(5, 256, 6000)
+    dec.upload_lin_w8a8("other", w2, sb2, 256, 6000)
+    r = np.random.default_rng(t)
+    xs = [r.standard_normal((t, k)).astype(np.float32) for _ in range(3)]
+    x2 = r.standard_normal((80, 6000)).astype(np.float32)
+    out = n if gelu is None else n // 2
+    with ref.Buffers(cc) as b:
+        dx, y, dx2, y2 = b.put(xs[0]), b.filled(t * out * 4), b.put(x2), b.filled(80 * 256 * 4)
+
+        def step():
+            if gelu is None:
+                dec.lin_forward_w8a8("big", dx, y, t, x_type=ffi.F32, y_type=ffi.F32)
+            else:
+                dec.lin_forward_w8a8_glu("big", dx, y, t, x_type=ffi.F32, y_type=ffi.F32, gelu=gelu)
+
+        def other():
+            dec.lin_forward_w8a8("other", dx2, y2, 80, x_type=ffi.F32, y_type=ffi.F32)
+
+        step()
+        other()
+        cc.capture_begin()
+        step()
+        first = cc.capture_end()
+        cc.capture_begin()
+        other()
+        step()
+        second = cc.capture_end()
+        want2 = ref.product(*ref.quantised(x2), w2, sv2)
+        for x in xs:
+            cc.h2d(dx, x)
+            step()
+            eager = cc.d2h(y, (t, out), np.float32)
+            if gelu is None:
+                assert np.array_equal(eager, ref.product(*ref.quantised(x), w, sv))
+            for graph in (first, second, first):
+                cc.h2d(y, np.zeros((t, out), np.float32))
+                graph.launch()
+                assert np.array_equal(cc.d2h(y, (t, out), np.float32), eager)
+                other()
+                assert np.array_equal(cc.d2h(y2, (80, 256), np.float32), want2)
+        first.destroy()
+        second.destroy()
 
 
 def test_a_capture_that_would_grow_the_scratch_is_refused():
