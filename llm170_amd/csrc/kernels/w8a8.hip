@@ -4,8 +4,9 @@
 #include "q8_common.hpp"
 
 // y[at .. at + 3] (those below `left`) as f32, f16 or bf16
-__device__ __forceinline__ void w8_store4(void* __restrict__ y, size_t at, int left, const float (&v)[4], int y_type) {
-    if (y_type == Q8_F32) {
+template <int T>
+__device__ __forceinline__ void w8_store4(void* __restrict__ y, size_t at, int left, const float (&v)[4]) {
+    if (T == Q8_F32) {
         float* const p = static_cast<float*>(y) + at;
         if (left >= 4) {
             u4_any_t o;
@@ -21,7 +22,7 @@ __device__ __forceinline__ void w8_store4(void* __restrict__ y, size_t at, int l
     }
     unsigned h[4];
 #pragma unroll
-    for (int i = 0; i < 4; i++) h[i] = y_type == Q8_F16 ? q8_to_16<Q8_F16>(v[i]) : q8_to_16<Q8_BF16>(v[i]);
+    for (int i = 0; i < 4; i++) h[i] = q8_to_16<T>(v[i]);
     uint16_t* const p = static_cast<uint16_t*>(y) + at;
     if (left >= 4) {
         u2_any_t o;
@@ -33,6 +34,11 @@ __device__ __forceinline__ void w8_store4(void* __restrict__ y, size_t at, int l
         for (int i = 0; i < 4; i++)
             if (i < left) p[i] = (uint16_t)h[i];
     }
+}
+__device__ __forceinline__ void w8_store4(void* __restrict__ y, size_t at, int left, const float (&v)[4], int y_type) {
+    if (y_type == Q8_F32) w8_store4<Q8_F32>(y, at, left, v);
+    else if (y_type == Q8_F16) w8_store4<Q8_F16>(y, at, left, v);
+    else w8_store4<Q8_BF16>(y, at, left, v);
 }
 
 // ------------------------------------------------------------------------------------------------ up to 64 rows
@@ -196,6 +202,10 @@ W8_SKINNY_T(w4a16_w8a8_skinny_r4, 4, true, _glu)
 // 672 us, this 650, 2.25 POP/s of int8.)  There the matrix units are busy half the time, at 2.0 GHz; with every load hitting the L1
 // 500 us: the L1's 24 KiB per k tile, the four waves' common step and the L2 share the rest.
 // nks > 1: slices of k go to several workgroups, which hand their sums over as those of the kernels above do.
+template <int T>
+struct w8_type {
+    static constexpr int value = T;
+};
 __device__ __forceinline__ void w8_lds_done() { __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local"); }  // global loads stay in flight
 __device__ __forceinline__ void w8_lds_barrier() {  // behind w8_lds_done
     __builtin_amdgcn_s_barrier();
@@ -209,6 +219,7 @@ __device__ __forceinline__ void tiled_body(const char* __restrict__ wt, const fl
     constexpr int J = BM / 16, XL = J / 4, WAVES = 4, PERIOD = XRING == AHEAD ? AHEAD * (AHEAD + 1) : AHEAD + 1;
     static_assert(BM % 64 == 0 && PERIOD % 3 == 0 && (XRING == AHEAD || XRING == AHEAD + 1), "rings and the three buffers fit the period");
     __shared__ __attribute__((aligned(1024))) char lds[3][BM * 64];  // a k tile of activations: [row block] of 1 KiB
+    __shared__ __attribute__((aligned(16))) float w_scale[256], x_scale[BM];
     __shared__ int last_one;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wn = wave;
     const int tok = lane & 15, kg = lane >> 4;
@@ -266,6 +277,9 @@ __device__ __forceinline__ void tiled_body(const char* __restrict__ wt, const fl
         for (int i = 0; i < 4; i++) acc[j][i] = (i4_t){0, 0, 0, 0};
     if (from < to) {
         i4_t first[XL];
+        // the tile's scales, for its end: gated, 128 of the gate and 128 of its values
+        const int c = n0 + (int)(GLU ? threadIdx.x & 127 : threadIdx.x), m = m0 + (int)threadIdx.x;
+        const float cs = c < out_n ? ws[GLU && threadIdx.x >= 128 ? out_n + c : c] : 0.f, ms = threadIdx.x < BM && m < t ? xs[m] : 0.f;
         load_x(first, from);
 #pragma unroll
         for (int u = 0; u < AHEAD; u++) {
@@ -273,6 +287,8 @@ __device__ __forceinline__ void tiled_body(const char* __restrict__ wt, const fl
             load_w(w[u], from + u);
             __builtin_amdgcn_sched_barrier(0);  // in the order of the loop, whose waits count them
         }
+        w_scale[threadIdx.x] = cs;
+        if (threadIdx.x < BM) x_scale[threadIdx.x] = ms;
         put_x(first, 0);
         put_x(x[1], 1);
         w8_lds_done();
@@ -329,24 +345,34 @@ summed:
         }
     }
     // D register e of lane (tok, kg): output column 4 kg + e of its row block, row tok
+    constexpr int OUT = GLU ? 2 : 4;
+    f4_t col[4];
 #pragma unroll
-    for (int j = 0; j < J; j++) {
-        const int m = m0 + j * 16 + tok;
-        if (m >= t) continue;
-        const float sx = xs[m];
+    for (int i = 0; i < 4; i++) col[i] = *reinterpret_cast<const f4_t*>(&w_scale[(GLU ? (i >> 1) * 128 + wave * 32 + (i & 1) * 16 : wave * 64 + i * 16) + kg * 4]);
+    const int c0 = wrb * 16 + kg * 4;
+    auto store = [&](auto type) {
+        constexpr int T = decltype(type)::value;
 #pragma unroll
-        for (int i = 0; i < (GLU ? 2 : 4); i++) {
-            const int c = (wrb + i) * 16 + kg * 4;
-            if (c >= out_n) continue;
-            float v[4];
+        for (int j = 0; j < J; j++) {
+            const int m = m0 + j * 16 + tok;
+            const float sx = x_scale[j * 16 + tok];
+            const size_t at = (size_t)m * out_n + c0;
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                v[e] = (float)acc[j][i][e] * sx * ws[c + e];
-                if (GLU) v[e] = w4_act_mul(v[e], (float)acc[j][i + 2][e] * sx * ws[out_n + c + e], act);
+            for (int i = 0; i < OUT; i++) {
+                float v[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    v[e] = (float)acc[j][i][e] * sx * col[i][e];
+                    if (GLU) v[e] = w4_act_mul(v[e], (float)acc[j][i + 2][e] * sx * col[i + 2][e], act);
+                }
+                if (m < t && c0 + i * 16 < out_n) w8_store4<T>(y, at + i * 16, out_n - c0 - i * 16, v);
             }
-            w8_store4(y, (size_t)m * out_n + c, out_n - c, v, y_type);
         }
-    }
+    };
+    // One type's code is run, and read for the first time: branches inside held up the launch's end
+    if (y_type == Q8_F32) store(w8_type<Q8_F32>{});
+    else if (y_type == Q8_F16) store(w8_type<Q8_F16>{});
+    else store(w8_type<Q8_BF16>{});
 }
 
 #define W8_TILED(NAME, BM, AHEAD, XRING, GLU)                                                                                     \
