@@ -159,7 +159,7 @@ extern "C" int w4a16_lin_w8a8_info(w4a16_ctx* ctx, const char* name, size_t* n, 
 }
 
 // ------------------------------------------------------------------------------------------------ forward
-// Launch of the kernel for up to 64 rows: row blocks per workgroup, waves, k slices; a function of the shape alone.
+// Launch of the kernel for groups of up to 64 rows: row blocks per workgroup, waves, k slices; a function of the shape alone.
 struct SkinnyPlan {
     int rb = 1, waves = 8, nks = 1;
     double price = 0.0;
@@ -167,29 +167,32 @@ struct SkinnyPlan {
 
 static SkinnyPlan plan_skinny(size_t n, size_t k, size_t t, size_t cus, bool glu) {
     const size_t kt = k_tiles(k), blocks16 = (n + 15) / 16;
-    const int tt = (int)((t + 15) / 16);
+    const size_t groups = (t + 63) / 64;
+    const int tt = (int)((t + 16 * groups - 1) / (16 * groups));
     SkinnyPlan best;
     best.price = 1e30;
     for (int rb = 4; rb >= (glu ? 2 : 1); rb /= 2) {
         for (int nks = 1; nks <= 8; nks++) {
-            const size_t blocks = (blocks16 + rb - 1) / rb, grid = blocks * nks;
+            const size_t blocks = (blocks16 + rb - 1) / rb, grid = blocks * nks * groups;
             if (nks > 1 && ((size_t)nks * 8 > kt || grid > 4 * cus)) break;
             const double run = (double)kt / nks;
             // Price in us, fitted to 3000 launches of 19 shapes (n 512 .. 65536, k 1024 .. 17408) at 1 .. 64 rows, cold weights: what it
             // picks is 1.7 % slower in the mean than the best of them.  A CU takes 50 KiB per us of weights and half of the activations'
             // (from the L2); workgroups over those that all CUs have cost nearly a whole one; slices cost a hand-over and their sums' way
             // through memory.  5120 x 17408 at t = 16: one row block, whole k 23.9 us, four and three slices 17.7; 7168 x 5120 at t = 64:
-            // 17.5, two row blocks 12.7.
+            // 17.5, two row blocks 12.7.  Several groups have the weights from the L2, too: fitted, with the launch itself, to 1100 launches
+            // of 19 shapes (n 64 .. 34816, k 320 .. 17408) at 65 .. 600 rows.
             const size_t full = grid / cus, rest = grid % cus;
             const double rounds = (double)full + (rest == 0 ? 0.0 : full == 0 ? 1.0 : 0.94 + 0.06 * (double)rest / (double)cus);
-            const double load = run * (rb + 0.48 * (t <= 4 ? 0.25 : tt));
+            const double load = run * (rb + (groups > 1 ? 0.28 : 0.48) * (t <= 4 ? 0.25 : tt));
+            const double sums = 1e-6 * nks * n * t * 8, join = nks == 1 ? 0.0 : groups > 1 ? 0.91 + 0.37 * sums : 2.07 + 0.24 * sums;
             SkinnyPlan p;
             p.rb = rb;
             p.nks = nks;
             // four waves where a CU has several workgroups and eight would have few k tiles each or hold many sums, or k is short
             p.waves = (grid > cus && (run <= 40 || rb * tt >= 16)) || run <= 16 ? 4 : 8;
             p.waves = (int)std::min<size_t>(p.waves, kt);
-            p.price = std::max(rounds * load / 49.6, (double)(blocks16 * kt) / 9079.0) + (nks > 1 ? 2.07 + 0.24e-6 * nks * n * t * 8 : 0.0);
+            p.price = (groups > 1 ? 4.3 : 0.0) + std::max(rounds * load / (groups > 1 ? 34.2 : 49.6), (double)(blocks16 * kt) / 9079.0) + join;
             if (p.price < best.price) best = p;
         }
     }
@@ -207,16 +210,17 @@ static int split_workspace(w4a16_ctx* ctx, size_t part_bytes, size_t tickets) {
 
 static int launch_skinny(w4a16_ctx* ctx, const W8Lin& L, const SkinnyPlan& P, uint64_t q, uint64_t s, size_t t, uint64_t y, int y_type, int act) {
     const bool glu = act >= 0;
-    const int tt = (int)((t + 15) / 16);
+    const size_t groups = (t + 63) / 64;  // of as many rows each as can be
+    const int tt = (int)((t + 16 * groups - 1) / (16 * groups));
     const size_t kt = k_tiles(L.k), blocks16 = (L.n + 15) / 16;
     char sym[64];
     snprintf(sym, sizeof sym, "w4a16_w8a8_skinny_r%d_t%d%s", P.rb, tt, glu ? "_glu" : "");
     const unsigned grid = glu ? ceil_div(blocks16 / 2, P.rb / 2) : ceil_div(blocks16, P.rb);
-    if (P.nks > 1) W4_TRY(split_workspace(ctx, (size_t)grid * P.nks * P.rb * tt * 1024, grid));
+    if (P.nks > 1) W4_TRY(split_workspace(ctx, (size_t)grid * groups * P.nks * P.rb * tt * 1024, grid * groups));
     uint64_t wt = L.q, ws = L.s, part = ctx->w8_part, tickets = ctx->w8_tickets;
     int ni = (int)L.n, kti = (int)kt, ti = (int)t, r = (int)tile_rows(t), wi = P.waves, ksi = P.nks;
     void* params[] = {&wt, &ws, &q, &s, &y, &ni, &kti, &ti, &r, &y_type, &act, &wi, &ksi, &part, &tickets};
-    return w4_launch(ctx, sym, grid, (unsigned)P.nks, (unsigned)P.waves * 64, 0, params);
+    return w4_launch(ctx, sym, grid, (unsigned)(P.nks * groups), (unsigned)P.waves * 64, 0, params);
 }
 
 // Launch of the tiled kernel: 64 or 128 rows per tile, k slices; a function of the shape alone.
@@ -233,18 +237,19 @@ static TiledPlan plan_tiled(size_t n, size_t k, size_t t, size_t cus, bool glu) 
         for (int nks = 1; nks <= 8; nks++) {
             const size_t grid = (t + bm - 1) / bm * tiles_n * nks;
             if (nks > 1 && ((size_t)nks * 8 > kt || grid > 2 * cus)) break;
-            // Price in us, fitted to 300 launches of 7 shapes (n 1000 .. 34816, k 2048 .. 17408) at 65 .. 4096 rows, cold weights: what it
-            // picks is 0.6 % slower in the mean than the best of them.  A k tile takes a workgroup 0.27 us (64 rows) or 0.44 us (128) alone
-            // on its CU, twice that where the CU has two of them; a round over that costs between its share and a whole one; slices cost
-            // their sums' way through memory.  5120 x 17408 at t = 300: 128 rows, whole k 113 us, four slices 53; t = 100: 64 rows, whole k
-            // 73 us, six slices 34; 22016 x 4096 gated at t = 1000: 64 rows 127 us, 128 rows 109.
-            const double alone = bm == 64 ? 0.27 : 0.44, pair = bm == 64 ? 0.54 : 0.83;
+            // Price in us, fitted to 1500 launches of 23 shapes (n 64 .. 34816, k 320 .. 17408) at 65 .. 4096 rows, cold weights: what it
+            // and the price above pick is 2.4 % slower in the mean than the best of both.  A k tile takes a workgroup 0.29 us (64 rows) or
+            // 0.45 us (128) alone on its CU, twice that where the CU has two of them; a round over that costs between its share and a
+            // whole one; slices cost their sums' way through memory.  5120 x 17408 at t = 300: 128 rows, whole k 113 us, four slices 53;
+            // 22016 x 4096 gated at t = 1000: 64 rows 127 us, 128 rows 100.  Against groups of 64 rows: 64 x 8256 at t = 256 groups 6.4 us,
+            // tiles 14.3; 4096 x 4096 at t = 128 10.0 and 13.3, at t = 400 19.5 and 17.0; 34816 x 5120 gated at t = 100 72 and 52.
+            const double alone = bm == 64 ? 0.29 : 0.45, pair = bm == 64 ? 0.58 : 0.90;
             const double load = (double)grid / (double)cus, rounds = load / 2.0;
-            const double per_k = load <= 1.0 ? alone : rounds <= 1.0 ? pair : pair * (0.6 * std::ceil(rounds) + 0.4 * rounds);
+            const double per_k = load <= 1.0 ? alone : rounds <= 1.0 ? pair : pair * (0.47 * std::ceil(rounds) + 0.53 * rounds);
             TiledPlan p;
             p.bm = bm;
             p.nks = nks;
-            p.price = (double)((kt + nks - 1) / nks) * per_k + (nks > 1 ? (1.2 * nks + 10.0 * load) * bm / 128.0 : 0.0);
+            p.price = 5.0 + (double)((kt + nks - 1) / nks) * per_k + (nks > 1 ? (1.0 * nks + 9.4 * load) * bm / 128.0 : 0.0);
             if (p.price < best.price) best = p;
         }
     }
@@ -257,7 +262,7 @@ static int launch_tiled(w4a16_ctx* ctx, const W8Lin& L, const TiledPlan& P, uint
     if (tiles * nks > 0x7ffffff0u) return w4_fail(W4A16_ERR_SHAPE, "lin_w8a8: t=%zu n=%zu exceed the grid", t, L.n);
     if (nks > 1) W4_TRY(split_workspace(ctx, tiles * nks * P.bm * 1024, tiles));
     uint64_t wt = L.q, ws = L.s, part = ctx->w8_part, tickets = ctx->w8_tickets;
-    // 1024 rows of tiles share their weights in the L2: 34816 x 5120 gated at t = 4096 666 us, 512 rows 679, 256 rows 727
+    // 1024 rows of tiles share their weights in the L2: 34816 x 5120 gated at t = 4096 673 us in an earlier state, 512 rows 679, 256 rows 727
     int ni = (int)L.n, kti = (int)k_tiles(L.k), ti = (int)t, ki = P.nks, band = 1024 / P.bm;
     char sym[64];
     snprintf(sym, sizeof sym, "w4a16_w8a8_tiled_m%d%s", P.bm, glu ? "_glu" : "");
@@ -293,8 +298,11 @@ static int forward_w8a8(w4a16_ctx* ctx, const char* api, const char* name, uint6
         xs = ctx->q8_scales;
     }
     const size_t cus = (size_t)std::max(ctx->cu_count, 1);
-    if (t <= 64) return launch_skinny(ctx, *L, plan_skinny(L->n, L->k, t, cus, act >= 0), x, xs, t, y, y_type, act);
-    return launch_tiled(ctx, *L, plan_tiled(L->n, L->k, t, cus, act >= 0), x, xs, t, y, y_type, act);
+    const SkinnyPlan few = plan_skinny(L->n, L->k, t, cus, act >= 0);
+    if (t <= 64) return launch_skinny(ctx, *L, few, x, xs, t, y, y_type, act);
+    const TiledPlan tiles = plan_tiled(L->n, L->k, t, cus, act >= 0);
+    if (t <= 1024 && few.price < tiles.price) return launch_skinny(ctx, *L, few, x, xs, t, y, y_type, act);
+    return launch_tiled(ctx, *L, tiles, x, xs, t, y, y_type, act);
 }
 
 extern "C" int w4a16_lin_forward_w8a8(w4a16_ctx* ctx, const char* name, uint64_t x_dev, int x_type, size_t ldx, uint64_t xs_dev, size_t t,

@@ -46,7 +46,7 @@ __device__ __forceinline__ void w8_store4(void* __restrict__ y, size_t at, int l
 // outputs each); the weights arrive as whole tiles straight in registers, DEPTH of them in flight per row block, meet TT tiles of 16
 // activation rows (from the L2), and the waves' sums are added in LDS: whole numbers, so in any order the same.  Where there are too
 // few row blocks for the chip, slices of k go to several workgroups (gridDim.y of them): each leaves its sums in the workspace and
-// draws a ticket of its row blocks, the last one adds them.
+// draws a ticket of its row blocks, the last one adds them.  More than TT * 16 rows: groups of so many, each through all of it.
 typedef unsigned long long w8_pair_t;
 
 template <int RB, int TT, bool GLU>
@@ -74,7 +74,9 @@ __device__ __forceinline__ void skinny_body(const char* __restrict__ wt, const f
     const char* const xp = xq + ((size_t)kg * R + tok % R) * 16;
     const size_t x_tile = (size_t)R * 64, x_block = x_tile * kt;
 
-    const int runs = nks * W, run = blockIdx.y * W + wave;
+    const int ks = blockIdx.y % (unsigned)nks, group = blockIdx.y / (unsigned)nks, groups = gridDim.y / (unsigned)nks;
+    const int runs = nks * W, run = ks * W + wave;
+    const int m0 = group * TT * 16, x_last = (t - 1) >> 4;  // rows of the group, and the last tile of 16 that there is
     const int lo = (int)((long long)kt * run / runs), hi = (int)((long long)kt * (run + 1) / runs);
     i4_t acc[RB][TT];
 #pragma unroll
@@ -86,7 +88,7 @@ __device__ __forceinline__ void skinny_body(const char* __restrict__ wt, const f
 #pragma unroll
         for (int i = 0; i < RB; i++) wv[d][i] = __builtin_nontemporal_load(reinterpret_cast<const i4_t*>(wp[i] + (size_t)k * 1024));
 #pragma unroll
-        for (int j = 0; j < TT; j++) xv[d][j] = *reinterpret_cast<const i4_t*>(xp + j * x_block + k * x_tile);
+        for (int j = 0; j < TT; j++) xv[d][j] = *reinterpret_cast<const i4_t*>(xp + min((m0 >> 4) + j, x_last) * x_block + k * x_tile);
     };
 #pragma unroll
     for (int d = 0; d < DEPTH; d++)
@@ -125,31 +127,32 @@ __device__ __forceinline__ void skinny_body(const char* __restrict__ wt, const f
         return v;
     };
     constexpr int U = GLU ? RB / 2 : RB;
-    const size_t slice = (size_t)gridDim.x * (TILES * 128);  // pairs of sums per k slice
-    w8_pair_t* const mine = part + (size_t)blockIdx.x * (TILES * 128) + lane;
+    const unsigned own = group * gridDim.x + blockIdx.x;
+    const size_t slice = (size_t)gridDim.x * groups * (TILES * 128);  // pairs of sums per k slice
+    w8_pair_t* const mine = part + (size_t)own * (TILES * 128) + lane;
     if (nks > 1) {
         // Device-scope stores, complete before the ticket is drawn; device-scope loads behind the barrier that follows the ticket's return.
         // Neither is served from a cache that is not coherent.
 #pragma unroll
         for (int u = 0; u < TILES; u++) {
-            if (u % W != wave || (u % TT) * 16 + tok >= t) continue;
+            if (u % W != wave || m0 + (u % TT) * 16 + tok >= t) continue;
             const i4_t v = W > 1 ? total(u) : acc[u / TT][u % TT];
-            w8_pair_t* const p = mine + blockIdx.y * slice + u * 128;
+            w8_pair_t* const p = mine + ks * slice + u * 128;
             __hip_atomic_store(p, (w8_pair_t)(unsigned)v[1] << 32 | (unsigned)v[0], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             __hip_atomic_store(p + 64, (w8_pair_t)(unsigned)v[3] << 32 | (unsigned)v[2], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         }
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
-        if (threadIdx.x == 0) last_one = __hip_atomic_fetch_add(tickets + blockIdx.x, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == nks - 1;
+        if (threadIdx.x == 0) last_one = __hip_atomic_fetch_add(tickets + own, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == nks - 1;
         __syncthreads();
         if (!last_one) return;
-        if (threadIdx.x == 0) __hip_atomic_store(tickets + blockIdx.x, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);  // for the next launch
+        if (threadIdx.x == 0) __hip_atomic_store(tickets + own, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);  // for the next launch
     }
 #pragma unroll
     for (int u = 0; u < U * TT; u++) {
         if (u % W != wave) continue;  // uniform for the wave
         const int i = GLU ? u / TT * 2 : u / TT, j = u % TT;
-        const int b = block_of(i), m = j * 16 + tok, c = b * 16 + kg * 4;
+        const int b = block_of(i), m = m0 + j * 16 + tok, c = b * 16 + kg * 4;
         if (b > last || m >= t) continue;
         auto sum_of = [&](int i_) {
             if (nks == 1) return W > 1 ? total(i_ * TT + j) : acc[i_][j];
