@@ -21,7 +21,7 @@
 #define SCORE_MAX_TOP 32
 #define SCORE_STAGE_BYTES 4096  // of a wave's stage, 64 per lane
 #define SCORE_WAVES 4
-#define SCORE_LIST 96          // places of a wave's list: SCORE_MAX_TOP carried over and 64 of one step
+#define SCORE_LIST 128         // places of a wave's list: 2 SCORE_MAX_TOP carried over and 64 of one step
 #define SCORE_BATCH 32         // lanes that put their elements down at a time, half as many where they have 32
 #define SCORE_RECORD 272       // bytes of a workgroup's record: max, S, U, padding, SCORE_MAX_TOP keys
 
@@ -110,7 +110,8 @@ struct ScoreTop {
         const unsigned long long all = __ballot(in);
         if (in) list[count + __builtin_amdgcn_mbcnt_hi((unsigned)(all >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)all, 0))] = key;
         count += __popcll(all);
-        if (count <= SCORE_MAX_TOP) return;
+        // Room beyond `top`, or the last of the first stage's keys would cost a cut each: 2538 rows of 1249 f16, top 32, 49 us, with room 29
+        if (count <= max(SCORE_MAX_TOP, 2 * top)) return;
         // cut to the `top` best, best first
         if (lane < 4) list[count + lane] = 0;  // the loop goes by four
         score_wave_sync();
