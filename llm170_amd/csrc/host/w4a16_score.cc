@@ -39,7 +39,9 @@ extern "C" int w4a16_token_logprobs(w4a16_ctx* ctx, uint64_t logits_dev, int log
         W4_TRY(w4_ensure(ctx, &ctx->score_ws, &ctx->score_ws_cap, t * segs * kW4ScoreRecord));
         if (t * 4 > ctx->score_tickets_cap) {
             W4_TRY(w4_ensure(ctx, &ctx->score_tickets, &ctx->score_tickets_cap, std::max<size_t>(t * 4, 8192)));
-            W4_TRY(w4a16_memset0(ctx, ctx->score_tickets, ctx->score_tickets_cap));
+            const int rc = w4a16_memset0(ctx, ctx->score_tickets, ctx->score_tickets_cap);
+            if (rc) ctx->score_tickets_cap = 0;  // not cleared: asked for anew
+            W4_TRY(rc);
         }
     }
     uint64_t ws = ctx->score_ws, tickets = ctx->score_tickets;

@@ -3,6 +3,8 @@
 #include <cmath>
 #include <cstdio>
 #include <cstring>
+#include <memory>
+#include <new>
 
 #include "w4a16_internal.h"
 
@@ -109,14 +111,15 @@ extern "C" int w4a16_upload_lin_w8a8(w4a16_ctx* ctx, const char* name, const voi
     L.n = n;
     L.k = k;
     const size_t row_blocks = (n + 15) / 16, kt = k_tiles(k), chunks = row_blocks * kt * 64;
-    std::vector<float> scales(row_blocks * 16, 0.0f);
+    std::unique_ptr<float[]> scales(new (std::nothrow) float[row_blocks * 16]());
+    if (!scales) return w4_fail(W4A16_ERR_ARG, "upload_lin_w8a8 %s: no host memory for %zu scales", name, n);
     for (size_t i = 0; i < n; i++) scales[i] = scale_at(s, s_type, i);
     uint64_t raw = 0;
     int rc = w4a16_alloc(ctx, chunks * 16, &L.q);
-    if (!rc) rc = w4a16_alloc(ctx, scales.size() * 4, &L.s);
+    if (!rc) rc = w4a16_alloc(ctx, row_blocks * 64, &L.s);
     if (!rc) rc = w4a16_alloc(ctx, qlen_bytes, &raw);
     if (!rc) rc = w4a16_h2d(ctx, raw, q, qlen_bytes);
-    if (!rc) rc = w4a16_h2d(ctx, L.s, scales.data(), scales.size() * 4);
+    if (!rc) rc = w4a16_h2d(ctx, L.s, scales.get(), row_blocks * 64);
     if (!rc) {
         size_t ns = n, cs = chunks;
         int ki = (int)k, kti = (int)kt;
@@ -203,7 +206,9 @@ static int split_workspace(w4a16_ctx* ctx, size_t part_bytes, size_t tickets) {
     W4_TRY(w4_ensure(ctx, &ctx->w8_part, &ctx->w8_part_cap, part_bytes));
     if (tickets * 4 > ctx->w8_tickets_cap) {
         W4_TRY(w4_ensure(ctx, &ctx->w8_tickets, &ctx->w8_tickets_cap, std::max<size_t>(tickets * 4, 16384)));
-        W4_TRY(w4a16_memset0(ctx, ctx->w8_tickets, ctx->w8_tickets_cap));
+        const int rc = w4a16_memset0(ctx, ctx->w8_tickets, ctx->w8_tickets_cap);
+        if (rc) ctx->w8_tickets_cap = 0;  // not cleared: asked for anew
+        W4_TRY(rc);
     }
     return 0;
 }

@@ -161,6 +161,23 @@ def test_one_row_or_many_give_the_same_alternatives_and_a_second_call_the_same_b
     check(first, z, targets, top)
 
 
+def test_rows_beyond_32_bits(dec):
+    v, ld, cc = 5000, 2_200_000_001, dec.cc
+    bits, z = ref.narrow(np.random.default_rng(2).standard_normal((2, v)).astype(np.float32) * 3, ffi.F16)
+    wide = cc.alloc(2 * (ld + v))
+    try:
+        with ref.Buffers(cc) as b:
+            for i in range(2):
+                cc.h2d(wide + 2 * i * ld, bits[i])
+            o = [b.filled(n * 4) for n in (2, 2, 64, 64)]
+            dec.token_logprobs(wide, 2, v, logits_type=ffi.F16, ld=ld, targets_dev=b.put(np.array([7, 4999], np.int32)), logp_dev=o[0], entropy_dev=o[1],
+                               top_k=32, top_idx_dev=o[2], top_logp_dev=o[3])
+            got = [cc.d2h(p, s, d) for p, s, d in zip(o, ((2,), (2,), (2, 32), (2, 32)), (np.float32, np.float32, np.int32, np.float32))]
+    finally:
+        cc.free(wide)
+    check(got, z, [7, 4999], 32)
+
+
 def test_capture_and_replay(dec):
     """A head and its scoring in one graph: tickets are back at zero after every replay, new logits give new results."""
     cc, v, k, t, top = dec.cc, 9000, 256, 3, 10

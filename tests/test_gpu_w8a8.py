@@ -338,6 +338,40 @@ def test_new_weights_under_an_old_name(dec):
         graph.destroy()
 
 
+def test_offsets_beyond_32_bits(dec):
+    """Rows 2.2e9 elements apart on the way in; results of more than 4 GiB on the way out, by tiles."""
+    k, n, cc = 1000, 32, dec.cc
+    r = np.random.default_rng(8)
+    x = r.standard_normal((3, k)).astype(np.float32)
+    w, sb, sv = ref.weights(3, n, k)
+    dec.upload_lin_w8a8("far", w, sb, n, k)
+    want = ref.product(*ref.quantised(x), w, sv)
+    ld = 550_000_000
+    with ref.Buffers(cc) as b:
+        wide, y = cc.alloc(4 * (2 * ld + k)), b.filled(3 * n * 4)
+        try:
+            for i in range(3):
+                cc.h2d(wide + 4 * i * ld, x[i])
+            dec.lin_forward_w8a8("far", wide, y, 3, x_type=ffi.F32, ldx=ld, y_type=ffi.F32)
+            assert np.array_equal(cc.d2h(y, (3, n), np.float32), want)
+        finally:
+            cc.free(wide)
+    t, n, k = 33000, 33000, 64
+    w, sb, sv = ref.weights(4, n, k)
+    dec.upload_lin_w8a8("far", w, sb, n, k)
+    bits, x = ref.narrow(r.standard_normal((t, k)).astype(np.float32), ffi.F16)
+    rows = [0, 1, 16270, 32535, 32540, t - 1]  # around 2^32 bytes, and the ends
+    want = ref.product(*ref.quantised(x[rows]), w, sv)
+    with ref.Buffers(cc) as b:
+        dx, y = b.put(bits), cc.alloc(t * n * 4)
+        try:
+            dec.lin_forward_w8a8("far", dx, y, t, x_type=ffi.F16, y_type=ffi.F32)
+            for i, row in enumerate(rows):
+                assert np.array_equal(cc.d2h(y + row * n * 4, (n,), np.float32), want[i]), row
+        finally:
+            cc.free(y)
+
+
 def test_captured_ffn_replays_the_eager_bits(dec):
     """norm, gated projection, down projection in one graph; replayed with eager work of other sizes in between, on new inputs."""
     h, f, cc = 384, 512, dec.cc
