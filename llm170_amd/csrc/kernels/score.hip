@@ -16,6 +16,9 @@
 // part of it is there once.
 // A row goes to one workgroup or, where there are few rows, to several: each leaves its record in the workspace and draws a
 // ticket, the last one joins them.
+// 2048 x 100003 f16 with its best token 90 us, 4.6 TB/s: the exponentials' issue and the stream, which a copy runs at 5.2 TB/s.  64 x
+// 131072 bf16, 20 best, 21.6 us, 1 x 32000 f32, 5 best, 9: chains of latencies (the first stage 2.4 us, each later one about 1.9, the
+// joining of the waves and of the records several), not bytes.
 #include "q8_common.hpp"
 
 #define SCORE_MAX_TOP 32
