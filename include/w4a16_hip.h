@@ -503,8 +503,7 @@ int w4a16_bench_chain(w4a16_ctx* ctx, const char* prefix, size_t n_layers, uint6
 
 /* ------------------------------------------------------------------------------------------------------------
  * W8A8 linears: int8 weights w [n][k] with one scale per output channel, activations quantised to int8 with one scale
- * per row.  The reference keeps its language-model heads this way (int8 weights, assets/head.cu); its activations stay
- * floats there.
+ * per row.  The reference keeps the weights of its language-model heads in int8 (assets/head.cu).
  *     y[m][c] = (sum_k q[m][k] w[c][k]) * s[m] * ws[c]
  * The sum is exact (32-bit whole numbers; k <= 131071), the two products are rounded to f32 in this order and the result
  * once more to y's type.

@@ -119,7 +119,7 @@ static const char* const kQuantSyms[] = {"w4a16_quant_rows_f32", "w4a16_quant_ro
 #define W8_TT(P, S) P "_t1" S, P "_t2" S, P "_t3" S, P "_t4" S
 static const char* const kW8a8Syms[] = {W8_TT("w4a16_w8a8_skinny_r1", ""), W8_TT("w4a16_w8a8_skinny_r2", ""), W8_TT("w4a16_w8a8_skinny_r4", ""),
                                         W8_TT("w4a16_w8a8_skinny_r2", "_glu"), W8_TT("w4a16_w8a8_skinny_r4", "_glu"),
-                                        "w4a16_w8a8_tiled_m128", "w4a16_w8a8_tiled_m128_glu", "w4a16_w8a8_tiled_m64", "w4a16_w8a8_tiled_m64_glu", nullptr};
+                                        "w4a16_w8a8_tiled_m128", "w4a16_w8a8_tiled_m128_glu", "w4a16_w8a8_tiled_m64", "w4a16_w8a8_tiled_m64_glu", "w4a16_w8a8_tiled_m64_n128", "w4a16_w8a8_tiled_m64_n128_glu", nullptr};
 static const char* const kScoreSyms[] = {"w4a16_token_logprobs_f32", "w4a16_token_logprobs_f16", "w4a16_token_logprobs_bf16", nullptr};
 
 struct W4Asset {

@@ -228,33 +228,35 @@ static int launch_skinny(w4a16_ctx* ctx, const W8Lin& L, const SkinnyPlan& P, ui
     return w4_launch(ctx, sym, grid, (unsigned)(P.nks * groups), (unsigned)P.waves * 64, 0, params);
 }
 
-// Launch of the tiled kernel: 64 or 128 rows per tile, k slices; a function of the shape alone.
+// Launch of the tiled kernel: rows and columns (of weights) per tile, k slices; a function of the shape alone.
 struct TiledPlan {
-    int bm = 64, nks = 1;
+    int bm = 64, bn = 128, nks = 1;
     double price = 0.0;
 };
 
-static TiledPlan plan_tiled(size_t n, size_t k, size_t t, size_t cus, bool glu) {
-    const size_t kt = k_tiles(k), tiles_n = glu ? (n / 2 + 127) / 128 : (n + 255) / 256;
+static TiledPlan plan_tiled(size_t n, size_t k, size_t t, size_t cus) {
+    // Price in us, fitted to 1100 launches of 15 shapes (n 688 .. 34816, k 320 .. 17408) at 65 .. 2048 rows, cold weights: what it and the
+    // price above pick is 1.6 % slower in the mean than the best of both.  us per k tile of a workgroup alone on its CU and of as many as
+    // a CU holds; a round over those costs between its share and a whole one; slices cost their sums' way through memory.  The best by
+    // tile: 16000 x 2048 at t = 128 64 x 128 11.8 us, 64 x 256 15.2, 128 x 256 17.9; 5120 x 17408 at t = 300 48.2 in two slices, 49.4 in
+    // two, 44.0 in four; 22016 x 4096 gated at t = 1000 123, 113, 91.  Against groups of 64 rows: 64 x 8256 at t = 256 groups
+    // 6.4 us, tiles 12; 4096 x 4096 at t = 128 10.0 and 10.8, at t = 400 19.5 and 15; 34816 x 5120 gated at t = 100 72 and 52.
+    static const struct { int bm, bn, per_cu; double alone, full; } kTiles[] = {{64, 128, 3, 0.18, 0.50}, {64, 256, 2, 0.29, 0.57}, {128, 256, 2, 0.42, 0.90}};
+    const size_t kt = k_tiles(k);
     TiledPlan best;
     best.price = 1e30;
-    for (int bm = 64; bm <= 128; bm *= 2) {
+    for (const auto& T : kTiles) {
         for (int nks = 1; nks <= 8; nks++) {
-            const size_t grid = (t + bm - 1) / bm * tiles_n * nks;
-            if (nks > 1 && ((size_t)nks * 8 > kt || grid > 2 * cus)) break;
-            // Price in us, fitted to 1500 launches of 23 shapes (n 64 .. 34816, k 320 .. 17408) at 65 .. 4096 rows, cold weights: what it
-            // and the price above pick is 2.4 % slower in the mean than the best of both.  A k tile takes a workgroup 0.29 us (64 rows) or
-            // 0.45 us (128) alone on its CU, twice that where the CU has two of them; a round over that costs between its share and a
-            // whole one; slices cost their sums' way through memory.  5120 x 17408 at t = 300: 128 rows, whole k 113 us, four slices 53;
-            // 22016 x 4096 gated at t = 1000: 64 rows 127 us, 128 rows 100.  Against groups of 64 rows: 64 x 8256 at t = 256 groups 6.4 us,
-            // tiles 14.3; 4096 x 4096 at t = 128 10.0 and 13.3, at t = 400 19.5 and 17.0; 34816 x 5120 gated at t = 100 72 and 52.
-            const double alone = bm == 64 ? 0.29 : 0.45, pair = bm == 64 ? 0.58 : 0.90;
-            const double load = (double)grid / (double)cus, rounds = load / 2.0;
-            const double per_k = load <= 1.0 ? alone : rounds <= 1.0 ? pair : pair * (0.47 * std::ceil(rounds) + 0.53 * rounds);
+            const size_t grid = (t + T.bm - 1) / T.bm * ((n + T.bn - 1) / T.bn) * nks;
+            if (nks > 1 && ((size_t)nks * 8 > kt || grid > T.per_cu * cus)) break;
+            const double load = (double)grid / (double)cus, rounds = load / T.per_cu;
+            const double per_k = rounds <= 1.0 ? T.alone + (T.full - T.alone) * (std::ceil(load) - 1.0) / (T.per_cu - 1)
+                                               : T.full * (0.5 * std::ceil(rounds) + 0.5 * rounds);
             TiledPlan p;
-            p.bm = bm;
+            p.bm = T.bm;
+            p.bn = T.bn;
             p.nks = nks;
-            p.price = 5.0 + (double)((kt + nks - 1) / nks) * per_k + (nks > 1 ? (1.0 * nks + 9.4 * load) * bm / 128.0 : 0.0);
+            p.price = 4.7 + (double)((kt + nks - 1) / nks) * per_k + (nks > 1 ? (nks + 8.5 * load) * T.bm * T.bn / 32768.0 : 0.0);
             if (p.price < best.price) best = p;
         }
     }
@@ -263,14 +265,14 @@ static TiledPlan plan_tiled(size_t n, size_t k, size_t t, size_t cus, bool glu) 
 
 static int launch_tiled(w4a16_ctx* ctx, const W8Lin& L, const TiledPlan& P, uint64_t q, uint64_t s, size_t t, uint64_t y, int y_type, int act) {
     const bool glu = act >= 0;
-    const size_t tiles = (t + P.bm - 1) / P.bm * (glu ? (L.n / 2 + 127) / 128 : (L.n + 255) / 256), nks = (size_t)P.nks;
+    const size_t tiles = (t + P.bm - 1) / P.bm * ((L.n + P.bn - 1) / P.bn), nks = (size_t)P.nks;
     if (tiles * nks > 0x7ffffff0u) return w4_fail(W4A16_ERR_SHAPE, "lin_w8a8: t=%zu n=%zu exceed the grid", t, L.n);
-    if (nks > 1) W4_TRY(split_workspace(ctx, tiles * nks * P.bm * 1024, tiles));
+    if (nks > 1) W4_TRY(split_workspace(ctx, tiles * nks * P.bm * P.bn * 4, tiles));
     uint64_t wt = L.q, ws = L.s, part = ctx->w8_part, tickets = ctx->w8_tickets;
     // 1024 rows of tiles share their weights in the L2: 34816 x 5120 gated at t = 4096 673 us in an earlier state, 512 rows 679, 256 rows 727
     int ni = (int)L.n, kti = (int)k_tiles(L.k), ti = (int)t, ki = P.nks, band = 1024 / P.bm;
     char sym[64];
-    snprintf(sym, sizeof sym, "w4a16_w8a8_tiled_m%d%s", P.bm, glu ? "_glu" : "");
+    snprintf(sym, sizeof sym, "w4a16_w8a8_tiled_m%d%s%s", P.bm, P.bn == 128 ? "_n128" : "", glu ? "_glu" : "");
     void* params[] = {&wt, &ws, &q, &s, &y, &ni, &kti, &ti, &y_type, &act, &ki, &band, &part, &tickets};
     return w4_launch(ctx, sym, (unsigned)((tiles * nks + 7) / 8 * 8), 1, 256, 0, params);
 }
@@ -305,7 +307,7 @@ static int forward_w8a8(w4a16_ctx* ctx, const char* api, const char* name, uint6
     const size_t cus = (size_t)std::max(ctx->cu_count, 1);
     const SkinnyPlan few = plan_skinny(L->n, L->k, t, cus, act >= 0);
     if (t <= 64) return launch_skinny(ctx, *L, few, x, xs, t, y, y_type, act);
-    const TiledPlan tiles = plan_tiled(L->n, L->k, t, cus, act >= 0);
+    const TiledPlan tiles = plan_tiled(L->n, L->k, t, cus);
     if (t <= 1024 && few.price < tiles.price) return launch_skinny(ctx, *L, few, x, xs, t, y, y_type, act);
     return launch_tiled(ctx, *L, tiles, x, xs, t, y, y_type, act);
 }

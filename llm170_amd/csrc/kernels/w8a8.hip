@@ -199,7 +199,7 @@ W8_SKINNY_T(w4a16_w8a8_skinny_r2, 2, true, _glu)
 W8_SKINNY_T(w4a16_w8a8_skinny_r4, 4, true, _glu)
 
 // ------------------------------------------------------------------------------------------------ tiles, any number of rows
-// Block tile BM = 64 or 128 rows x 256 columns, four waves along n, wave tile BM x 64 on v_mfma_i32_16x16x64_i8 (the 32 x 32 x 32 form
+// Block tile BM = 64 or 128 rows x NB * 64 = 128 or 256 columns, four waves along n, wave tile BM x NB * 16 on v_mfma_i32_16x16x64_i8 (the 32 x 32 x 32 form
 // keeps up 3.3 POP/s on random bytes, this one 4.1).  Weights go straight into registers, activations through registers into LDS, a k tile
 // of 64 at a time, both asked for AHEAD k tiles ahead: a line's first reader of an XCD waits up to 2 us for it.  Nothing waits for the
 // newest loads: a k tile's barrier orders LDS alone, and with three LDS buffers the next tile's first blocks are read ahead of it.  The
@@ -218,19 +218,19 @@ __device__ __forceinline__ void w8_lds_barrier() {  // behind w8_lds_done
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
-template <int BM, int AHEAD, int XRING, bool GLU>
+template <int BM, int NB, int AHEAD, int XRING, bool GLU>
 __device__ __forceinline__ void tiled_body(const char* __restrict__ wt, const float* __restrict__ ws, const char* __restrict__ xq,
                                            const float* __restrict__ xs, void* __restrict__ y, int n, int kt, int t, int y_type, int act, int nks,
                                            int band, w8_pair_t* __restrict__ part, int* __restrict__ tickets) {
     constexpr int J = BM / 16, XL = J / 4, WAVES = 4, PERIOD = XRING == AHEAD ? AHEAD * (AHEAD + 1) : AHEAD + 1;
     static_assert(BM % 64 == 0 && PERIOD % 3 == 0 && (XRING == AHEAD || XRING == AHEAD + 1), "rings and the three buffers fit the period");
     __shared__ __attribute__((aligned(1024))) char lds[3][BM * 64];  // a k tile of activations: [row block] of 1 KiB
-    __shared__ __attribute__((aligned(16))) float w_scale[256], x_scale[BM];
+    __shared__ __attribute__((aligned(16))) float w_scale[NB * 64], x_scale[BM];
     __shared__ int last_one;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wn = wave;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int tok = lane & 15, kg = lane >> 4;
     const int out_n = GLU ? n >> 1 : n, half_rb = GLU ? n >> 5 : 0, row_blocks = (n + 15) >> 4;
-    constexpr int BN = GLU ? 128 : 256;
+    constexpr int BN = GLU ? NB * 32 : NB * 64;  // outputs
     // Block tiles: every XCD takes a consecutive eighth of them (and of their slices), bands of `band` tile rows, in a band m fastest
     const int tiles_m = (t + BM - 1) / BM, tiles_n = (out_n + BN - 1) / BN;
     const unsigned work = (unsigned)tiles_m * (unsigned)tiles_n * (unsigned)nks, xcd = blockIdx.x & 7;
@@ -245,26 +245,26 @@ __device__ __forceinline__ void tiled_body(const char* __restrict__ wt, const fl
     const int x_blocks = (t + 15) >> 4;
     const __amdgpu_buffer_rsrc_t xr = w4_make_rsrc(xq + (size_t)(m0 >> 4) * kt * 1024, (unsigned)min(x_blocks - (m0 >> 4), BM / 16) * (unsigned)kt * 1024u);
     // first row block of the wave's columns and what is left of the matrix behind it
-    const int wrb = (n0 >> 4) + wn * (GLU ? 2 : 4), w_end = GLU ? half_rb : row_blocks;
+    const int wrb = (n0 >> 4) + wave * (GLU ? NB / 2 : NB), w_end = GLU ? half_rb : row_blocks;
     auto w_rsrc = [&](int first, int count) {
         first = __builtin_amdgcn_readfirstlane(count > 0 ? first : 0);  // uniform, and known to be
         count = __builtin_amdgcn_readfirstlane(max(count, 0));
         return w4_make_rsrc(wt + (size_t)(unsigned)first * (unsigned)kt * 1024, (unsigned)count * (unsigned)kt * 1024u);
     };
-    const __amdgpu_buffer_rsrc_t wr0 = w_rsrc(wrb, min(w_end - wrb, GLU ? 2 : 4)),
-                                 wr1 = GLU ? w_rsrc(half_rb + wrb, min(w_end - wrb, 2)) : wr0;
-    // row block slot i of the wave: gated, slots 0 and 1 are the gate's, 2 and 3 its values'
-    unsigned wo[4], xo[XL];
+    const __amdgpu_buffer_rsrc_t wr0 = w_rsrc(wrb, min(w_end - wrb, GLU ? NB / 2 : NB)),
+                                 wr1 = GLU ? w_rsrc(half_rb + wrb, min(w_end - wrb, NB / 2)) : wr0;
+    // row block slot i of the wave: gated, the first half are the gate's, the second its values'
+    unsigned wo[NB], xo[XL];
 #pragma unroll
-    for (int i = 0; i < 4; i++) wo[i] = (unsigned)(GLU ? i & 1 : i) * (unsigned)kt * 1024u + lane * 16u;
+    for (int i = 0; i < NB; i++) wo[i] = (unsigned)(GLU ? i % (NB / 2) : i) * (unsigned)kt * 1024u + lane * 16u;
 #pragma unroll
     for (int i = 0; i < XL; i++) xo[i] = (unsigned)(wave + 4 * i) * (unsigned)kt * 1024u + lane * 16u;
     const int from = (int)((long long)kt * slice / nks), to = (int)((long long)kt * (slice + 1) / nks);
-    i4_t w[AHEAD + 1][4], x[XRING][XL], a[4];  // k tiles i .. i + AHEAD of the weights, i + 2 .. i + AHEAD + 1 of the activations
-    auto load_w = [&](i4_t (&d)[4], int k) {
+    i4_t w[AHEAD + 1][NB], x[XRING][XL], a[4];  // k tiles i .. i + AHEAD of the weights, i + 2 .. i + AHEAD + 1 of the activations
+    auto load_w = [&](i4_t (&d)[NB], int k) {
         const int at = min(k, to - 1) * 1024;  // behind the end the last tile again, not used
 #pragma unroll
-        for (int i = 0; i < 4; i++) d[i] = __builtin_bit_cast(i4_t, __builtin_amdgcn_raw_buffer_load_b128(GLU && i >= 2 ? wr1 : wr0, wo[i], at, 0));
+        for (int i = 0; i < NB; i++) d[i] = __builtin_bit_cast(i4_t, __builtin_amdgcn_raw_buffer_load_b128(GLU && i >= NB / 2 ? wr1 : wr0, wo[i], at, 0));
     };
     auto load_x = [&](i4_t (&d)[XL], int k) {
         const int at = min(k, to - 1) * 1024;
@@ -276,16 +276,16 @@ __device__ __forceinline__ void tiled_body(const char* __restrict__ wt, const fl
         for (int i = 0; i < XL; i++) *reinterpret_cast<i4_t*>(lds[buf] + (wave + 4 * i) * 1024 + lane * 16) = s[i];
     };
     auto get_x = [&](int buf, int j) { return *reinterpret_cast<const i4_t*>(lds[buf] + j * 1024 + lane * 16); };
-    i4_t acc[J][4];
+    i4_t acc[J][NB];
 #pragma unroll
     for (int j = 0; j < J; j++)
 #pragma unroll
-        for (int i = 0; i < 4; i++) acc[j][i] = (i4_t){0, 0, 0, 0};
+        for (int i = 0; i < NB; i++) acc[j][i] = (i4_t){0, 0, 0, 0};
     if (from < to) {
         i4_t first[XL];
-        // the tile's scales, for its end: gated, 128 of the gate and 128 of its values
-        const int c = n0 + (int)(GLU ? threadIdx.x & 127 : threadIdx.x), m = m0 + (int)threadIdx.x;
-        const float cs = c < out_n ? ws[GLU && threadIdx.x >= 128 ? out_n + c : c] : 0.f, ms = threadIdx.x < BM && m < t ? xs[m] : 0.f;
+        // the tile's scales, for its end: gated, first those of the gate, then of its values
+        const int c = n0 + (int)(GLU ? threadIdx.x % BN : threadIdx.x), m = m0 + (int)threadIdx.x;
+        const float cs = threadIdx.x < NB * 64 && c < out_n ? ws[GLU && threadIdx.x >= BN ? out_n + c : c] : 0.f, ms = threadIdx.x < BM && m < t ? xs[m] : 0.f;
         load_x(first, from);
 #pragma unroll
         for (int u = 0; u < AHEAD; u++) {
@@ -293,7 +293,7 @@ __device__ __forceinline__ void tiled_body(const char* __restrict__ wt, const fl
             load_w(w[u], from + u);
             __builtin_amdgcn_sched_barrier(0);  // in the order of the loop, whose waits count them
         }
-        w_scale[threadIdx.x] = cs;
+        if (threadIdx.x < NB * 64) w_scale[threadIdx.x] = cs;
         if (threadIdx.x < BM) x_scale[threadIdx.x] = ms;
         put_x(first, 0);
         put_x(x[1], 1);
@@ -313,7 +313,7 @@ __device__ __forceinline__ void tiled_body(const char* __restrict__ wt, const fl
                     __builtin_amdgcn_sched_barrier(0);
                     if (j == J / 2 - (J == 4 ? 2 : 1)) put_x(x[(u + 2) % XRING], (u + 2) % 3);  // read last a tile ago, which the barrier since then ends
 #pragma unroll
-                    for (int i = 0; i < 4; i++) acc[j][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[u % (AHEAD + 1)][i], a[j & 3], acc[j][i], 0, 0, 0);
+                    for (int i = 0; i < NB; i++) acc[j][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[u % (AHEAD + 1)][i], a[j & 3], acc[j][i], 0, 0, 0);
                     __builtin_amdgcn_sched_barrier(0);
                     if (j == J - 4) w8_lds_done();
                     a[j & 3] = j < J - 4 ? get_x(u % 3, j + 4) : get_x((u + 1) % 3, j + 4 - J);  // written a tile ago: there behind the last barrier
@@ -327,14 +327,14 @@ summed:
     if (nks > 1) {
         // [tile][slice][wave][block of 16 x 16][64 lanes] of 16 bytes, at device scope: past this XCD's L2
         constexpr int DEVICE = 16;  // sc1
-        constexpr unsigned MINE = J * 4 * 1024;
+        constexpr unsigned MINE = J * NB * 1024;
         char* const base = reinterpret_cast<char*>(part) + (size_t)tile * nks * WAVES * MINE;
         const __amdgpu_buffer_rsrc_t pr = w4_make_rsrc(base, (unsigned)nks * WAVES * MINE);
 #pragma unroll
         for (int j = 0; j < J; j++)
 #pragma unroll
-            for (int i = 0; i < 4; i++)
-                __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4_t, acc[j][i]), pr, lane * 16, ((int)slice * WAVES + wave) * (int)MINE + (j * 4 + i) * 1024, DEVICE);
+            for (int i = 0; i < NB; i++)
+                __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4_t, acc[j][i]), pr, lane * 16, ((int)slice * WAVES + wave) * (int)MINE + (j * NB + i) * 1024, DEVICE);
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
         if (threadIdx.x == 0) last_one = __hip_atomic_fetch_add(tickets + tile, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == nks - 1;
@@ -346,15 +346,15 @@ summed:
 #pragma unroll
             for (int j = 0; j < J; j++)
 #pragma unroll
-                for (int i = 0; i < 4; i++)
-                    acc[j][i] += __builtin_bit_cast(i4_t, __builtin_amdgcn_raw_buffer_load_b128(pr, lane * 16, (o * WAVES + wave) * (int)MINE + (j * 4 + i) * 1024, DEVICE));
+                for (int i = 0; i < NB; i++)
+                    acc[j][i] += __builtin_bit_cast(i4_t, __builtin_amdgcn_raw_buffer_load_b128(pr, lane * 16, (o * WAVES + wave) * (int)MINE + (j * NB + i) * 1024, DEVICE));
         }
     }
     // D register e of lane (tok, kg): output column 4 kg + e of its row block, row tok
-    constexpr int OUT = GLU ? 2 : 4;
-    f4_t col[4];
+    constexpr int OUT = GLU ? NB / 2 : NB;
+    f4_t col[NB];
 #pragma unroll
-    for (int i = 0; i < 4; i++) col[i] = *reinterpret_cast<const f4_t*>(&w_scale[(GLU ? (i >> 1) * 128 + wave * 32 + (i & 1) * 16 : wave * 64 + i * 16) + kg * 4]);
+    for (int i = 0; i < NB; i++) col[i] = *reinterpret_cast<const f4_t*>(&w_scale[(GLU ? i / OUT * BN : 0) + wave * OUT * 16 + i % OUT * 16 + kg * 4]);
     const int c0 = wrb * 16 + kg * 4;
     auto store = [&](auto type) {
         constexpr int T = decltype(type)::value;
@@ -369,7 +369,7 @@ summed:
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
                     v[e] = (float)acc[j][i][e] * sx * col[i][e];
-                    if (GLU) v[e] = w4_act_mul(v[e], (float)acc[j][i + 2][e] * sx * col[i + 2][e], act);
+                    if (GLU) v[e] = w4_act_mul(v[e], (float)acc[j][i + OUT][e] * sx * col[i + OUT][e], act);
                 }
                 if (m < t && c0 + i * 16 < out_n) w8_store4<T>(y, at + i * 16, out_n - c0 - i * 16, v);
             }
@@ -381,13 +381,15 @@ summed:
     else store(w8_type<Q8_BF16>{});
 }
 
-#define W8_TILED(NAME, BM, AHEAD, XRING, GLU)                                                                                     \
+#define W8_TILED(NAME, BM, NB, AHEAD, XRING, GLU)                                                                                 \
     extern "C" __global__ __launch_bounds__(256, 2) void NAME(const char* wt, const float* ws, const char* xq, const float* xs, void* y, int n, \
                                                               int kt, int t, int y_type, int act, int nks, int band, w8_pair_t* part,  \
                                                               int* tickets) {                                                     \
-        tiled_body<BM, AHEAD, XRING, GLU>(wt, ws, xq, xs, y, n, kt, t, y_type, act, nks, band, part, tickets);                    \
+        tiled_body<BM, NB, AHEAD, XRING, GLU>(wt, ws, xq, xs, y, n, kt, t, y_type, act, nks, band, part, tickets);                \
     }
-W8_TILED(w4a16_w8a8_tiled_m128, 128, 3, 3, false)
-W8_TILED(w4a16_w8a8_tiled_m128_glu, 128, 3, 3, true)
-W8_TILED(w4a16_w8a8_tiled_m64, 64, 5, 6, false)
-W8_TILED(w4a16_w8a8_tiled_m64_glu, 64, 5, 6, true)
+W8_TILED(w4a16_w8a8_tiled_m128, 128, 4, 3, 3, false)
+W8_TILED(w4a16_w8a8_tiled_m128_glu, 128, 4, 3, 3, true)
+W8_TILED(w4a16_w8a8_tiled_m64, 64, 4, 5, 6, false)
+W8_TILED(w4a16_w8a8_tiled_m64_glu, 64, 4, 5, 6, true)
+W8_TILED(w4a16_w8a8_tiled_m64_n128, 64, 2, 8, 9, false)
+W8_TILED(w4a16_w8a8_tiled_m64_n128_glu, 64, 2, 8, 9, true)

@@ -150,8 +150,9 @@ SHAPES = [(1, 16, 64), (1, 1, 1), (1, 4096, 4096), (1, 16500, 640), (2, 33, 130)
           (65, 256, 128), (65, 1, 1), (100, 513, 1000), (128, 256, 384), (129, 300, 64), (300, 520, 2051), (1000, 257, 129), (513, 4100, 640), (2049, 1030, 256),
           # groups of 64 rows, with k whole and in slices
           (65, 256, 1000), (70, 300, 2048), (129, 1000, 2048), (66, 300, 17408), (100, 700, 12000), (257, 5, 8000), (400, 10000, 128), (577, 1300, 4100),
-          # tiles of 64 and 128 rows, with k whole and in slices
-          (200, 10000, 8000), (1025, 300, 128), (1100, 256, 1000), (1089, 515, 2048), (1100, 70, 8000), (1100, 4100, 128), (130, 10016, 4096), (1025, 2000, 8000)]
+          # tiles of 64 x 128, 64 x 256 and 128 x 256, with k whole and in slices
+          (200, 10000, 8000), (1025, 300, 128), (1100, 256, 1000), (1089, 515, 2048), (1100, 70, 8000), (1100, 4100, 128), (130, 10016, 4096), (1025, 2000, 8000),
+          (129, 6000, 4096), (200, 6001, 8000)]
 
 
 @pytest.mark.parametrize("t,n,k", SHAPES)
@@ -239,7 +240,7 @@ def test_rows_with_no_number_stay_alone(dec, t):
 @pytest.mark.parametrize("gelu", [False, True])
 @pytest.mark.parametrize("t,n,k", [(1, 32, 64), (1, 34816, 256), (2, 96, 200), (4, 22016, 128), (16, 1056, 777), (17, 64, 64), (33, 33000 // 32 * 32, 128), (48, 320, 100),
                                    (64, 2080, 640), (65, 32, 64), (70, 544, 333), (257, 1088, 512), (70, 800, 9000), (140, 2080, 4100), (450, 9984, 128),
-                                   (1030, 96, 128), (1100, 544, 2050), (1025, 64, 8000), (1100, 4128, 128), (130, 10016, 4096)])
+                                   (1030, 96, 128), (1100, 544, 2050), (1025, 64, 8000), (1100, 4128, 128), (130, 10016, 4096), (129, 6016, 4096), (201, 10016, 8000)])
 def test_gated_is_the_linear_and_its_activation(dec, t, n, k, gelu):
     say("glu", t, n, k, gelu)
     w, sb, sv = ref.weights(n + k, n, k)
@@ -420,7 +421,7 @@ def test_captured_ffn_replays_the_eager_bits(dec):
 
 
 @pytest.mark.parametrize("t,n,k,gelu", [(16, 1024, 8000, None), (60, 640, 4096, False), (70, 512, 4096, None), (130, 2048, 8192, True), (200, 10000, 8000, None),
-                                        (1100, 300, 4096, None), (1030, 256, 8000, False)])
+                                        (1100, 300, 4096, None), (1030, 256, 8000, False), (129, 6000, 4096, None)])
 def test_captured_slices_of_k_replay_the_eager_bits(dec, t, n, k, gelu):
     """Slices hand their sums over through scratch and tickets that every call of the context shares: graphs and eager calls in turn."""
     cc = dec.cc

@@ -49,4 +49,4 @@ def test_no_barrier_with_lds_dma_in_flight():
         bad, dma = open_barriers(insns)
         seen += "tiled" in name
         assert not bad and dma == 0, name
-    assert seen == 4
+    assert seen == 6
