@@ -87,6 +87,7 @@ __device__ __forceinline__ void skinny_body(const char* __restrict__ wt, const f
         for (int j = 0; j < TT; j++) acc[i][j] = (i4_t){0, 0, 0, 0};
     i4_t wv[DEPTH][RB], xv[DEPTH][TT];
     auto load = [&](int d, int k) {
+        // Non-temporal weights: 34816 x 5120 gated at t = 1 31.3 us, else 35.2; 4096 x 4096 at t = 128 in two groups 9.7, else 9.9
 #pragma unroll
         for (int i = 0; i < RB; i++) wv[d][i] = __builtin_nontemporal_load(reinterpret_cast<const i4_t*>(wp[i] + (size_t)k * 1024));
 #pragma unroll
