@@ -14,7 +14,7 @@ __device__ __forceinline__ unsigned quant_block_max(unsigned m, unsigned* red, i
 
 // s[r] = step of row r, q = round(x / s) in tiles of R rows.  A workgroup per row, a thread per 16 columns and round; the first
 // KEEP rounds stay in registers between the two passes over the row, what lies behind them is read again from the cache.
-// 4096 x 5120 f16 17 us, 300 x 17408 9.6, 4096 x 17408 65: the conversions' instructions bound the large ones, latency the small.
+// 4096 x 5120 f16 17 us, 300 x 17408 8.2, 4096 x 17408 52: the conversions' instructions bound the large ones, latency the small.
 #define QUANT_KEEP 2
 template <int T>
 __device__ __forceinline__ void quant_body(const void* __restrict__ x, size_t ldx, int k, int kt, int R, char* __restrict__ q,
