@@ -65,9 +65,9 @@ extern "C" int w4a16_norm_resid_q8(w4a16_ctx* ctx, uint64_t x_dev, uint64_t nw_d
     if (x_dev % 4 || nw_dev % 4 || ab_dev % 4 || s_dev % 4 || q_dev % 16)
         return w4_fail(W4A16_ERR_ARG, "norm_resid_q8: f32 operands must be aligned to 4 bytes, q to 16");
     W4_TRY(w4_hip(hipSetDevice(ctx->device), "hipSetDevice"));
-    int wo = (int)w_off, h = (int)hidden, kt = (int)k_tiles(hidden), r = (int)tile_rows(t);
-    void* params[] = {&x_dev, &nw_dev, &ab_dev, &q_dev, &s_dev, &wo, &h, &kt, &r};
-    return w4_launch(ctx, "w4a16_norm_resid_q8", (unsigned)t, 1, 1024, 0, params);
+    int wo = (int)w_off, h = (int)hidden, kt = (int)k_tiles(hidden), r = (int)tile_rows(t), ti = (int)t;
+    void* params[] = {&x_dev, &nw_dev, &ab_dev, &q_dev, &s_dev, &wo, &h, &kt, &r, &ti};
+    return w4_launch(ctx, "w4a16_norm_resid_q8", r == 16 ? ceil_div(t, 128) * 128 : (unsigned)t, 1, 1024, 0, params);
 }
 
 // ------------------------------------------------------------------------------------------------ registration

@@ -1,6 +1,13 @@
 // Quantisation of activation rows to int8 with one scale per row, and the re-layout of int8 weights at upload.
 #include "q8_common.hpp"
 
+// Sixteen neighbouring rows share their 256-byte runs of the tiles: they go to one XCD (block b runs on XCD b % 8), whose L2
+// joins their 16-byte pieces.
+__device__ __forceinline__ int q8_row_of_block(int R) {
+    const int b = blockIdx.x;
+    return R == 16 ? ((b >> 7) * 8 + (b & 7)) * 16 + ((b >> 3) & 15) : b;
+}
+
 // Largest of one value per thread over the workgroup.
 __device__ __forceinline__ unsigned quant_block_max(unsigned m, unsigned* red, int waves) {
     m = q8_wave_max(m);
@@ -20,9 +27,7 @@ template <int T>
 __device__ __forceinline__ void quant_body(const void* __restrict__ x, size_t ldx, int k, int kt, int R, char* __restrict__ q,
                                            float* __restrict__ s, int t, int threads) {
     __shared__ unsigned red[16];
-    // Sixteen neighbouring rows share their 256-byte runs of the tiles: they go to one XCD (block b runs on XCD b % 8), whose
-    // L2 joins their 16-byte pieces.
-    const int b = blockIdx.x, row = R == 16 ? ((b >> 7) * 8 + (b & 7)) * 16 + ((b >> 3) & 15) : b;
+    const int row = q8_row_of_block(R);
     if (row >= t) return;
     const char* const xr = static_cast<const char*>(x) + (size_t)row * ldx * (T == Q8_F32 ? 4 : 2);
     const int chunks = (k + 15) >> 4;
@@ -150,12 +155,15 @@ QUANT_FEW(w4a16_quant_few_bf16, Q8_BF16)
 
 // w4a16_norm_resid (glue.hip) and the quantisation of its f32 result in one pass: the same arithmetic in the same order, so the
 // rows are those of the two launches bit for bit.  x <- x + ab; xn = x * inv * nw[w_off + c] is rounded twice and never stored.
+// 4096 x 5120 50 us (the norm alone 51, its bytes 53 at a copy's rate), 300 x 5120 7.2; with byte stores and rows of a tile on all XCDs 59 and 8.7.
 extern "C" __global__ __launch_bounds__(1024) void w4a16_norm_resid_q8(float* __restrict__ x, const float* __restrict__ nw,
                                                                        const float* __restrict__ ab, char* __restrict__ q,
-                                                                       float* __restrict__ s, int w_off, int hidden, int kt, int R) {
+                                                                       float* __restrict__ s, int w_off, int hidden, int kt, int R, int t) {
     __shared__ float red[1024];
     __shared__ unsigned redm[16];
-    const int tid = threadIdx.x, row = blockIdx.x;
+    __shared__ __attribute__((aligned(16))) char line[8192];
+    const int tid = threadIdx.x, row = q8_row_of_block(R);
+    if (row >= t) return;
     const size_t base = (size_t)row * hidden;
     float v[8], y[8];
     float ss = 0.0f;
@@ -208,9 +216,13 @@ extern "C" __global__ __launch_bounds__(1024) void w4a16_norm_resid_q8(float* __
     unsigned o[2];
     q8_pack<8>(y, step, rs, o);
 #pragma unroll
-    for (int j = 0; j < 8; j++) {
-        const int c = j * 1024 + tid;
-        if (c < hidden) q[q8_chunk_at(row, c >> 4, kt, R) + (c & 15)] = (char)(o[j / 4] >> (8 * (j % 4)));
+    for (int j = 0; j < 8; j++) line[j * 1024 + tid] = (char)(o[j / 4] >> (8 * (j % 4)));
+    __syncthreads();
+    const int c = tid * 16;  // whole chunks, of the last one the bytes that there are
+    if (c + 16 <= hidden) {
+        *reinterpret_cast<u4_t*>(q + q8_chunk_at(row, tid, kt, R)) = *reinterpret_cast<const u4_t*>(line + c);
+    } else {
+        for (int i = c; i < hidden; i++) q[q8_chunk_at(row, tid, kt, R) + (i & 15)] = line[i];
     }
 }
 
