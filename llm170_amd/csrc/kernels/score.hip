@@ -2,8 +2,11 @@
 // tokens with theirs.  One pass over the row with a running maximum:
 //   S = sum 2^(z L - r),  U = sum (z L - r) 2^(z L - r),  L = log2 e, r = fl(max z * L), each term one fused multiply-add;
 //   log p_j = ln 2 * ((z_j L - r) - log2 S),  entropy = ln 2 * (log2 S - U / S).
-// r is the same rounded number in every term, so its rounding cancels; where z L could leave f32 (beyond 1e38: the lowest value of a
-// type as a mask) the difference is taken before the factor.  A row that holds NaN or +infinity has NaN for all its
+// r is the same rounded number in every term: what its rounding (half a last place of m L, m the largest z so far) puts on an exponent is on all
+// of them, and cancels.  That holds while it is far below one; from |m| = 2^20 on (2^-4 there; 128 and more from 2^31 on, where the largest power
+// leaves f32) the difference is taken before the factor, (z - m) L, and where z L itself could leave f32 (beyond 1e38: the lowest value of a type as a
+// mask) the exponent is held at -200.  Lanes of either kind meet where finite masks leave some lanes nothing else: a joining needs the distance of
+// their references, which one fused multiply-add gives.  A row that holds NaN or +infinity has NaN for all its
 // numbers; a row of -infinity alone gives its tokens -infinity and the entropy 0.
 //
 // The best tokens: an element is the key (order-preserving image of its value << 32 | ~index), so that no two are alike and equal
@@ -31,13 +34,25 @@
 typedef unsigned long long key_t_;
 
 struct ScoreStats {
-    float m, s, u;  // largest logit, S and U relative to fl(m * L)
+    float m, s, u;  // largest logit, S and U relative to score_ref(m)
 };
 
-__device__ __forceinline__ float score_ref(float m) { return m * 1.44269504088896341f; }
-#define SCORE_BIG 1e38f
-// ref(a) - ref(b) for a <= b; numbers so large that ref overflows are either equal or worlds apart
-__device__ __forceinline__ float score_ref_diff(float a, float b) { return a == b ? 0.f : __builtin_fmaxf(score_ref(a) - score_ref(b), -1e30f); }
+#define SCORE_LOG2E 1.44269504088896341f
+#define SCORE_BIG 1048576.0f  // maxima from here on are taken off before the factor
+#define SCORE_FAR 1e38f       // their product with the factor could leave f32
+// A term of z is 2^((z - c) L - r); one of c and r is 0.  NaN and the infinities count as big.
+struct ScoreRef {
+    float c, r;
+};
+__device__ __forceinline__ ScoreRef score_ref(float m) {
+    const bool big = !(__builtin_fabsf(m) < SCORE_BIG);
+    return {big ? m : 0.f, big ? 0.f : m * SCORE_LOG2E};
+}
+// What the powers relative to a's reference are multiplied with, as an exponent, to be relative to b's; a <= b
+__device__ __forceinline__ float score_ref_diff(float a, float b) {
+    const ScoreRef ra = score_ref(a), rb = score_ref(b);
+    return a == b ? 0.f : __builtin_fmaxf(__builtin_fmaf(ra.c - rb.c, SCORE_LOG2E, ra.r - rb.r), -1e30f);
+}
 __device__ __forceinline__ float score_exp2(float d) { return __builtin_amdgcn_exp2f(d); }
 
 // Sums relative to one maximum, re-expressed relative to a larger one and added.  -infinity: nothing there yet.
@@ -218,10 +233,10 @@ struct ScoreChunk {
     }
     // value(e) * L - r, one rounding; an f16 enters the multiply-add as it is
     __device__ __forceinline__ float scaled(int e, float r) const {
-        if (T != Q8_F16) return __builtin_fmaf(value(e), 1.44269504088896341f, -r);
+        if (T != Q8_F16) return __builtin_fmaf(value(e), SCORE_LOG2E, -r);
         float d;
         const unsigned h = w[e / PER][e % PER / 2];
-        const float l = 1.44269504088896341f;
+        const float l = SCORE_LOG2E;
         if (e & 1) asm("v_fma_mix_f32 %0, %1, %2, -%3 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(d) : "v"(h), "s"(l), "v"(r));
         else asm("v_fma_mix_f32 %0, %1, %2, -%3 op_sel_hi:[1,0,0]" : "=v"(d) : "v"(h), "s"(l), "v"(r));
         return d;
@@ -303,15 +318,12 @@ __device__ __forceinline__ void score_body(const void* __restrict__ logits, size
                 st.s *= g;
                 st.m = m;
             }
-            const float mm = st.m == -__builtin_inff() ? 0.f : st.m, r = score_ref(mm);  // nothing so far: every element is -infinity
-            const bool big = !(__builtin_fabsf(mm) < SCORE_BIG);
-            if (__any(big || !(least > -SCORE_BIG))) {
+            const ScoreRef rel = score_ref(st.m == -__builtin_inff() ? 0.f : st.m);  // nothing so far: every element is -infinity
+            if (__any(rel.c != 0.f || !(least > -SCORE_FAR))) {
 #pragma unroll
                 for (int e = 0; e < E; e++) {
-                    const float v = cur.value(e);
                     // -infinity (masked, or none at all) becomes a term whose power is 0, and stays out of U
-                    const float d = __builtin_fmaxf(big ? (v - mm) * 1.44269504088896341f : __builtin_fmaf(v, 1.44269504088896341f, -r), -200.f),
-                                p = score_exp2(d);
+                    const float d = __builtin_fmaxf(__builtin_fmaf(cur.value(e) - rel.c, SCORE_LOG2E, -rel.r), -200.f), p = score_exp2(d);
                     st.s += p;
                     st.u = __builtin_fmaf(d, p, st.u);
                     if (e % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // not all terms' registers at once
@@ -319,7 +331,7 @@ __device__ __forceinline__ void score_body(const void* __restrict__ logits, size
             } else {
 #pragma unroll
                 for (int e = 0; e < E; e++) {
-                    const float d = cur.scaled(e, r), p = score_exp2(d);
+                    const float d = cur.scaled(e, rel.r), p = score_exp2(d);
                     st.s += p;
                     st.u = __builtin_fmaf(d, p, st.u);
                 }
@@ -454,12 +466,13 @@ __device__ __forceinline__ void score_body(const void* __restrict__ logits, size
     }
     if (wave != 0) return;
     const bool none = st.m == -__builtin_inff(), bad = !(st.m < __builtin_inff());
-    const float log_s = __builtin_amdgcn_logf(st.s), r = score_ref(st.m);  // base 2
+    const float log_s = __builtin_amdgcn_logf(st.s);  // base 2
+    const ScoreRef rel = score_ref(st.m);
     auto log_p = [&](float v) {
         if (bad) return __builtin_nanf("");
         if (none) return -__builtin_inff();
-        if (!(__builtin_fabsf(v) < SCORE_BIG) || !(__builtin_fabsf(st.m) < SCORE_BIG)) return (v - st.m) - log_s * 0.693147180559945309f;
-        return (__builtin_fmaf(v, 1.44269504088896341f, -r) - log_s) * 0.693147180559945309f;
+        if (!(__builtin_fabsf(v) < SCORE_FAR) || rel.c != 0.f) return (v - st.m) - log_s * 0.693147180559945309f;
+        return (__builtin_fmaf(v, SCORE_LOG2E, -rel.r) - log_s) * 0.693147180559945309f;
     };
     if (lane == 0) {
         if (entropy) entropy[row] = bad ? __builtin_nanf("") : none ? 0.f : __builtin_fmaxf((log_s - st.u / st.s) * 0.693147180559945309f, 0.f);

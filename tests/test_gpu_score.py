@@ -122,6 +122,47 @@ def test_masks_ties_and_what_is_no_number(dec, v, kind):
             check(one, z[i:i + 1], targets[i:i + 1], top)
 
 
+@pytest.mark.parametrize("kind", [ffi.F32, ffi.BF16])
+@pytest.mark.parametrize("v", [40, 5000, 20000])
+def test_finite_masks_and_logits_of_any_size(dec, v, kind):
+    """Masks far below the logits that are not the type's lowest value, and logits where a step of the type passes one: every magnitude up to 3e38.
+    The differences of such logits are rounded once more, |z - max| p u in the mean over the terms, less than one; the joins, of which there are at most
+    20 levels, leave room for it."""
+    r = np.random.default_rng(v + 1)
+    base = (r.standard_normal(v) * 2).astype(np.float32)
+    few = r.permutation(v)[:20]
+    rows = []
+    for mask in (-2e6, -1e8, -1e9, -2e9, -1e10, -1e12, -1e20, -1e30, -5e37, -2e38):
+        z = np.full(v, mask, np.float32)
+        rows.append(z.copy())            # nothing is left
+        z[few] = base[few]
+        rows.append(z.copy())            # twenty tokens are
+        z = base.copy()
+        z[:v // 2] = mask
+        rows.append(z)                   # whole stretches are masked
+    for top in (1e6, 3e7, 1e9, 1.45e9, 5e9, 1e12, 1e30, 3e38):
+        z = base.copy()
+        z[v // 3] = top
+        rows.append(z)                   # one token has it all
+        rows.append(np.where(np.arange(v) % 3 == 0, np.float32(top), base))
+        for sign in (1, -1):             # steps of the type apart, around the size
+            rows.append(np.float32(sign * top) + np.float32(np.spacing(np.float32(top))) * np.rint(base))
+    for size in (2.0**19, 2.0**20, 2.0**21, 2.0**23, 2.0**30):
+        for sign in (1, -1):             # on both sides of a power of two, in one row
+            rows.append((np.float64(sign * size) + base).astype(np.float32))
+    rows.append((base * 1e36).astype(np.float32))
+    bits, z = ref.narrow(np.stack(rows).astype(np.float32), kind)
+    assert np.isfinite(z).all()
+    t = len(rows)
+    targets = np.where(np.arange(t) % 2 == 0, few[0], (np.arange(t) * 7919) % v)
+    for top in (0, 20):
+        with ref.Buffers(dec.cc) as b:
+            got = call(dec, b, bits, t, v, kind, targets, top)
+            check(got, z, targets, top)
+    for i in (0, 1, 2, 13, 14, 31, 40, t - 1):  # alone: segments and their records
+        with ref.Buffers(dec.cc) as b:
+            check(call(dec, b, bits[i:i + 1], 1, v, kind, targets[i:i + 1], 20), z[i:i + 1], targets[i:i + 1], 20)
+
 @pytest.mark.parametrize("kind,off,ld", [(ffi.F16, 2, 5003), (ffi.BF16, 6, 5010), (ffi.F32, 4, 5001), (ffi.F16, 14, 6000)])
 def test_any_alignment_and_stride(dec, kind, off, ld):
     t, v, top = 9, 5000, 20
