@@ -66,7 +66,8 @@ int w4a16_module_load(w4a16_ctx* ctx, const char* key, const void* image, size_t
 /* CudaCtx::function (ctx/mod.rs:262-267): 0 if `symbol` is resolved, W4A16_ERR_SYMBOL otherwise. */
 int w4a16_has_symbol(w4a16_ctx* ctx, const char* symbol);
 /* CudaCtx::launch / launch_shared (ctx/mod.rs:270-363): hipModuleLaunchKernel(f, gx,gy,1, block,1,1, shmem,
- * launch stream, params, NULL); params is an array of pointers to the argument values (args.rs:4-31). */
+ * launch stream, params, NULL); params is an array of pointers to the argument values (args.rs:4-31).  gx * block stays
+ * below 2^32 (W4A16_ERR_SHAPE), here and in every call that launches: HIP would run a part of such a grid and report nothing. */
 int w4a16_launch(w4a16_ctx* ctx, const char* symbol, unsigned gx, unsigned gy, unsigned block, unsigned shmem,
                  void** params);
 

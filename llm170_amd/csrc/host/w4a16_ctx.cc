@@ -280,6 +280,9 @@ int w4_launch(w4a16_ctx* ctx, const char* symbol, unsigned gx, unsigned gy, unsi
     if (it == ctx->functions.end()) return w4_fail(W4A16_ERR_SYMBOL, "function: symbol %s is not loaded", symbol);
     if (gx == 0 || gy == 0 || block == 0 || block > 1024)
         return w4_fail(W4A16_ERR_ARG, "launch %s: grid %ux%u block %u", symbol, gx, gy, block);
+    // HIP counts a dimension's threads in 32 bits and runs what is left of them without an error
+    if ((uint64_t)gx * block > 0xffffffffu)
+        return w4_fail(W4A16_ERR_SHAPE, "launch %s: %u workgroups of %u threads are 2^32 threads or more", symbol, gx, block);
     hipError_t e = hipSuccess;
     if (shmem > 64 * 1024) {  // beyond the default limit on dynamic LDS the function has to be told (gfx950: 160 KiB)
         if (shmem > 160 * 1024) return w4_fail(W4A16_ERR_ARG, "launch %s: %u bytes of LDS", symbol, shmem);
