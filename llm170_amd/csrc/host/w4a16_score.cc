@@ -46,7 +46,16 @@ extern "C" int w4a16_token_logprobs(w4a16_ctx* ctx, uint64_t logits_dev, int log
     }
     uint64_t ws = ctx->score_ws, tickets = ctx->score_tickets;
     int v = (int)n_vocab, top = (int)top_k, sg = (int)segs, sl = (int)std::min<size_t>(seg_len, 0x7fffffff);
-    void* params[] = {&logits_dev, &ld, &v, &targets_dev, &logp_dev, &entropy_dev, &top, &top_idx_dev, &top_logp_dev, &sg, &sl, &ws, &tickets};
     const char* sym = logits_type == W4A16_F32 ? "w4a16_token_logprobs_f32" : logits_type == W4A16_F16 ? "w4a16_token_logprobs_f16" : "w4a16_token_logprobs_bf16";
-    return w4_launch(ctx, sym, (unsigned)(t * segs), 1, 256, 0, params);
+    // HIP takes fewer than 2^32 threads in a launch: more rows go in several.  Rows in segments are fewer than 1024.
+    const size_t most = 0xffffffu;
+    for (size_t at = 0; at < t; at += most) {
+        const size_t rows = std::min(most, t - at);
+        auto from = [&](uint64_t p, size_t bytes) { return p ? p + at * bytes : 0; };
+        uint64_t z = logits_dev + at * ld * (logits_type == W4A16_F32 ? 4 : 2), tg = from(targets_dev, 4), lp = from(logp_dev, 4), en = from(entropy_dev, 4),
+                 ti = from(top_idx_dev, top_k * 4), tl = from(top_logp_dev, top_k * 4);
+        void* params[] = {&z, &ld, &v, &tg, &lp, &en, &top, &ti, &tl, &sg, &sl, &ws, &tickets};
+        W4_TRY(w4_launch(ctx, sym, (unsigned)(rows * segs), 1, 256, 0, params));
+    }
+    return 0;
 }

@@ -31,6 +31,10 @@ extern "C" size_t w4a16_q8_bytes(size_t t, size_t k) {
     return (t + r - 1) / r * r * k_tiles(k) * 64;
 }
 
+// Rows of a launch with a workgroup of `block` threads each: HIP takes fewer than 2^32 threads.  More rows go in several launches, of whole
+// tiles and, for the rows' order over the XCDs, of 128.
+static size_t rows_per_launch(unsigned block) { return 0xffffffffu / block / 128 * 128; }
+
 static int quant_rows(w4a16_ctx* ctx, uint64_t x, int x_type, size_t ldx, size_t t, size_t k, uint64_t q, uint64_t s) {
     char sym[64];
     // Few rows: a thread per four columns; else one per sixteen, of at most 768 (300 x 17408 f16 10.1 us with 1024, 8.2; 4096 rows 65 and 52)
@@ -38,10 +42,16 @@ static int quant_rows(w4a16_ctx* ctx, uint64_t x, int x_type, size_t ldx, size_t
     snprintf(sym, sizeof sym, "w4a16_quant_%s_%s", few ? "few" : "rows", type_name(x_type));
     const int r = (int)tile_rows(t);
     const unsigned block = (unsigned)std::min<size_t>(few ? (k + 255) / 256 * 64 : (k + 1023) / 1024 * 64, few ? 1024 : 768);
-    const unsigned grid = few ? (unsigned)t : ceil_div(t, 128) * 128;
-    int ki = (int)k, kt = (int)k_tiles(k), ri = r, ti = (int)t, bi = (int)block;
-    void* params[] = {&x, &ldx, &ki, &kt, &ri, &q, &s, &ti, &bi};
-    return w4_launch(ctx, sym, grid, few ? ceil_div(k, block * 4) : 1, block, 0, params);
+    int ki = (int)k, kt = (int)k_tiles(k), ri = r, bi = (int)block;
+    const size_t most = rows_per_launch(block);
+    for (size_t at = 0; at < t; at += most) {
+        const size_t rows = std::min(most, t - at);
+        uint64_t x_at = x + at * ldx * type_bytes(x_type), q_at = q + at * kt * 64, s_at = s + at * 4;
+        int ti = (int)rows;
+        void* params[] = {&x_at, &ldx, &ki, &kt, &ri, &q_at, &s_at, &ti, &bi};
+        W4_TRY(w4_launch(ctx, sym, few ? (unsigned)rows : ceil_div(rows, 128) * 128, few ? ceil_div(k, block * 4) : 1, block, 0, params));
+    }
+    return 0;
 }
 
 extern "C" int w4a16_quant_rows(w4a16_ctx* ctx, uint64_t x_dev, int x_type, size_t ldx, size_t t, size_t k, uint64_t q_dev, uint64_t s_dev) {
@@ -65,9 +75,16 @@ extern "C" int w4a16_norm_resid_q8(w4a16_ctx* ctx, uint64_t x_dev, uint64_t nw_d
     if (x_dev % 4 || nw_dev % 4 || ab_dev % 4 || s_dev % 4 || q_dev % 16)
         return w4_fail(W4A16_ERR_ARG, "norm_resid_q8: f32 operands must be aligned to 4 bytes, q to 16");
     W4_TRY(w4_hip(hipSetDevice(ctx->device), "hipSetDevice"));
-    int wo = (int)w_off, h = (int)hidden, kt = (int)k_tiles(hidden), r = (int)tile_rows(t), ti = (int)t;
-    void* params[] = {&x_dev, &nw_dev, &ab_dev, &q_dev, &s_dev, &wo, &h, &kt, &r, &ti};
-    return w4_launch(ctx, "w4a16_norm_resid_q8", r == 16 ? ceil_div(t, 128) * 128 : (unsigned)t, 1, 1024, 0, params);
+    int wo = (int)w_off, h = (int)hidden, kt = (int)k_tiles(hidden), r = (int)tile_rows(t);
+    const size_t most = rows_per_launch(1024);
+    for (size_t at = 0; at < t; at += most) {
+        const size_t rows = std::min(most, t - at);
+        uint64_t x_at = x_dev + at * hidden * 4, ab_at = ab_dev + at * hidden * 4, q_at = q_dev + at * kt * 64, s_at = s_dev + at * 4;
+        int ti = (int)rows;
+        void* params[] = {&x_at, &nw_dev, &ab_at, &q_at, &s_at, &wo, &h, &kt, &r, &ti};
+        W4_TRY(w4_launch(ctx, "w4a16_norm_resid_q8", r == 16 ? ceil_div(rows, 128) * 128 : (unsigned)rows, 1, 1024, 0, params));
+    }
+    return 0;
 }
 
 // ------------------------------------------------------------------------------------------------ registration
@@ -266,7 +283,7 @@ static TiledPlan plan_tiled(size_t n, size_t k, size_t t, size_t cus) {
 static int launch_tiled(w4a16_ctx* ctx, const W8Lin& L, const TiledPlan& P, uint64_t q, uint64_t s, size_t t, uint64_t y, int y_type, int act) {
     const bool glu = act >= 0;
     const size_t tiles = (t + P.bm - 1) / P.bm * ((L.n + P.bn - 1) / P.bn), nks = (size_t)P.nks;
-    if (tiles * nks > 0x7ffffff0u) return w4_fail(W4A16_ERR_SHAPE, "lin_w8a8: t=%zu n=%zu exceed the grid", t, L.n);
+    if (tiles * nks > 0xfffff8u) return w4_fail(W4A16_ERR_SHAPE, "lin_w8a8: t=%zu n=%zu exceed the grid", t, L.n);
     if (nks > 1) W4_TRY(split_workspace(ctx, tiles * nks * P.bm * P.bn * 4, tiles));
     uint64_t wt = L.q, ws = L.s, part = ctx->w8_part, tickets = ctx->w8_tickets;
     // 1024 rows of tiles share their weights in the L2: 34816 x 5120 gated at t = 4096 673 us in an earlier state, 512 rows 679, 256 rows 727
