@@ -523,8 +523,8 @@ int w4a16_upload_lin_w8a8(w4a16_ctx* ctx, const char* name, const void* q, size_
 int w4a16_lin_w8a8_info(w4a16_ctx* ctx, const char* name, size_t* n, size_t* k);
 
 /* Bytes of a buffer for t quantised rows of k (0 where no such rows exist).  The rows lie in tiles: with R = 1 (t == 1), 4 (t <= 4)
- * or 16, element (m, j) is byte ((m / R * K + j / 16) * R + m % R) * 16 + j % 16, K = 8 * ceil(k / 128).  Bytes of no
- * element are left as they are, and never matter. */
+ * or 16, element (m, j) is byte ((m / R * K + j / 16) * R + m % R) * 16 + j % 16, K = 8 * ceil(k / 128).  The calls that write
+ * rows fill a row's last 16 bytes up with zeros; other bytes of no element are left as they are, and none of them matter. */
 size_t w4a16_q8_bytes(size_t t, size_t k);
 /* x (f32, f16 or bf16, rows ldx elements apart, 0 = k) -> q (w4a16_q8_bytes(t, k) bytes, 16-byte aligned) and s f32 [t]. */
 int w4a16_quant_rows(w4a16_ctx* ctx, uint64_t x_dev, int x_type, size_t ldx, size_t t, size_t k, uint64_t q_dev, uint64_t s_dev);

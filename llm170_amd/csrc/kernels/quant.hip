@@ -218,12 +218,8 @@ extern "C" __global__ __launch_bounds__(1024) void w4a16_norm_resid_q8(float* __
 #pragma unroll
     for (int j = 0; j < 8; j++) line[j * 1024 + tid] = (char)(o[j / 4] >> (8 * (j % 4)));
     __syncthreads();
-    const int c = tid * 16;  // whole chunks, of the last one the bytes that there are
-    if (c + 16 <= hidden) {
-        *reinterpret_cast<u4_t*>(q + q8_chunk_at(row, tid, kt, R)) = *reinterpret_cast<const u4_t*>(line + c);
-    } else {
-        for (int i = c; i < hidden; i++) q[q8_chunk_at(row, tid, kt, R) + (i & 15)] = line[i];
-    }
+    // whole chunks: behind the row's end v and y, and so the bytes, are 0
+    if (tid * 16 < hidden) *reinterpret_cast<u4_t*>(q + q8_chunk_at(row, tid, kt, R)) = *reinterpret_cast<const u4_t*>(line + tid * 16);
 }
 
 // Weights int8 [n][k] -> tiles [row_blocks][kt], zeros behind n and k: a thread per 16-byte chunk of the result.

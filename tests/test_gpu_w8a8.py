@@ -134,6 +134,26 @@ def test_norm_resid_q8_is_norm_resid_and_quant_rows(dec, t, hidden, w_off):
         assert (np.abs(qb * sb[:, None].astype(np.float64) - want) <= sb[:, None] * 0.5001).all()
 
 
+@pytest.mark.parametrize("t,hidden", [(1, 7), (3, 100), (18, 1000), (5, 8185), (2, 16)])
+def test_both_ways_to_quantised_rows_write_the_same_bytes(dec, t, hidden):
+    """Of the whole buffer: elements, zeros behind a row's end inside its last 16 bytes, and the bytes that neither touches; a row of no number among them."""
+    r = np.random.default_rng(hidden)
+    x, ab, nw = (r.standard_normal(n).astype(np.float32) for n in ((t, hidden), (t, hidden), hidden))
+    if t > 1:
+        x[1, 3] = np.nan
+    cc, n = dec.cc, ops.q8_bytes(t, hidden)
+    with ref.Buffers(cc) as b:
+        x1, x2, dab, dnw, xn, s2, q2 = b.put(x), b.put(x), b.put(ab), b.put(nw), b.filled(t * hidden * 4), b.filled(t * 4), b.filled(n)
+        dec.norm_resid(x1, dnw, dab, xn, t, hidden)
+        q1, _ = run_quant(dec, b, xn, t, hidden, ffi.F32)
+        dec.norm_resid_q8(x2, dnw, dab, q2, s2, t, hidden)
+        first, second = cc.d2h(q1, (n,), np.uint8), cc.d2h(q2, (n,), np.uint8)
+    assert np.array_equal(first, second)
+    place = np.arange(n).reshape(-1, -(-hidden // 128) * 8, 1 if t == 1 else 4 if t <= 4 else 16, 16).transpose(0, 2, 1, 3).reshape(-1, -(-hidden // 128) * 128)
+    whole = -(-hidden // 16) * 16
+    assert not first[place[:t, hidden:whole]].any() and (first[place[:t, whole:]] == 0xA5).all() and (first[place[t:]] == 0xA5).all()
+
+
 def test_norm_resid_q8_of_infinity(dec):
     t, h = 3, 256
     x, ab, nw = np.ones((t, h), np.float32), np.ones((t, h), np.float32), np.ones(h, np.float32)
