@@ -541,6 +541,11 @@ int w4a16_lin_forward_w8a8(w4a16_ctx* ctx, const char* name, uint64_t x_dev, int
  * values of w4a16_lin_forward_w8a8, rounded once to y's type.  act: W4A16_ACT_SILU or W4A16_ACT_GELU_TANH. */
 int w4a16_lin_forward_w8a8_glu(w4a16_ctx* ctx, const char* name, uint64_t x_dev, int x_type, size_t ldx, uint64_t xs_dev, size_t t,
                                uint64_t y_dev, int y_type, int act);
+/* The launch that t rows through a W8A8 linear go to on a GPU of `cu_count` compute units: the kernel's name (`cap` bytes, at least 64),
+ * workgroups, waves of each, and slices of k that are handed over between them.  W4A16_ERR_SHAPE where the launch would hold 2^32 threads.  Needs
+ * neither a context nor a GPU.  Out pointers may be NULL. */
+int w4a16_plan_w8a8(size_t n, size_t k, size_t t, int cu_count, int glu, char* kernel, size_t cap, size_t* workgroups, int* waves,
+                    int* k_slices);
 
 /* Scores rows of logits z [t][n_vocab] (f32, f16 or bf16, rows ld elements apart, 0 = n_vocab); results of no interest are 0.
  *   targets int32 [t], logp f32 [t]: log softmax(z)[target]; 0 for a negative target (none is asked for), NaN for one >= n_vocab;

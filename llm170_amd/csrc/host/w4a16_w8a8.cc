@@ -230,21 +230,6 @@ static int split_workspace(w4a16_ctx* ctx, size_t part_bytes, size_t tickets) {
     return 0;
 }
 
-static int launch_skinny(w4a16_ctx* ctx, const W8Lin& L, const SkinnyPlan& P, uint64_t q, uint64_t s, size_t t, uint64_t y, int y_type, int act) {
-    const bool glu = act >= 0;
-    const size_t groups = (t + 63) / 64;  // of as many rows each as can be
-    const int tt = (int)((t + 16 * groups - 1) / (16 * groups));
-    const size_t kt = k_tiles(L.k), blocks16 = (L.n + 15) / 16;
-    char sym[64];
-    snprintf(sym, sizeof sym, "w4a16_w8a8_skinny_r%d_t%d%s", P.rb, tt, glu ? "_glu" : "");
-    const unsigned grid = glu ? ceil_div(blocks16 / 2, P.rb / 2) : ceil_div(blocks16, P.rb);
-    if (P.nks > 1) W4_TRY(split_workspace(ctx, (size_t)grid * groups * P.nks * P.rb * tt * 1024, grid * groups));
-    uint64_t wt = L.q, ws = L.s, part = ctx->w8_part, tickets = ctx->w8_tickets;
-    int ni = (int)L.n, kti = (int)kt, ti = (int)t, r = (int)tile_rows(t), wi = P.waves, ksi = P.nks;
-    void* params[] = {&wt, &ws, &q, &s, &y, &ni, &kti, &ti, &r, &y_type, &act, &wi, &ksi, &part, &tickets};
-    return w4_launch(ctx, sym, grid, (unsigned)(P.nks * groups), (unsigned)P.waves * 64, 0, params);
-}
-
 // Launch of the tiled kernel: rows and columns (of weights) per tile, k slices; a function of the shape alone.
 struct TiledPlan {
     int bm = 64, bn = 128, nks = 1;
@@ -280,18 +265,63 @@ static TiledPlan plan_tiled(size_t n, size_t k, size_t t, size_t cus) {
     return best;
 }
 
-static int launch_tiled(w4a16_ctx* ctx, const W8Lin& L, const TiledPlan& P, uint64_t q, uint64_t s, size_t t, uint64_t y, int y_type, int act) {
-    const bool glu = act >= 0;
-    const size_t tiles = (t + P.bm - 1) / P.bm * ((L.n + P.bn - 1) / P.bn), nks = (size_t)P.nks;
-    if (tiles * nks > 0xfffff8u) return w4_fail(W4A16_ERR_SHAPE, "lin_w8a8: t=%zu n=%zu exceed the grid", t, L.n);
-    if (nks > 1) W4_TRY(split_workspace(ctx, tiles * nks * P.bm * P.bn * 4, tiles));
+// The kernel that t rows through a linear go to, its grid, and the scratch of its k slices
+struct W8Launch {
+    char kernel[64] = "";
+    size_t grid_x = 0, grid_y = 1, tickets = 0, part_bytes = 0;
+    int block = 256, nks = 1, band = 0;  // band: tile rows of a band, 0 = the kernel for groups of up to 64 rows
+};
+
+static int plan_w8a8(const char* what, size_t n, size_t k, size_t t, size_t cus, bool glu, W8Launch* out) {
+    W8Launch& P = *out;
+    const SkinnyPlan few = plan_skinny(n, k, t, cus, glu);
+    const TiledPlan tiles = t <= 64 ? TiledPlan() : plan_tiled(n, k, t, cus);
+    if (t <= 64 || (t <= 1024 && few.price < tiles.price)) {
+        const size_t groups = (t + 63) / 64;  // of as many rows each as can be
+        const int tt = (int)((t + 16 * groups - 1) / (16 * groups));
+        const size_t blocks16 = (n + 15) / 16;
+        snprintf(P.kernel, sizeof P.kernel, "w4a16_w8a8_skinny_r%d_t%d%s", few.rb, tt, glu ? "_glu" : "");
+        P.nks = few.nks;
+        P.grid_x = glu ? ceil_div(blocks16 / 2, few.rb / 2) : ceil_div(blocks16, few.rb);
+        P.grid_y = few.nks * groups;
+        P.block = few.waves * 64;
+        P.tickets = P.grid_x * groups;
+        P.part_bytes = P.tickets * few.nks * few.rb * tt * 1024;
+    } else {
+        snprintf(P.kernel, sizeof P.kernel, "w4a16_w8a8_tiled_m%d%s%s", tiles.bm, tiles.bn == 128 ? "_n128" : "", glu ? "_glu" : "");
+        P.nks = tiles.nks;
+        P.tickets = (t + tiles.bm - 1) / tiles.bm * ((n + tiles.bn - 1) / tiles.bn);
+        P.part_bytes = P.tickets * tiles.nks * tiles.bm * tiles.bn * 4;
+        P.grid_x = (P.tickets * tiles.nks + 7) / 8 * 8;
+        // 1024 rows of tiles share their weights in the L2: 34816 x 5120 gated at t = 4096 673 us in an earlier state, 512 rows 679, 256 rows 727
+        P.band = 1024 / tiles.bm;
+    }
+    if (P.grid_x * P.block > 0xffffffffu) return w4_fail(W4A16_ERR_SHAPE, "%s: t=%zu n=%zu exceed the grid", what, t, n);
+    return 0;
+}
+
+extern "C" int w4a16_plan_w8a8(size_t n, size_t k, size_t t, int cu_count, int glu, char* kernel, size_t cap, size_t* workgroups, int* waves, int* k_slices) {
+    if (cu_count <= 0 || (kernel && cap < sizeof(W8Launch::kernel)))
+        return w4_fail(W4A16_ERR_ARG, "plan_w8a8: cus=%d, %zu bytes for a name of up to %zu", cu_count, cap, sizeof(W8Launch::kernel));
+    W4_TRY(check_rows("plan_w8a8", t, k));
+    if (n == 0 || n > 0x7fffff00u || (glu && n % 32 != 0))
+        return w4_fail(W4A16_ERR_SHAPE, "plan_w8a8: n=%zu outside 1..2^31-256, or gated and no multiple of 32", n);
+    W8Launch P;
+    W4_TRY(plan_w8a8("plan_w8a8", n, k, t, (size_t)cu_count, glu != 0, &P));
+    if (kernel) memcpy(kernel, P.kernel, sizeof P.kernel);
+    if (workgroups) *workgroups = P.grid_x * P.grid_y;
+    if (waves) *waves = P.block / 64;
+    if (k_slices) *k_slices = P.nks;
+    return 0;
+}
+
+static int launch_w8a8(w4a16_ctx* ctx, const W8Lin& L, const W8Launch& P, uint64_t q, uint64_t s, size_t t, uint64_t y, int y_type, int act) {
+    if (P.nks > 1) W4_TRY(split_workspace(ctx, P.part_bytes, P.tickets));
     uint64_t wt = L.q, ws = L.s, part = ctx->w8_part, tickets = ctx->w8_tickets;
-    // 1024 rows of tiles share their weights in the L2: 34816 x 5120 gated at t = 4096 673 us in an earlier state, 512 rows 679, 256 rows 727
-    int ni = (int)L.n, kti = (int)k_tiles(L.k), ti = (int)t, ki = P.nks, band = 1024 / P.bm;
-    char sym[64];
-    snprintf(sym, sizeof sym, "w4a16_w8a8_tiled_m%d%s%s", P.bm, P.bn == 128 ? "_n128" : "", glu ? "_glu" : "");
-    void* params[] = {&wt, &ws, &q, &s, &y, &ni, &kti, &ti, &y_type, &act, &ki, &band, &part, &tickets};
-    return w4_launch(ctx, sym, (unsigned)((tiles * nks + 7) / 8 * 8), 1, 256, 0, params);
+    int ni = (int)L.n, kti = (int)k_tiles(L.k), ti = (int)t, r = (int)tile_rows(t), wi = P.block / 64, ksi = P.nks, band = P.band;
+    void* few[] = {&wt, &ws, &q, &s, &y, &ni, &kti, &ti, &r, &y_type, &act, &wi, &ksi, &part, &tickets};
+    void* tiles[] = {&wt, &ws, &q, &s, &y, &ni, &kti, &ti, &y_type, &act, &ksi, &band, &part, &tickets};
+    return w4_launch(ctx, P.kernel, (unsigned)P.grid_x, (unsigned)P.grid_y, (unsigned)P.block, 0, P.band ? tiles : few);
 }
 
 static int forward_w8a8(w4a16_ctx* ctx, const char* api, const char* name, uint64_t x, int x_type, size_t ldx, uint64_t xs, size_t t, uint64_t y,
@@ -313,6 +343,8 @@ static int forward_w8a8(w4a16_ctx* ctx, const char* api, const char* name, uint6
     }
     if (y % type_bytes(y_type) || x % (x_type == W4A16_Q8 ? 16 : type_bytes(x_type)) || xs % 4)
         return w4_fail(W4A16_ERR_ARG, "%s %s: operands must be aligned to their elements, quantised rows to 16 bytes", api, name);
+    W8Launch P;
+    W4_TRY(plan_w8a8(api, L->n, L->k, t, (size_t)std::max(ctx->cu_count, 1), act >= 0, &P));
     W4_TRY(w4_hip(hipSetDevice(ctx->device), "hipSetDevice"));
     if (x_type != W4A16_Q8) {
         W4_TRY(w4_ensure(ctx, &ctx->q8, &ctx->q8_cap, w4a16_q8_bytes(t, L->k)));
@@ -321,12 +353,7 @@ static int forward_w8a8(w4a16_ctx* ctx, const char* api, const char* name, uint6
         x = ctx->q8;
         xs = ctx->q8_scales;
     }
-    const size_t cus = (size_t)std::max(ctx->cu_count, 1);
-    const SkinnyPlan few = plan_skinny(L->n, L->k, t, cus, act >= 0);
-    if (t <= 64) return launch_skinny(ctx, *L, few, x, xs, t, y, y_type, act);
-    const TiledPlan tiles = plan_tiled(L->n, L->k, t, cus);
-    if (t <= 1024 && few.price < tiles.price) return launch_skinny(ctx, *L, few, x, xs, t, y, y_type, act);
-    return launch_tiled(ctx, *L, tiles, x, xs, t, y, y_type, act);
+    return launch_w8a8(ctx, *L, P, x, xs, t, y, y_type, act);
 }
 
 extern "C" int w4a16_lin_forward_w8a8(w4a16_ctx* ctx, const char* name, uint64_t x_dev, int x_type, size_t ldx, uint64_t xs_dev, size_t t,

@@ -137,6 +137,8 @@ _SIGS = {
                                          C.c_int]),
     "w4a16_lin_forward_w8a8_glu": (C.c_int, [C.c_void_p, C.c_char_p, C.c_uint64, C.c_int, C.c_size_t, C.c_uint64, C.c_size_t, C.c_uint64,
                                              C.c_int, C.c_int]),
+    "w4a16_plan_w8a8": (C.c_int, [C.c_size_t, C.c_size_t, C.c_size_t, C.c_int, C.c_int, C.c_char_p, C.c_size_t, C.POINTER(C.c_size_t),
+                                  C.POINTER(C.c_int), C.POINTER(C.c_int)]),
     "w4a16_token_logprobs": (C.c_int, [C.c_void_p, C.c_uint64, C.c_int, C.c_size_t, C.c_size_t, C.c_size_t, C.c_uint64, C.c_uint64,
                                        C.c_uint64, C.c_size_t, C.c_uint64, C.c_uint64]),
     "w4a16_bench_moe": (C.c_int, [C.c_void_p, C.POINTER(C.c_char_p), C.c_size_t, C.c_uint64, C.c_uint64, C.c_uint64,

@@ -62,6 +62,13 @@ def plan_moe(t, top_k, n_experts, h, n_ff, group=32, scales=0, cu_count=256):
     return {"segment": seg.value, "gate_up": names[0].value.decode(), "down": names[1].value.decode()}
 
 
+def plan_w8a8(t, n, k, cu_count=256, glu=False):
+    """Launch of t rows through a W8A8 linear (no context, no GPU): dict of kernel, workgroups, waves, k_slices."""
+    name, wgs, waves, nks = C.create_string_buffer(64), C.c_size_t(), C.c_int(), C.c_int()
+    ffi.check(ffi.load().w4a16_plan_w8a8(n, k, t, cu_count, int(bool(glu)), name, 64, C.byref(wgs), C.byref(waves), C.byref(nks)))
+    return {"kernel": name.value.decode(), "workgroups": wgs.value, "waves": waves.value, "k_slices": nks.value}
+
+
 def check_shapes(t, qlen, slen, xlen, n, k, group):
     """gptq4.rs:31-58.  Raises W4a16Error(ERR_SHAPE) on violation."""
     ffi.check(ffi.load().w4a16_check_shapes(t, qlen, slen, xlen, n, k, group))

@@ -197,6 +197,65 @@ def test_linear_bit_for_bit(dec, t, n, k):
             assert (dec.cc.d2h(y + t * n * size, (64,), np.uint8) == 0xA5).all()  # nothing behind the last row
 
 
+def gated(dec, b, want, gelu):
+    """f16 bits of act(gate) * up of f32 products [t][n], by the separate kernel."""
+    t, n = want.shape
+    a = b.filled(t * n)
+    dec.act_mul_f16(b.put(want), n // 2, t, a, gelu=gelu)
+    return dec.cc.d2h(a, (t, n // 2), np.uint16)
+
+
+@pytest.mark.parametrize("t,n,k,glu,kernel,slices", ref.BUILDS)
+def test_every_build_bit_for_bit(dec, t, n, k, glu, kernel, slices):
+    say("build", t, n, k, glu, kernel, slices)
+    w, sb, sv = ref.weights(n * 5 + k, n, k)
+    bits, x = ref.narrow(np.random.default_rng(t + k).standard_normal((t, k)).astype(np.float32), ffi.F16)
+    dec.upload_lin_w8a8("b", w, sb, n, k)
+    want = ref.product(*ref.quantised(x), w, sv)
+    with ref.Buffers(dec.cc) as b:
+        dx, y = b.put(bits), b.filled(t * n * 4 + 64)
+        if glu:
+            for gelu in (False, True):
+                dec.lin_forward_w8a8_glu("b", dx, y, t, x_type=ffi.F16, y_type=ffi.F16, gelu=gelu)
+                assert dec.cc.last_launch_symbol() == "w4a16_w8a8_" + kernel
+                assert np.array_equal(dec.cc.d2h(y, (t, n // 2), np.uint16), gated(dec, b, want, gelu))
+            assert (dec.cc.d2h(y + t * n, (64,), np.uint8) == 0xA5).all()  # nothing behind the last row
+        else:
+            for y_type, size in ((ffi.F16, 2), (ffi.BF16, 2), (ffi.F32, 4)):
+                dec.lin_forward_w8a8("b", dx, y, t, x_type=ffi.F16, y_type=y_type)
+                assert dec.cc.last_launch_symbol() == "w4a16_w8a8_" + kernel
+                assert np.array_equal(dec.cc.d2h(y, (t, n), ref.bits_type(y_type)), ref.as_type(want, y_type)), y_type
+                assert size == 4 or y_type == ffi.BF16 or (dec.cc.d2h(y + t * n * size, (64,), np.uint8) == 0xA5).all()
+            assert (dec.cc.d2h(y + t * n * 4, (64,), np.uint8) == 0xA5).all()
+
+
+@pytest.mark.parametrize("t,n,k,glu,kernel", [(4, 131072, 5120, False, "skinny_r4_t1"), (8, 5120, 17408, False, "skinny_r4_t1"), (16, 5120, 17408, False, "skinny_r4_t1"),
+                                              (32, 34816, 5120, True, "skinny_r4_t2_glu"), (64, 34816, 5120, True, "skinny_r4_t4_glu"),
+                                              (300, 34816, 5120, True, "tiled_m128_glu"), (300, 5120, 17408, False, "tiled_m128")])
+def test_layers_and_a_head_of_full_size(dec, t, n, k, glu, kernel):
+    """What the wide layers and heads of a model launch, at 1000 of the outputs and the ends."""
+    say("layer", t, n, k, glu, kernel)
+    w, sb, sv = ref.weights(7, n, k)
+    bits, x = ref.narrow(np.random.default_rng(t).standard_normal((t, k)).astype(np.float32), ffi.F16)
+    dec.upload_lin_w8a8("layer", w, sb, n, k)
+    out = n // 2 if glu else n
+    at = np.unique(np.concatenate([[0, out - 1], np.random.default_rng(1).integers(0, out, 1000)]))
+    rows = np.concatenate([at, at + out]) if glu else at
+    want = ref.product(*ref.quantised(x), w[rows], sv[rows])
+    with ref.Buffers(dec.cc) as b:
+        dx, y = b.put(bits), b.filled(t * out * 4)
+        if glu:
+            dec.lin_forward_w8a8_glu("layer", dx, y, t, x_type=ffi.F16, y_type=ffi.F16)
+            ran = dec.cc.last_launch_symbol()
+            got, want = dec.cc.d2h(y, (t, out), np.uint16)[:, at], gated(dec, b, want, False)
+        else:
+            dec.lin_forward_w8a8("layer", dx, y, t, x_type=ffi.F16, y_type=ffi.F32)
+            ran = dec.cc.last_launch_symbol()
+            got, want = dec.cc.d2h(y, (t, out), np.uint32)[:, at], want.view(np.uint32)
+    assert ran == "w4a16_w8a8_" + kernel
+    assert np.array_equal(got, want)
+
+
 @pytest.mark.parametrize("t", [1, 3, 16, 40, 64, 65, 200])
 def test_linear_on_quantised_rows_and_on_rows_of_floats(dec, t):
     """The same rows through quant_rows and through the linear's own quantisation, with a stride, every type; several linears of one q."""

@@ -6,6 +6,43 @@ from llm170_amd import ffi, ops
 TYPES = {ffi.F32: np.float32, ffi.F16: np.float16}
 
 
+# One shape or more, of ragged sizes, for every kernel of kernels/w8a8.hip with whole k and with k in slices on 256 compute units: (rows, n, k, gated, kernel
+# behind "w4a16_w8a8_", slices)
+BUILDS = [
+    (1, 34, 152, False, "skinny_r1_t1", False), (2, 34, 151, False, "skinny_r1_t1", False), (5, 34, 154, False, "skinny_r1_t1", False),
+    (1, 33, 6839, False, "skinny_r1_t1", True), (2, 33, 6701, False, "skinny_r1_t1", True), (7, 33, 5054, False, "skinny_r1_t1", True),
+    (17, 34, 156, False, "skinny_r1_t2", False), (17, 34, 3849, False, "skinny_r1_t2", True), (33, 35, 152, False, "skinny_r1_t3", False),
+    (70, 34, 159, False, "skinny_r1_t3", False), (33, 33, 3317, False, "skinny_r1_t3", True), (66, 33, 1556, False, "skinny_r1_t3", True),
+    (50, 34, 154, False, "skinny_r1_t4", False), (99, 36, 151, False, "skinny_r1_t4", False), (50, 33, 2949, False, "skinny_r1_t4", True),
+    (105, 33, 1431, False, "skinny_r1_t4", True), (1, 4180, 160, False, "skinny_r2_t1", False), (2, 4121, 154, False, "skinny_r2_t1", False),
+    (5, 4220, 157, False, "skinny_r2_t1", False), (1, 1063, 8791, False, "skinny_r2_t1", True), (2, 1029, 8885, False, "skinny_r2_t1", True),
+    (5, 829, 6061, False, "skinny_r2_t1", True), (1, 32, 150, True, "skinny_r2_t1_glu", False), (2, 32, 150, True, "skinny_r2_t1_glu", False),
+    (5, 32, 150, True, "skinny_r2_t1_glu", False), (1, 32, 3591, True, "skinny_r2_t1_glu", True), (2, 32, 3590, True, "skinny_r2_t1_glu", True),
+    (5, 32, 3100, True, "skinny_r2_t1_glu", True), (17, 4194, 153, False, "skinny_r2_t2", False), (17, 895, 4496, False, "skinny_r2_t2", True),
+    (17, 32, 150, True, "skinny_r2_t2_glu", False), (17, 32, 2691, True, "skinny_r2_t2_glu", True), (33, 4243, 151, False, "skinny_r2_t3", False),
+    (76, 2077, 152, False, "skinny_r2_t3", False), (33, 823, 4015, False, "skinny_r2_t3", True), (76, 678, 2856, False, "skinny_r2_t3", True),
+    (33, 32, 151, True, "skinny_r2_t3_glu", False), (67, 32, 155, True, "skinny_r2_t3_glu", False), (33, 32, 2433, True, "skinny_r2_t3_glu", True),
+    (65, 32, 1430, True, "skinny_r2_t3_glu", True), (50, 4193, 151, False, "skinny_r2_t4", False), (390, 589, 150, False, "skinny_r2_t4", False),
+    (50, 839, 4227, False, "skinny_r2_t4", True), (206, 338, 3182, False, "skinny_r2_t4", True), (50, 32, 151, True, "skinny_r2_t4_glu", False),
+    (97, 32, 152, True, "skinny_r2_t4_glu", False), (50, 32, 2177, True, "skinny_r2_t4_glu", True), (97, 32, 1317, True, "skinny_r2_t4_glu", True),
+    (1, 12328, 153, False, "skinny_r4_t1", False), (2, 12201, 150, False, "skinny_r4_t1", False), (5, 12328, 152, False, "skinny_r4_t1", False),
+    (1, 4107, 10310, False, "skinny_r4_t1", True), (2, 4145, 9825, False, "skinny_r4_t1", True), (5, 1681, 8045, False, "skinny_r4_t1", True),
+    (1, 8800, 156, True, "skinny_r4_t1_glu", False), (2, 8672, 158, True, "skinny_r4_t1_glu", False), (5, 8224, 154, True, "skinny_r4_t1_glu", False),
+    (1, 2816, 5694, True, "skinny_r4_t1_glu", True), (2, 2752, 5836, True, "skinny_r4_t1_glu", True), (5, 1664, 4057, True, "skinny_r4_t1_glu", True),
+    (17, 8293, 153, False, "skinny_r4_t2", False), (17, 1649, 6201, False, "skinny_r4_t2", True), (17, 8704, 150, True, "skinny_r4_t2_glu", False),
+    (17, 2080, 3677, True, "skinny_r4_t2_glu", True), (33, 8231, 153, False, "skinny_r4_t3", False), (67, 4106, 162, False, "skinny_r4_t3", False),
+    (33, 2058, 5809, False, "skinny_r4_t3", True), (65, 1065, 7288, False, "skinny_r4_t3", True), (40, 8352, 151, True, "skinny_r4_t3_glu", False),
+    (66, 4320, 162, True, "skinny_r4_t3_glu", False), (33, 2080, 4795, True, "skinny_r4_t3_glu", True), (65, 1408, 4070, True, "skinny_r4_t3_glu", True),
+    (50, 8218, 156, False, "skinny_r4_t4", False), (196, 2089, 153, False, "skinny_r4_t4", False), (50, 2072, 5749, False, "skinny_r4_t4", True),
+    (909, 164, 6711, False, "skinny_r4_t4", True), (50, 8224, 153, True, "skinny_r4_t4_glu", False), (593, 832, 153, True, "skinny_r4_t4_glu", False),
+    (50, 2784, 3846, True, "skinny_r4_t4_glu", True), (203, 736, 5381, True, "skinny_r4_t4_glu", True), (66, 33153, 151, False, "tiled_m128", False),
+    (610, 3215, 4145, False, "tiled_m128", True), (773, 5056, 160, True, "tiled_m128_glu", False), (1240, 1568, 4321, True, "tiled_m128_glu", True),
+    (65, 16778, 152, False, "tiled_m64", False), (199, 4177, 3732, False, "tiled_m64", True), (661, 3008, 160, True, "tiled_m64_glu", False),
+    (66, 8224, 3748, True, "tiled_m64_glu", True), (1079, 34, 160, False, "tiled_m64_n128", False), (1029, 36, 961, False, "tiled_m64_n128", True),
+    (1044, 32, 152, True, "tiled_m64_n128_glu", False), (1034, 32, 913, True, "tiled_m64_n128_glu", True),
+]
+
+
 def to_bf16(v):
     """f32 -> bf16 bits, to nearest even (finite values)."""
     b = np.ascontiguousarray(v, np.float32).view(np.uint32).astype(np.uint64)
