@@ -211,7 +211,7 @@ static SkinnyPlan plan_skinny(size_t n, size_t k, size_t t, size_t cus, bool glu
             p.nks = nks;
             // four waves where a CU has several workgroups and eight would have few k tiles each or hold many sums, or k is short
             p.waves = (grid > cus && (run <= 40 || rb * tt >= 16)) || run <= 16 ? 4 : 8;
-            p.waves = (int)std::min<size_t>(p.waves, kt);
+            p.waves = (int)std::min<size_t>(p.waves, kt);  // kt is 2 at least, and so are they
             p.price = (groups > 1 ? 4.3 : 0.0) + std::max(rounds * load / (groups > 1 ? 34.2 : 49.6), (double)(blocks16 * kt) / 9079.0) + join;
             if (p.price < best.price) best = p;
         }

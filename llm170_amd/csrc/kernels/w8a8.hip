@@ -42,7 +42,7 @@ __device__ __forceinline__ void w8_store4(void* __restrict__ y, size_t at, int l
 }
 
 // ------------------------------------------------------------------------------------------------ up to 64 rows
-// The weight stream bounds these launches.  A workgroup's waves take consecutive runs of a k slice of the same RB row blocks (16
+// The weight stream bounds these launches.  A workgroup's waves, two at least, take consecutive runs of a k slice of the same RB row blocks (16
 // outputs each); the weights arrive as whole tiles straight in registers, DEPTH of them in flight per row block, meet TT tiles of 16
 // activation rows (from the L2), and the waves' sums are added in LDS: whole numbers, so in any order the same.  Where there are too
 // few row blocks for the chip, slices of k go to several workgroups (gridDim.y of them): each leaves its sums in the workspace and
@@ -96,10 +96,8 @@ __device__ __forceinline__ void skinny_body(const char* __restrict__ wt, const f
 #pragma unroll
     for (int d = 0; d < DEPTH; d++)
         if (lo + d < hi) load(d, lo + d);
-    if (W > 1) {
-        for (int i = threadIdx.x; i < TILES * 256; i += W * 64) (&sums[0][0][0])[i] = 0;
-        __syncthreads();
-    }
+    for (int i = threadIdx.x; i < TILES * 256; i += W * 64) (&sums[0][0][0])[i] = 0;
+    __syncthreads();
     for (int k = lo; k < hi; k += DEPTH) {
 #pragma unroll
         for (int d = 0; d < DEPTH; d++) {
@@ -112,16 +110,14 @@ __device__ __forceinline__ void skinny_body(const char* __restrict__ wt, const f
             }
         }
     }
-    if (W > 1) {
 #pragma unroll
-        for (int i = 0; i < RB; i++)
+    for (int i = 0; i < RB; i++)
 #pragma unroll
-            for (int j = 0; j < TT; j++)
+        for (int j = 0; j < TT; j++)
 #pragma unroll
-                for (int e = 0; e < 4; e++)
-                    __hip_atomic_fetch_add(&sums[i * TT + j][e][lane], acc[i][j][e], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-        __syncthreads();
-    }
+            for (int e = 0; e < 4; e++)
+                __hip_atomic_fetch_add(&sums[i * TT + j][e][lane], acc[i][j][e], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+    __syncthreads();
     // A wave finishes every W-th tile (gated: a gate and its values)
     auto total = [&](int tile) {
         i4_t v;
@@ -139,7 +135,7 @@ __device__ __forceinline__ void skinny_body(const char* __restrict__ wt, const f
 #pragma unroll
         for (int u = 0; u < TILES; u++) {
             if (u % W != wave || m0 + (u % TT) * 16 + tok >= t) continue;
-            const i4_t v = W > 1 ? total(u) : acc[u / TT][u % TT];
+            const i4_t v = total(u);
             w8_pair_t* const p = mine + ks * slice + u * 128;
             __hip_atomic_store(p, (w8_pair_t)(unsigned)v[1] << 32 | (unsigned)v[0], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             __hip_atomic_store(p + 64, (w8_pair_t)(unsigned)v[3] << 32 | (unsigned)v[2], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -158,7 +154,7 @@ __device__ __forceinline__ void skinny_body(const char* __restrict__ wt, const f
         const int b = block_of(i), m = m0 + j * 16 + tok, c = b * 16 + kg * 4;
         if (b > last || m >= t) continue;
         auto sum_of = [&](int i_) {
-            if (nks == 1) return W > 1 ? total(i_ * TT + j) : acc[i_][j];
+            if (nks == 1) return total(i_ * TT + j);
             i4_t v = {0, 0, 0, 0};
             const w8_pair_t* p = mine + (i_ * TT + j) * 128;
 #pragma unroll 4
