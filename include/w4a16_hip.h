@@ -511,7 +511,8 @@ int w4a16_bench_chain(w4a16_ctx* ctx, const char* prefix, size_t n_layers, uint6
  * A row x is quantised as s = fl32(max |x| / 127), q = the whole number nearest to x / s (halves to the even one), exactly;
  * a row whose s would fall below 2^-126 counts as zeros (s = 0), a row that holds infinity or NaN has s = NaN (and so has
  * every output of it) and q = 0.
- * Every call is ordered on the launch stream, may be captured, and does not synchronise.
+ * Every call but an upload is ordered on the launch stream, may be captured, and does not synchronise, except where scratch of the context has to
+ * grow: that waits for the stream, makes earlier graphs stale, and under capture is refused.  Rows beyond what one launch holds take several.
  * ---------------------------------------------------------------------------------------------------------- */
 enum { W4A16_F32 = 0, W4A16_F16 = 1, W4A16_BF16 = 2, W4A16_Q8 = 3 }; /* element types; Q8: quantised rows, see below */
 
@@ -553,7 +554,7 @@ int w4a16_plan_w8a8(size_t n, size_t k, size_t t, int cu_count, int glu, char* k
  *   top_idx int32 [t][top_k], top_logp f32 [t][top_k]: the top_k (up to 32) most likely tokens, best first, of equal logits the lower
  *     token first, NaN ahead of everything, and their log probabilities.
  * -infinity rules a token out: log probability -infinity, no part in the entropy.  A row of nothing else has entropy 0 and gives every
- * token -infinity.  A row that holds NaN or +infinity has NaN for logp, entropy and top_logp. */
+ * token -infinity.  Finite logits may be of any size.  A row that holds NaN or +infinity has NaN for logp, entropy and top_logp. */
 int w4a16_token_logprobs(w4a16_ctx* ctx, uint64_t logits_dev, int logits_type, size_t ld, size_t t, size_t n_vocab, uint64_t targets_dev,
                          uint64_t logp_dev, uint64_t entropy_dev, size_t top_k, uint64_t top_idx_dev, uint64_t top_logp_dev);
 

@@ -37,7 +37,7 @@ static size_t rows_per_launch(unsigned block) { return 0xffffffffu / block / 128
 
 static int quant_rows(w4a16_ctx* ctx, uint64_t x, int x_type, size_t ldx, size_t t, size_t k, uint64_t q, uint64_t s) {
     char sym[64];
-    // Few rows: a thread per four columns; else one per sixteen, of at most 768 (300 x 17408 f16 10.1 us with 1024, 8.2; 4096 rows 65 and 52)
+    // Few rows: a thread per four columns; else one per sixteen, of at most 768 (300 x 17408 f16 10.7 us with 1024, 8.7; 4096 rows 64 and 52)
     const bool few = t <= 16;
     snprintf(sym, sizeof sym, "w4a16_quant_%s_%s", few ? "few" : "rows", type_name(x_type));
     const int r = (int)tile_rows(t);

@@ -21,7 +21,8 @@ __device__ __forceinline__ unsigned quant_block_max(unsigned m, unsigned* red, i
 
 // s[r] = step of row r, q = round(x / s) in tiles of R rows.  A workgroup per row, a thread per 16 columns and round; the first
 // KEEP rounds stay in registers between the two passes over the row, what lies behind them is read again from the cache.
-// 4096 x 5120 f16 17 us, 300 x 17408 8.2, 4096 x 17408 52: the conversions' instructions bound the large ones, latency the small.
+// Launches back to back: 4096 x 5120 f16 19.0 us, 300 x 17408 8.7, 4096 x 17408 51.6.  The waves wait (65 % of their cycles at 4096 x 5120; for the
+// issue of instructions 10 %): a workgroup loads its row, reduces it and stores it one after another.
 #define QUANT_KEEP 2
 template <int T>
 __device__ __forceinline__ void quant_body(const void* __restrict__ x, size_t ldx, int k, int kt, int R, char* __restrict__ q,
@@ -155,7 +156,8 @@ QUANT_FEW(w4a16_quant_few_bf16, Q8_BF16)
 
 // w4a16_norm_resid (glue.hip) and the quantisation of its f32 result in one pass: the same arithmetic in the same order, so the
 // rows are those of the two launches bit for bit.  x <- x + ab; xn = x * inv * nw[w_off + c] is rounded twice and never stored.
-// 4096 x 5120 50 us (the norm alone 51, its bytes 53 at a copy's rate), 300 x 5120 7.2; with byte stores and rows of a tile on all XCDs 59 and 8.7.
+// Launches back to back, cold rows: 4096 x 5120 64 us (w4a16_norm_resid, which writes f32, 75; the bytes at a copy's rate 53), 300 x 5120 9.6 (9.0).  On the
+// same rows again and again 50 and 7.2; with byte stores and rows of a tile on all XCDs 59 and 8.7.
 extern "C" __global__ __launch_bounds__(1024) void w4a16_norm_resid_q8(float* __restrict__ x, const float* __restrict__ nw,
                                                                        const float* __restrict__ ab, char* __restrict__ q,
                                                                        float* __restrict__ s, int w_off, int hidden, int kt, int R, int t) {

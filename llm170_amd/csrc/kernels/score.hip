@@ -19,9 +19,10 @@
 // part of it is there once.
 // A row goes to one workgroup or, where there are few rows, to several: each leaves its record in the workspace and draws a
 // ticket, the last one joins them.
-// 2048 x 100003 f16 with its best token 90 us, 4.6 TB/s: the exponentials' issue and the stream, which a copy runs at 5.2 TB/s.  64 x
-// 131072 bf16, 20 best, 21.6 us, 1 x 32000 f32, 5 best, 9: chains of latencies (the first stage 2.4 us, each later one about 1.9, the
-// joining of the waves and of the records several), not bytes.
+// Launches back to back: 2048 x 100003 f16 with its best token 90 us, 4.6 TB/s: the exponentials' issue and the stream, which a copy runs at 5.1
+// TB/s.  64 x 131072 bf16, 20 best, 20.7 us, without alternatives 12.5; 1 x 32000 f32, 5 best, 9.9, without 5.4: chains of latencies, not bytes: one
+// stage for every wave, the ranking of its candidates, the joining of the waves and of the records.  64 x 131072 with 99.9 % ruled out 36.5 us: where a
+// stage holds nothing else, all lanes of -infinity reach the bound.
 #include "q8_common.hpp"
 
 #define SCORE_MAX_TOP 32
@@ -492,6 +493,8 @@ __device__ __forceinline__ void score_body(const void* __restrict__ logits, size
     }
 }
 
+// The most waves per SIMD whose registers (79, 88, 111) need no spilling.  One wave more, spilled: 2048 x 50001 f32, 20 best, 124 us for 84, 2048 x
+// 100003 f16, 1 best, 108 for 90, bf16 114 for 90.
 #define SCORE_KERNEL(NAME, T, WAVES_PER_SIMD)                                                                                                              \
     extern "C" __global__ __launch_bounds__(256, WAVES_PER_SIMD) void NAME(const void* logits, size_t ld, int vocab, const int* targets, float* logp,       \
                                                            float* entropy, int top, int* top_idx, float* top_logp, int segs, int seg_len,  \

@@ -47,8 +47,8 @@ __device__ __forceinline__ void w8_store4(void* __restrict__ y, size_t at, int l
 // activation rows (from the L2), and the waves' sums are added in LDS: whole numbers, so in any order the same.  Where there are too
 // few row blocks for the chip, slices of k go to several workgroups (gridDim.y of them): each leaves its sums in the workspace and
 // draws a ticket of its row blocks, the last one adds them.  More than TT * 16 rows: groups of so many, each through all of it.
-// 34816 x 5120 gated at t = 1 30 us (6.0 TB/s), 131072 x 5120 at t = 4 101 us (6.6), where a kernel that only reads gets 6.0 and a copy
-// 5.2; 4096 x 4096 at t = 1 4.5 us, of which about 2 are the launch's way to its first weights.
+// Launches back to back: 34816 x 5120 gated at t = 1 31.5 us (5.7 TB/s), 131072 x 5120 at t = 4 98 us (6.8), where a library's sum reads at 6.0 and a
+// copy moves 5.1; 4096 x 4096 at t = 1 5.2 us, of which about 2 are the launch's way to its first weights.
 typedef unsigned long long w8_pair_t;
 
 template <int RB, int TT, bool GLU>
@@ -201,9 +201,10 @@ W8_SKINNY_T(w4a16_w8a8_skinny_r4, 4, true, _glu)
 // of 64 at a time, both asked for AHEAD k tiles ahead: a line's first reader of an XCD waits up to 2 us for it.  Nothing waits for the
 // newest loads: a k tile's barrier orders LDS alone, and with three LDS buffers the next tile's first blocks are read ahead of it.  The
 // scales are fetched with the first tiles and the results' type is chosen once, or the tile's end took half as long as its products.
-// 34816 x 5120 gated at t = 4096: 591 us, 2.47 POP/s of int8 (a library's product of this size without activation or scales 785); the
-// matrix units are busy 63 % of the time, at 1.9 GHz.  In the states before: LDS DMA, whose barriers have to wait for every load of the
-// wave, 672; 650 with scales fetched at the end; with the loads one by one between the products within 3 % of this, both ways.
+// 34816 x 5120 gated at t = 4096, launches back to back: 632 us, 2.3 POP/s of int8 (a library's product of this size without activation or scales
+// 796); 604 to 736 in traces, by the clock that the power limit leaves.  The matrix units are busy 63 % of the time.  On a card where this took 591: LDS
+// DMA, whose barriers have to wait for every load of the wave, 672; 650 with scales fetched at the end; with the loads one by one between the products
+// within 3 % of this, both ways.
 // nks > 1: slices of k go to several workgroups, which hand their sums over as those of the kernels above do.
 template <int T>
 struct w8_type {
