@@ -514,7 +514,7 @@ int w4a16_bench_chain(w4a16_ctx* ctx, const char* prefix, size_t n_layers, uint6
  * Every call but an upload is ordered on the launch stream, may be captured, and does not synchronise, except where scratch of the context has to
  * grow: that waits for the stream, makes earlier graphs stale, and under capture is refused.  Rows beyond what one launch holds take several.
  * ---------------------------------------------------------------------------------------------------------- */
-enum { W4A16_F32 = 0, W4A16_F16 = 1, W4A16_BF16 = 2, W4A16_Q8 = 3 }; /* element types; Q8: quantised rows, see below */
+enum { W4A16_F32 = 0, W4A16_F16 = 1, W4A16_BF16 = 2, W4A16_Q8 = 3, W4A16_F8 = 4 }; /* element types; Q8, F8: quantised rows, see below */
 
 /* Registers w int8 [n][k] (row-major, any n and k) and its scales [n] (s_type: f32, f16 or bf16) under `name`, in a name
  * space of its own.  A name registered before gets the new weights; graphs captured until then are stale
@@ -547,6 +547,43 @@ int w4a16_lin_forward_w8a8_glu(w4a16_ctx* ctx, const char* name, uint64_t x_dev,
  * neither a context nor a GPU.  Out pointers may be NULL. */
 int w4a16_plan_w8a8(size_t n, size_t k, size_t t, int cu_count, int glu, char* kernel, size_t cap, size_t* workgroups, int* waves,
                     int* k_slices);
+
+/* ------------------------------------------------------------------------------------------------------------
+ * FP8 linears: e4m3 weights w [n][k] (OCP: largest 448, no infinity) with an f32 scale for each block of 128 x 128, activations quantised to e4m3 with a scale
+ * for each 128 k of a row.
+ *     y[m][c] = sum_b sx[b][m] * sw[c / 128][b] * sum_{k in block b} q[m][k] w[c][k]
+ * A block of a row x is quantised with the least power of two s >= 2^-126 that brings its largest magnitude to 448 or below; q = x / s to the nearest e4m3
+ * number (halves to the even one), exactly: powers of two make the quotients exact and cost no relative precision.  A block of zeros has s = 0, one that holds infinity or
+ * NaN s = NaN (and so has every output of its row) and q = 0.
+ * Sums are held in f32, a block's products summed first; the result is rounded once more to y's type.  f32 results, and any of up to 64 rows, are sums of 32 bits.
+ * For f16 and bf16 results of more rows the products of a block may be summed by the e4m3 matrix instruction, which drops of a product what lies more than 2^-13 below the
+ * largest of its group: 1.6e-5 of the results' size on normal numbers, 1 / 17 of an f16 result's own rounding.  The same call gives the same bits every time.
+ * Streams, captures, scratch and the number of rows: as for the W8A8 linears above.
+ * ---------------------------------------------------------------------------------------------------------- */
+
+/* Registers w e4m3 [n][k] (row-major, any n and k) and its scales [ceil(n / 128)][ceil(k / 128)] (s_type: f32, f16 or bf16) under `name`, in a name space of its
+ * own.  A name registered before gets the new weights; graphs captured until then are stale (W4A16_ERR_STALE_GRAPH).  Only the re-laid-out copy stays on the device. */
+int w4a16_upload_lin_f8(w4a16_ctx* ctx, const char* name, const void* q, size_t qlen_bytes, const void* s, size_t slen_bytes, size_t n, size_t k,
+                        int s_type);
+int w4a16_lin_f8_info(w4a16_ctx* ctx, const char* name, size_t* n, size_t* k);
+
+/* x (f32, f16 or bf16, rows ldx elements apart, 0 = k) -> q (w4a16_q8_bytes(t, k) bytes in the tiles described there, 16-byte aligned) and s f32
+ * [ceil(k / 128)][t].  Unlike int8 rows these are filled up with zeros to whole blocks of 128; rows of other origin have to be, too. */
+int w4a16_quant_rows_f8(w4a16_ctx* ctx, uint64_t x_dev, int x_type, size_t ldx, size_t t, size_t k, uint64_t q_dev, uint64_t s_dev);
+/* w4a16_norm_resid with its f32 result quantised as by w4a16_quant_rows_f8 instead of stored, in one launch; the same bits as the two.
+ * x <- x + ab. */
+int w4a16_norm_resid_f8(w4a16_ctx* ctx, uint64_t x_dev, uint64_t nw_dev, uint64_t ab_dev, uint64_t q_dev, uint64_t s_dev, size_t t, size_t w_off,
+                        size_t hidden);
+
+/* y [t][n] (f32, f16 or bf16).  x: rows of floats (x_type, ldx as above, xs_dev = 0), quantised into a buffer of the context on the
+ * way; or x_type = W4A16_F8: x_dev and xs_dev are the q and s of t rows of k, which several linears may read (ldx = 0); s may be any f32 numbers. */
+int w4a16_lin_forward_f8(w4a16_ctx* ctx, const char* name, uint64_t x_dev, int x_type, size_t ldx, uint64_t xs_dev, size_t t, uint64_t y_dev, int y_type);
+/* A fused gate|up linear (rows 0..n/2 gate, n/2..n up; n a multiple of 256) with its activation: y [t][n/2] = act(gate) * up on the f32 sums, rounded once
+ * to y's type.  act: W4A16_ACT_SILU or W4A16_ACT_GELU_TANH. */
+int w4a16_lin_forward_f8_glu(w4a16_ctx* ctx, const char* name, uint64_t x_dev, int x_type, size_t ldx, uint64_t xs_dev, size_t t, uint64_t y_dev,
+                             int y_type, int act);
+/* The launch that t rows through an FP8 linear with results of y_type go to, as w4a16_plan_w8a8. */
+int w4a16_plan_f8(size_t n, size_t k, size_t t, int cu_count, int glu, int y_type, char* kernel, size_t cap, size_t* workgroups, int* waves, int* k_slices);
 
 /* Scores rows of logits z [t][n_vocab] (f32, f16 or bf16, rows ld elements apart, 0 = n_vocab); results of no interest are 0.
  *   targets int32 [t], logp f32 [t]: log softmax(z)[target]; 0 for a negative target (none is asked for), NaN for one >= n_vocab;

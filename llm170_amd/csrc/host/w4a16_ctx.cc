@@ -120,6 +120,12 @@ static const char* const kQuantSyms[] = {"w4a16_quant_rows_f32", "w4a16_quant_ro
 static const char* const kW8a8Syms[] = {W8_TT("w4a16_w8a8_skinny_r1", ""), W8_TT("w4a16_w8a8_skinny_r2", ""), W8_TT("w4a16_w8a8_skinny_r4", ""),
                                         W8_TT("w4a16_w8a8_skinny_r2", "_glu"), W8_TT("w4a16_w8a8_skinny_r4", "_glu"),
                                         "w4a16_w8a8_tiled_m128", "w4a16_w8a8_tiled_m128_glu", "w4a16_w8a8_tiled_m64", "w4a16_w8a8_tiled_m64_glu", "w4a16_w8a8_tiled_m64_n128", "w4a16_w8a8_tiled_m64_n128_glu", nullptr};
+static const char* const kF8QuantSyms[] = {"w4a16_quant_rows_f8_f32", "w4a16_quant_rows_f8_f16", "w4a16_quant_rows_f8_bf16", "w4a16_norm_resid_f8", nullptr};
+// as W8A8's; tiles with e4m3 products and with f16 ones (kernels/f8.hip)
+#define F8_TILES(P) P "_m64", P "_m64_glu", P "_m64_n128", P "_m64_n128_glu"
+static const char* const kF8Syms[] = {W8_TT("w4a16_f8_skinny_r1", ""), W8_TT("w4a16_f8_skinny_r2", ""), W8_TT("w4a16_f8_skinny_r4", ""),
+                                      W8_TT("w4a16_f8_skinny_r2", "_glu"), W8_TT("w4a16_f8_skinny_r4", "_glu"),
+                                      F8_TILES("w4a16_f8_tiled"), F8_TILES("w4a16_f8_exact"), nullptr};
 static const char* const kScoreSyms[] = {"w4a16_token_logprobs_f32", "w4a16_token_logprobs_f16", "w4a16_token_logprobs_bf16", nullptr};
 
 struct W4Asset {
@@ -138,6 +144,8 @@ static const W4Asset kAssets[] = {
     {"util", kUtilSyms},
     {"quant", kQuantSyms},
     {"w8a8", kW8a8Syms},
+    {"f8_quant", kF8QuantSyms},
+    {"f8", kF8Syms},
     {"score", kScoreSyms},
 };
 static const size_t kAssetCount = sizeof kAssets / sizeof kAssets[0];

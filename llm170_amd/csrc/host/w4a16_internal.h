@@ -35,6 +35,12 @@ struct W8Lin {
     size_t n = 0, k = 0;
 };
 
+// One registered FP8 linear: e4m3 weights in the same tiles, f32 scales [ceil(n / 128)][ceil(k / 128)].
+struct F8Lin {
+    uint64_t q = 0, s = 0;
+    size_t n = 0, k = 0;
+};
+
 // The experts of one MoE layer: two arenas in the tiled layout, experts at a fixed stride
 // (reference: moe_m13 / moe_s13 / moe_m2 / moe_s2, w4a16_dec/upload.rs:1116-1235).
 struct W4Experts {
@@ -90,9 +96,10 @@ struct w4a16_ctx {
     std::map<std::string, W4Lin, std::less<>> lins;
     std::map<std::string, W4Experts, std::less<>> experts;
     std::map<std::string, W8Lin, std::less<>> w8lins;
-    uint64_t q8 = 0, q8_scales = 0;  // quantised rows of a W8A8 linear that was given rows of floats
+    std::map<std::string, F8Lin, std::less<>> f8lins;
+    uint64_t q8 = 0, q8_scales = 0;  // quantised rows of a W8A8 or FP8 linear that was given rows of floats
     size_t q8_cap = 0, q8_scales_cap = 0;
-    uint64_t w8_part = 0, w8_tickets = 0;  // sums of the k slices of a W8A8 launch, one ticket per workgroup of a slice
+    uint64_t w8_part = 0, w8_tickets = 0;  // sums of the k slices of a W8A8 or FP8 launch, one ticket per workgroup of a slice
     size_t w8_part_cap = 0, w8_tickets_cap = 0;
     uint64_t score_ws = 0, score_tickets = 0;  // records of the segments of a row of logits, one ticket per row
     size_t score_ws_cap = 0, score_tickets_cap = 0;
@@ -173,6 +180,21 @@ int w4_lin_forward_fixed_ws(w4a16_ctx* ctx, const char* name, uint64_t x_dev, ui
 // per-device fixed scratch of the allocation-free entry point (w4a16_noalloc.hip)
 int w4_noalloc_init(w4a16_ctx* ctx);
 void w4_noalloc_release(w4a16_ctx* ctx);
+
+// ---- what the 8-bit linears share (w4a16_w8a8.cc)
+inline bool w4_float_type(int type) { return type == W4A16_F32 || type == W4A16_F16 || type == W4A16_BF16; }
+inline size_t w4_type_bytes(int type) { return type == W4A16_F32 ? 4 : 2; }
+inline const char* w4_type_name(int type) { return type == W4A16_F32 ? "f32" : type == W4A16_F16 ? "f16" : "bf16"; }
+// blocks of 128 k, two k tiles each (q8_common.hpp), and rows of an activation tile
+inline size_t w4_q8_blocks(size_t k) { return (k + 127) / 128; }
+inline size_t w4_q8_tile_rows(size_t t) { return t == 1 ? 1 : t <= 4 ? 4 : 16; }
+// Rows of a launch with a workgroup of `block` threads each: HIP takes fewer than 2^32 threads.  More rows go in several launches, of whole
+// tiles and, for the rows' order over the XCDs, of 128.
+inline size_t w4_rows_per_launch(unsigned block) { return 0xffffffffu / block / 128 * 128; }
+int w4_q8_check_rows(const char* what, size_t t, size_t k);
+float w4_scale_at(const void* s, int type, size_t i);  // element i of f32, f16 or bf16 numbers
+// scratch for k slices: their sums, and tickets that are zero between launches
+int w4_split_workspace(w4a16_ctx* ctx, size_t part_bytes, size_t tickets);
 
 #define W4_TRY(expr)          \
     do {                      \

@@ -10,16 +10,9 @@
 
 static inline unsigned ceil_div(size_t a, size_t b) { return (unsigned)((a + b - 1) / b); }
 
-// k tiles of a row block: whole pairs of 64 k (q8_common.hpp)
-static size_t k_tiles(size_t k) { return (k + 127) / 128 * 2; }
-// rows of an activation tile
-static size_t tile_rows(size_t t) { return t == 1 ? 1 : t <= 4 ? 4 : 16; }
+static size_t k_tiles(size_t k) { return w4_q8_blocks(k) * 2; }
 
-static size_t type_bytes(int type) { return type == W4A16_F32 ? 4 : 2; }
-static bool float_type(int type) { return type == W4A16_F32 || type == W4A16_F16 || type == W4A16_BF16; }
-static const char* type_name(int type) { return type == W4A16_F32 ? "f32" : type == W4A16_F16 ? "f16" : "bf16"; }
-
-static int check_rows(const char* what, size_t t, size_t k) {
+int w4_q8_check_rows(const char* what, size_t t, size_t k) {
     if (t == 0 || t > 0x7fffff00u || k == 0 || k > kW4Q8MaxK)
         return w4_fail(W4A16_ERR_SHAPE, "%s: t=%zu k=%zu outside 1..2^31-256 and 1..%d", what, t, k, kW4Q8MaxK);
     return 0;
@@ -27,26 +20,22 @@ static int check_rows(const char* what, size_t t, size_t k) {
 
 extern "C" size_t w4a16_q8_bytes(size_t t, size_t k) {
     if (t == 0 || t > 0x7fffff00u || k == 0 || k > kW4Q8MaxK) return 0;
-    const size_t r = tile_rows(t);
+    const size_t r = w4_q8_tile_rows(t);
     return (t + r - 1) / r * r * k_tiles(k) * 64;
 }
-
-// Rows of a launch with a workgroup of `block` threads each: HIP takes fewer than 2^32 threads.  More rows go in several launches, of whole
-// tiles and, for the rows' order over the XCDs, of 128.
-static size_t rows_per_launch(unsigned block) { return 0xffffffffu / block / 128 * 128; }
 
 static int quant_rows(w4a16_ctx* ctx, uint64_t x, int x_type, size_t ldx, size_t t, size_t k, uint64_t q, uint64_t s) {
     char sym[64];
     // Few rows: a thread per four columns; else one per sixteen, of at most 768 (300 x 17408 f16 10.7 us with 1024, 8.7; 4096 rows 64 and 52)
     const bool few = t <= 16;
-    snprintf(sym, sizeof sym, "w4a16_quant_%s_%s", few ? "few" : "rows", type_name(x_type));
-    const int r = (int)tile_rows(t);
+    snprintf(sym, sizeof sym, "w4a16_quant_%s_%s", few ? "few" : "rows", w4_type_name(x_type));
+    const int r = (int)w4_q8_tile_rows(t);
     const unsigned block = (unsigned)std::min<size_t>(few ? (k + 255) / 256 * 64 : (k + 1023) / 1024 * 64, few ? 1024 : 768);
     int ki = (int)k, kt = (int)k_tiles(k), ri = r, bi = (int)block;
-    const size_t most = rows_per_launch(block);
+    const size_t most = w4_rows_per_launch(block);
     for (size_t at = 0; at < t; at += most) {
         const size_t rows = std::min(most, t - at);
-        uint64_t x_at = x + at * ldx * type_bytes(x_type), q_at = q + at * kt * 64, s_at = s + at * 4;
+        uint64_t x_at = x + at * ldx * w4_type_bytes(x_type), q_at = q + at * kt * 64, s_at = s + at * 4;
         int ti = (int)rows;
         void* params[] = {&x_at, &ldx, &ki, &kt, &ri, &q_at, &s_at, &ti, &bi};
         W4_TRY(w4_launch(ctx, sym, few ? (unsigned)rows : ceil_div(rows, 128) * 128, few ? ceil_div(k, block * 4) : 1, block, 0, params));
@@ -56,11 +45,11 @@ static int quant_rows(w4a16_ctx* ctx, uint64_t x, int x_type, size_t ldx, size_t
 
 extern "C" int w4a16_quant_rows(w4a16_ctx* ctx, uint64_t x_dev, int x_type, size_t ldx, size_t t, size_t k, uint64_t q_dev, uint64_t s_dev) {
     if (!ctx || !x_dev || !q_dev || !s_dev) return w4_fail(W4A16_ERR_ARG, "quant_rows: null operand");
-    if (!float_type(x_type)) return w4_fail(W4A16_ERR_ARG, "quant_rows: x type %d (0 = f32, 1 = f16, 2 = bf16)", x_type);
-    W4_TRY(check_rows("quant_rows", t, k));
+    if (!w4_float_type(x_type)) return w4_fail(W4A16_ERR_ARG, "quant_rows: x type %d (0 = f32, 1 = f16, 2 = bf16)", x_type);
+    W4_TRY(w4_q8_check_rows("quant_rows", t, k));
     if (ldx == 0) ldx = k;
     if (ldx < k) return w4_fail(W4A16_ERR_SHAPE, "quant_rows: ldx=%zu below k=%zu", ldx, k);
-    if (x_dev % type_bytes(x_type) || s_dev % 4 || q_dev % 16)
+    if (x_dev % w4_type_bytes(x_type) || s_dev % 4 || q_dev % 16)
         return w4_fail(W4A16_ERR_ARG, "quant_rows: x and s must be aligned to their elements, q to 16 bytes");
     W4_TRY(w4_hip(hipSetDevice(ctx->device), "hipSetDevice"));
     return quant_rows(ctx, x_dev, x_type, ldx, t, k, q_dev, s_dev);
@@ -71,12 +60,12 @@ extern "C" int w4a16_norm_resid_q8(w4a16_ctx* ctx, uint64_t x_dev, uint64_t nw_d
     if (!ctx || !x_dev || !nw_dev || !ab_dev || !q_dev || !s_dev) return w4_fail(W4A16_ERR_ARG, "norm_resid_q8: null operand");
     if (hidden == 0 || hidden > 8192) return w4_fail(W4A16_ERR_SHAPE, "norm_resid_q8: hidden=%zu outside 1..8192", hidden);
     if (w_off > 0x7fffffffu - hidden) return w4_fail(W4A16_ERR_SHAPE, "norm_resid_q8: w_off=%zu too large", w_off);
-    W4_TRY(check_rows("norm_resid_q8", t, hidden));
+    W4_TRY(w4_q8_check_rows("norm_resid_q8", t, hidden));
     if (x_dev % 4 || nw_dev % 4 || ab_dev % 4 || s_dev % 4 || q_dev % 16)
         return w4_fail(W4A16_ERR_ARG, "norm_resid_q8: f32 operands must be aligned to 4 bytes, q to 16");
     W4_TRY(w4_hip(hipSetDevice(ctx->device), "hipSetDevice"));
-    int wo = (int)w_off, h = (int)hidden, kt = (int)k_tiles(hidden), r = (int)tile_rows(t);
-    const size_t most = rows_per_launch(1024);
+    int wo = (int)w_off, h = (int)hidden, kt = (int)k_tiles(hidden), r = (int)w4_q8_tile_rows(t);
+    const size_t most = w4_rows_per_launch(1024);
     for (size_t at = 0; at < t; at += most) {
         const size_t rows = std::min(most, t - at);
         uint64_t x_at = x_dev + at * hidden * 4, ab_at = ab_dev + at * hidden * 4, q_at = q_dev + at * kt * 64, s_at = s_dev + at * 4;
@@ -101,7 +90,7 @@ static float w4_f16_to_f32(uint16_t h) {
     return sign * (exp ? std::ldexp((float)(1024 + frac), exp - 25) : std::ldexp((float)frac, -24));
 }
 
-static float scale_at(const void* s, int type, size_t i) {
+float w4_scale_at(const void* s, int type, size_t i) {
     uint32_t b = 0;
     if (type == W4A16_F32) {
         memcpy(&b, static_cast<const char*>(s) + i * 4, 4);
@@ -119,8 +108,8 @@ static float scale_at(const void* s, int type, size_t i) {
 extern "C" int w4a16_upload_lin_w8a8(w4a16_ctx* ctx, const char* name, const void* q, size_t qlen_bytes, const void* s, size_t slen_bytes, size_t n,
                                      size_t k, int s_type) {
     if (!ctx || !name || !q || !s) return w4_fail(W4A16_ERR_ARG, "upload_lin_w8a8: null argument");
-    if (!float_type(s_type)) return w4_fail(W4A16_ERR_ARG, "upload_lin_w8a8 %s: scale type %d (0 = f32, 1 = f16, 2 = bf16)", name, s_type);
-    if (n == 0 || n > 0x7fffff00u || k == 0 || k > kW4Q8MaxK || qlen_bytes != n * k || slen_bytes != n * type_bytes(s_type))
+    if (!w4_float_type(s_type)) return w4_fail(W4A16_ERR_ARG, "upload_lin_w8a8 %s: scale type %d (0 = f32, 1 = f16, 2 = bf16)", name, s_type);
+    if (n == 0 || n > 0x7fffff00u || k == 0 || k > kW4Q8MaxK || qlen_bytes != n * k || slen_bytes != n * w4_type_bytes(s_type))
         return w4_fail(W4A16_ERR_SHAPE, "upload_lin_w8a8 %s: q=%zu s=%zu bytes for n=%zu k=%zu (k up to %d)", name, qlen_bytes, slen_bytes, n, k,
                        kW4Q8MaxK);
     W4_TRY(w4_hip(hipSetDevice(ctx->device), "hipSetDevice"));
@@ -130,7 +119,7 @@ extern "C" int w4a16_upload_lin_w8a8(w4a16_ctx* ctx, const char* name, const voi
     const size_t row_blocks = (n + 15) / 16, kt = k_tiles(k), chunks = row_blocks * kt * 64;
     std::unique_ptr<float[]> scales(new (std::nothrow) float[row_blocks * 16]());
     if (!scales) return w4_fail(W4A16_ERR_ARG, "upload_lin_w8a8 %s: no host memory for %zu scales", name, n);
-    for (size_t i = 0; i < n; i++) scales[i] = scale_at(s, s_type, i);
+    for (size_t i = 0; i < n; i++) scales[i] = w4_scale_at(s, s_type, i);
     uint64_t raw = 0;
     int rc = w4a16_alloc(ctx, chunks * 16, &L.q);
     if (!rc) rc = w4a16_alloc(ctx, row_blocks * 64, &L.s);
@@ -219,7 +208,7 @@ static SkinnyPlan plan_skinny(size_t n, size_t k, size_t t, size_t cus, bool glu
     return best;
 }
 
-static int split_workspace(w4a16_ctx* ctx, size_t part_bytes, size_t tickets) {
+int w4_split_workspace(w4a16_ctx* ctx, size_t part_bytes, size_t tickets) {
     W4_TRY(w4_ensure(ctx, &ctx->w8_part, &ctx->w8_part_cap, part_bytes));
     if (tickets * 4 > ctx->w8_tickets_cap) {
         W4_TRY(w4_ensure(ctx, &ctx->w8_tickets, &ctx->w8_tickets_cap, std::max<size_t>(tickets * 4, 16384)));
@@ -303,7 +292,7 @@ static int plan_w8a8(const char* what, size_t n, size_t k, size_t t, size_t cus,
 extern "C" int w4a16_plan_w8a8(size_t n, size_t k, size_t t, int cu_count, int glu, char* kernel, size_t cap, size_t* workgroups, int* waves, int* k_slices) {
     if (cu_count <= 0 || (kernel && cap < sizeof(W8Launch::kernel)))
         return w4_fail(W4A16_ERR_ARG, "plan_w8a8: cus=%d, %zu bytes for a name of up to %zu", cu_count, cap, sizeof(W8Launch::kernel));
-    W4_TRY(check_rows("plan_w8a8", t, k));
+    W4_TRY(w4_q8_check_rows("plan_w8a8", t, k));
     if (n == 0 || n > 0x7fffff00u || (glu && n % 32 != 0))
         return w4_fail(W4A16_ERR_SHAPE, "plan_w8a8: n=%zu outside 1..2^31-256, or gated and no multiple of 32", n);
     W8Launch P;
@@ -316,9 +305,9 @@ extern "C" int w4a16_plan_w8a8(size_t n, size_t k, size_t t, int cu_count, int g
 }
 
 static int launch_w8a8(w4a16_ctx* ctx, const W8Lin& L, const W8Launch& P, uint64_t q, uint64_t s, size_t t, uint64_t y, int y_type, int act) {
-    if (P.nks > 1) W4_TRY(split_workspace(ctx, P.part_bytes, P.tickets));
+    if (P.nks > 1) W4_TRY(w4_split_workspace(ctx, P.part_bytes, P.tickets));
     uint64_t wt = L.q, ws = L.s, part = ctx->w8_part, tickets = ctx->w8_tickets;
-    int ni = (int)L.n, kti = (int)k_tiles(L.k), ti = (int)t, r = (int)tile_rows(t), wi = P.block / 64, ksi = P.nks, band = P.band;
+    int ni = (int)L.n, kti = (int)k_tiles(L.k), ti = (int)t, r = (int)w4_q8_tile_rows(t), wi = P.block / 64, ksi = P.nks, band = P.band;
     void* few[] = {&wt, &ws, &q, &s, &y, &ni, &kti, &ti, &r, &y_type, &act, &wi, &ksi, &part, &tickets};
     void* tiles[] = {&wt, &ws, &q, &s, &y, &ni, &kti, &ti, &y_type, &act, &ksi, &band, &part, &tickets};
     return w4_launch(ctx, P.kernel, (unsigned)P.grid_x, (unsigned)P.grid_y, (unsigned)P.block, 0, P.band ? tiles : few);
@@ -329,10 +318,10 @@ static int forward_w8a8(w4a16_ctx* ctx, const char* api, const char* name, uint6
     const W8Lin* L = nullptr;
     W4_TRY(find_w8(ctx, name, &L));
     if (!x || !y) return w4_fail(W4A16_ERR_ARG, "%s %s: null operand", api, name);
-    if (x_type != W4A16_Q8 && !float_type(x_type))
+    if (x_type != W4A16_Q8 && !w4_float_type(x_type))
         return w4_fail(W4A16_ERR_ARG, "%s %s: x type %d (0 = f32, 1 = f16, 2 = bf16, 3 = quantised rows)", api, name, x_type);
-    if (!float_type(y_type)) return w4_fail(W4A16_ERR_ARG, "%s %s: y type %d (0 = f32, 1 = f16, 2 = bf16)", api, name, y_type);
-    W4_TRY(check_rows(api, t, L->k));
+    if (!w4_float_type(y_type)) return w4_fail(W4A16_ERR_ARG, "%s %s: y type %d (0 = f32, 1 = f16, 2 = bf16)", api, name, y_type);
+    W4_TRY(w4_q8_check_rows(api, t, L->k));
     if (x_type == W4A16_Q8 ? !xs || ldx != 0 : xs != 0)
         return w4_fail(W4A16_ERR_ARG, "%s %s: quantised rows come with their scales and without a row stride, others without scales", api, name);
     if (act >= 0 && L->n % 32 != 0)
@@ -341,7 +330,7 @@ static int forward_w8a8(w4a16_ctx* ctx, const char* api, const char* name, uint6
         if (ldx == 0) ldx = L->k;
         if (ldx < L->k) return w4_fail(W4A16_ERR_SHAPE, "%s %s: ldx=%zu below k=%zu", api, name, ldx, L->k);
     }
-    if (y % type_bytes(y_type) || x % (x_type == W4A16_Q8 ? 16 : type_bytes(x_type)) || xs % 4)
+    if (y % w4_type_bytes(y_type) || x % (x_type == W4A16_Q8 ? 16 : w4_type_bytes(x_type)) || xs % 4)
         return w4_fail(W4A16_ERR_ARG, "%s %s: operands must be aligned to their elements, quantised rows to 16 bytes", api, name);
     W8Launch P;
     W4_TRY(plan_w8a8(api, L->n, L->k, t, (size_t)std::max(ctx->cu_count, 1), act >= 0, &P));

@@ -1,4 +1,4 @@
-// Device helpers of the 8-bit kernels: the layout of quantised rows and weights, element types, quantisation of a value.
+// Device helpers of the 8-bit kernels: the layout of quantised rows and weights, element types, quantisation of a value, stores of results.
 //
 // Tiles ("T16x64"): 16 rows x 64 k of int8, 1 KiB: 64 chunks of 16 consecutive k, chunk c * 16 + r = row r, k = 16 c .. 16 c + 15
 // (c = 0..3).  The 64 chunks in order are the operand of v_mfma_i32_16x16x64_i8 (lane l: row l % 16, k group l / 16), and a
@@ -145,7 +145,88 @@ __device__ __forceinline__ unsigned q8_wave_max(unsigned v) {
     return (unsigned)__builtin_amdgcn_readlane((int)v, 63);
 }
 
+// The sum of one value per thread of 1024, the same bits as in w4a16_norm_resid (pairwise at strides 512 .. 1) with one barrier: strides 512 .. 64 pair
+// waves, so every lane adds the sixteen waves' partials of its own lane in that order; strides 32 .. 1 pair lanes, and lane 0 has the sum.
+__device__ __forceinline__ float q8_norm_sum(float ss, float* red) {
+    const int tid = threadIdx.x;
+    red[tid] = ss;
+    __syncthreads();
+    float w[16];
+#pragma unroll
+    for (int i = 0; i < 16; i++) w[i] = red[i * 64 + (tid & 63)];
+#pragma unroll
+    for (int st = 8; st > 0; st >>= 1)
+#pragma unroll
+        for (int i = 0; i < st; i++) w[i] = w[i] + w[i + st];
+    float r = w[0];
+    auto bits = [](float v) { return __builtin_bit_cast(unsigned, v); };
+    r = r + q8_f32(__builtin_amdgcn_permlane32_swap(bits(r), bits(r), false, false)[1]);
+    r = r + q8_f32(__builtin_amdgcn_permlane16_swap(bits(r), bits(r), false, false)[1]);
+    r = r + q8_f32((unsigned)__builtin_amdgcn_update_dpp(0, (int)bits(r), 0x108, 0xf, 0xf, true));  // row_shl:8, 4, 2, 1
+    r = r + q8_f32((unsigned)__builtin_amdgcn_update_dpp(0, (int)bits(r), 0x104, 0xf, 0xf, true));
+    r = r + q8_f32((unsigned)__builtin_amdgcn_update_dpp(0, (int)bits(r), 0x102, 0xf, 0xf, true));
+    r = r + q8_f32((unsigned)__builtin_amdgcn_update_dpp(0, (int)bits(r), 0x101, 0xf, 0xf, true));
+    return q8_f32((unsigned)__builtin_amdgcn_readlane((int)bits(r), 0));
+}
+
 // Byte offset of chunk (row, 16 k from kc * 16) in a buffer of quantised rows with kt k tiles, tiles of R rows
 __device__ __forceinline__ size_t q8_chunk_at(int row, int kc, int kt, int R) {
     return ((((size_t)(row / R) * kt + (kc >> 2)) * 4 + (kc & 3)) * R + row % R) * 16;
 }
+
+// Sixteen neighbouring rows share their 256-byte runs of the tiles: they go to one XCD (block b runs on XCD b % 8), whose L2
+// joins their 16-byte pieces.
+__device__ __forceinline__ int q8_row_of_block(int R) {
+    const int b = blockIdx.x;
+    return R == 16 ? ((b >> 7) * 8 + (b & 7)) * 16 + ((b >> 3) & 15) : b;
+}
+
+// y[at .. at + 3] (those below `left`) as f32, f16 or bf16
+template <int T>
+__device__ __forceinline__ void w8_store4(void* __restrict__ y, size_t at, int left, const float (&v)[4]) {
+    if (T == Q8_F32) {
+        float* const p = static_cast<float*>(y) + at;
+        if (left >= 4) {
+            u4_any_t o;
+#pragma unroll
+            for (int i = 0; i < 4; i++) o[i] = __builtin_bit_cast(unsigned, v[i]);
+            *reinterpret_cast<u4_any_t*>(p) = o;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (i < left) p[i] = v[i];
+        }
+        return;
+    }
+    unsigned h[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) h[i] = q8_to_16<T>(v[i]);
+    uint16_t* const p = static_cast<uint16_t*>(y) + at;
+    if (left >= 4) {
+        u2_any_t o;
+        o[0] = h[0] | h[1] << 16;
+        o[1] = h[2] | h[3] << 16;
+        *reinterpret_cast<u2_any_t*>(p) = o;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            if (i < left) p[i] = (uint16_t)h[i];
+    }
+}
+__device__ __forceinline__ void w8_store4(void* __restrict__ y, size_t at, int left, const float (&v)[4], int y_type) {
+    if (y_type == Q8_F32) w8_store4<Q8_F32>(y, at, left, v);
+    else if (y_type == Q8_F16) w8_store4<Q8_F16>(y, at, left, v);
+    else w8_store4<Q8_BF16>(y, at, left, v);
+}
+
+template <int T>
+struct w8_type {
+    static constexpr int value = T;
+};
+__device__ __forceinline__ void w8_lds_done() { __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local"); }  // global loads stay in flight
+__device__ __forceinline__ void w8_lds_barrier() {  // behind w8_lds_done
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
+typedef unsigned long long w8_pair_t;  // two 32-bit sums of a k slice, handed over at once

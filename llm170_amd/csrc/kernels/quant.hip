@@ -1,13 +1,6 @@
 // Quantisation of activation rows to int8 with one scale per row, and the re-layout of int8 weights at upload.
 #include "q8_common.hpp"
 
-// Sixteen neighbouring rows share their 256-byte runs of the tiles: they go to one XCD (block b runs on XCD b % 8), whose L2
-// joins their 16-byte pieces.
-__device__ __forceinline__ int q8_row_of_block(int R) {
-    const int b = blockIdx.x;
-    return R == 16 ? ((b >> 7) * 8 + (b & 7)) * 16 + ((b >> 3) & 15) : b;
-}
-
 // Largest of one value per thread over the workgroup.
 __device__ __forceinline__ unsigned quant_block_max(unsigned m, unsigned* red, int waves) {
     m = q8_wave_max(m);
@@ -180,26 +173,7 @@ extern "C" __global__ __launch_bounds__(1024) void w4a16_norm_resid_q8(float* __
             ss = __builtin_fmaf(v[j], v[j], ss);
         }
     }
-    // The pairwise sums of w4a16_norm_resid (strides 512 .. 1 of the 1024 partials) with one barrier: strides 512 .. 64 pair waves, so every
-    // lane adds the sixteen waves' partials of its own lane in that order; strides 32 .. 1 pair lanes, and lane 0 has the sum.
-    red[tid] = ss;
-    __syncthreads();
-    float w[16];
-#pragma unroll
-    for (int i = 0; i < 16; i++) w[i] = red[i * 64 + (tid & 63)];
-#pragma unroll
-    for (int st = 8; st > 0; st >>= 1)
-#pragma unroll
-        for (int i = 0; i < st; i++) w[i] = w[i] + w[i + st];
-    float r = w[0];
-    auto bits = [](float v) { return __builtin_bit_cast(unsigned, v); };
-    r = r + q8_f32(__builtin_amdgcn_permlane32_swap(bits(r), bits(r), false, false)[1]);
-    r = r + q8_f32(__builtin_amdgcn_permlane16_swap(bits(r), bits(r), false, false)[1]);
-    r = r + q8_f32((unsigned)__builtin_amdgcn_update_dpp(0, (int)bits(r), 0x108, 0xf, 0xf, true));  // row_shl:8, 4, 2, 1
-    r = r + q8_f32((unsigned)__builtin_amdgcn_update_dpp(0, (int)bits(r), 0x104, 0xf, 0xf, true));
-    r = r + q8_f32((unsigned)__builtin_amdgcn_update_dpp(0, (int)bits(r), 0x102, 0xf, 0xf, true));
-    r = r + q8_f32((unsigned)__builtin_amdgcn_update_dpp(0, (int)bits(r), 0x101, 0xf, 0xf, true));
-    r = q8_f32((unsigned)__builtin_amdgcn_readlane((int)bits(r), 0));
+    const float r = q8_norm_sum(ss, red);
     const float inv = 1.0f / sqrtf(r / (float)hidden + 1e-6f);
     unsigned m = 0;
 #pragma unroll

@@ -3,44 +3,6 @@
 // y[m][c] = act(gate) * value, [t][n/2].
 #include "q8_common.hpp"
 
-// y[at .. at + 3] (those below `left`) as f32, f16 or bf16
-template <int T>
-__device__ __forceinline__ void w8_store4(void* __restrict__ y, size_t at, int left, const float (&v)[4]) {
-    if (T == Q8_F32) {
-        float* const p = static_cast<float*>(y) + at;
-        if (left >= 4) {
-            u4_any_t o;
-#pragma unroll
-            for (int i = 0; i < 4; i++) o[i] = __builtin_bit_cast(unsigned, v[i]);
-            *reinterpret_cast<u4_any_t*>(p) = o;
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-                if (i < left) p[i] = v[i];
-        }
-        return;
-    }
-    unsigned h[4];
-#pragma unroll
-    for (int i = 0; i < 4; i++) h[i] = q8_to_16<T>(v[i]);
-    uint16_t* const p = static_cast<uint16_t*>(y) + at;
-    if (left >= 4) {
-        u2_any_t o;
-        o[0] = h[0] | h[1] << 16;
-        o[1] = h[2] | h[3] << 16;
-        *reinterpret_cast<u2_any_t*>(p) = o;
-    } else {
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-            if (i < left) p[i] = (uint16_t)h[i];
-    }
-}
-__device__ __forceinline__ void w8_store4(void* __restrict__ y, size_t at, int left, const float (&v)[4], int y_type) {
-    if (y_type == Q8_F32) w8_store4<Q8_F32>(y, at, left, v);
-    else if (y_type == Q8_F16) w8_store4<Q8_F16>(y, at, left, v);
-    else w8_store4<Q8_BF16>(y, at, left, v);
-}
-
 // ------------------------------------------------------------------------------------------------ up to 64 rows
 // The weight stream bounds these launches.  A workgroup's waves, two at least, take consecutive runs of a k slice of the same RB row blocks (16
 // outputs each); the weights arrive as whole tiles straight in registers, DEPTH of them in flight per row block, meet TT tiles of 16
@@ -49,8 +11,6 @@ __device__ __forceinline__ void w8_store4(void* __restrict__ y, size_t at, int l
 // draws a ticket of its row blocks, the last one adds them.  More than TT * 16 rows: groups of so many, each through all of it.
 // Launches back to back: 34816 x 5120 gated at t = 1 31.5 us (5.7 TB/s), 131072 x 5120 at t = 4 98 us (6.8), where a library's sum reads at 6.0 and a
 // copy moves 5.1; 4096 x 4096 at t = 1 5.2 us, of which about 2 are the launch's way to its first weights.
-typedef unsigned long long w8_pair_t;
-
 template <int RB, int TT, bool GLU>
 __device__ __forceinline__ void skinny_body(const char* __restrict__ wt, const float* __restrict__ ws, const char* __restrict__ xq,
                                             const float* __restrict__ xs, void* __restrict__ y, int n, int kt, int t, int R, int y_type, int act, int W,
@@ -206,16 +166,6 @@ W8_SKINNY_T(w4a16_w8a8_skinny_r4, 4, true, _glu)
 // DMA, whose barriers have to wait for every load of the wave, 672; 650 with scales fetched at the end; with the loads one by one between the products
 // within 3 % of this, both ways.
 // nks > 1: slices of k go to several workgroups, which hand their sums over as those of the kernels above do.
-template <int T>
-struct w8_type {
-    static constexpr int value = T;
-};
-__device__ __forceinline__ void w8_lds_done() { __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local"); }  // global loads stay in flight
-__device__ __forceinline__ void w8_lds_barrier() {  // behind w8_lds_done
-    __builtin_amdgcn_s_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
-}
-
 template <int BM, int NB, int AHEAD, int XRING, bool GLU>
 __device__ __forceinline__ void tiled_body(const char* __restrict__ wt, const float* __restrict__ ws, const char* __restrict__ xq,
                                            const float* __restrict__ xs, void* __restrict__ y, int n, int kt, int t, int y_type, int act, int nks,

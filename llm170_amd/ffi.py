@@ -10,7 +10,7 @@ ERR_SHAPE, ERR_SYMBOL, ERR_UNSUPPORTED, ERR_NOT_FOUND, ERR_ARG, ERR_ASSET, ERR_S
     10001, 10002, 10003, 10004, 10005, 10006, 10007)
 PATH_AUTO, PATH_LANE, PATH_DECODE, PATH_PREFILL, PATH_STREAM = 0, 1, 2, 3, 4
 ACT_SILU, ACT_GELU_TANH = 0, 1
-F32, F16, BF16, Q8 = 0, 1, 2, 3
+F32, F16, BF16, Q8, F8 = 0, 1, 2, 3, 4
 
 
 class W4a16Error(RuntimeError):
@@ -139,6 +139,16 @@ _SIGS = {
                                              C.c_int, C.c_int]),
     "w4a16_plan_w8a8": (C.c_int, [C.c_size_t, C.c_size_t, C.c_size_t, C.c_int, C.c_int, C.c_char_p, C.c_size_t, C.POINTER(C.c_size_t),
                                   C.POINTER(C.c_int), C.POINTER(C.c_int)]),
+    "w4a16_quant_rows_f8": (C.c_int, [C.c_void_p, C.c_uint64, C.c_int, C.c_size_t, C.c_size_t, C.c_size_t, C.c_uint64, C.c_uint64]),
+    "w4a16_norm_resid_f8": (C.c_int, [C.c_void_p, C.c_uint64, C.c_uint64, C.c_uint64, C.c_uint64, C.c_uint64, C.c_size_t, C.c_size_t,
+                                      C.c_size_t]),
+    "w4a16_upload_lin_f8": (C.c_int, [C.c_void_p, C.c_char_p, C.c_void_p, C.c_size_t, C.c_void_p, C.c_size_t, C.c_size_t, C.c_size_t, C.c_int]),
+    "w4a16_lin_f8_info": (C.c_int, [C.c_void_p, C.c_char_p, C.POINTER(C.c_size_t), C.POINTER(C.c_size_t)]),
+    "w4a16_lin_forward_f8": (C.c_int, [C.c_void_p, C.c_char_p, C.c_uint64, C.c_int, C.c_size_t, C.c_uint64, C.c_size_t, C.c_uint64, C.c_int]),
+    "w4a16_lin_forward_f8_glu": (C.c_int, [C.c_void_p, C.c_char_p, C.c_uint64, C.c_int, C.c_size_t, C.c_uint64, C.c_size_t, C.c_uint64,
+                                           C.c_int, C.c_int]),
+    "w4a16_plan_f8": (C.c_int, [C.c_size_t, C.c_size_t, C.c_size_t, C.c_int, C.c_int, C.c_int, C.c_char_p, C.c_size_t, C.POINTER(C.c_size_t),
+                                C.POINTER(C.c_int), C.POINTER(C.c_int)]),
     "w4a16_token_logprobs": (C.c_int, [C.c_void_p, C.c_uint64, C.c_int, C.c_size_t, C.c_size_t, C.c_size_t, C.c_uint64, C.c_uint64,
                                        C.c_uint64, C.c_size_t, C.c_uint64, C.c_uint64]),
     "w4a16_bench_moe": (C.c_int, [C.c_void_p, C.POINTER(C.c_char_p), C.c_size_t, C.c_uint64, C.c_uint64, C.c_uint64,

@@ -69,6 +69,13 @@ def plan_w8a8(t, n, k, cu_count=256, glu=False):
     return {"kernel": name.value.decode(), "workgroups": wgs.value, "waves": waves.value, "k_slices": nks.value}
 
 
+def plan_f8(t, n, k, cu_count=256, glu=False, y_type=ffi.F16):
+    """Launch of t rows through an FP8 linear with results of y_type (no context, no GPU): dict of kernel, workgroups, waves, k_slices."""
+    name, wgs, waves, nks = C.create_string_buffer(64), C.c_size_t(), C.c_int(), C.c_int()
+    ffi.check(ffi.load().w4a16_plan_f8(n, k, t, cu_count, int(bool(glu)), y_type, name, 64, C.byref(wgs), C.byref(waves), C.byref(nks)))
+    return {"kernel": name.value.decode(), "workgroups": wgs.value, "waves": waves.value, "k_slices": nks.value}
+
+
 def check_shapes(t, qlen, slen, xlen, n, k, group):
     """gptq4.rs:31-58.  Raises W4a16Error(ERR_SHAPE) on violation."""
     ffi.check(ffi.load().w4a16_check_shapes(t, qlen, slen, xlen, n, k, group))
@@ -474,6 +481,37 @@ class W4a16Dec:
         ffi.check(self.cc.lib.w4a16_lin_forward_w8a8_glu(self.cc.h, name.encode(), x_dev, x_type, ldx, xs_dev, t, dst_dev, y_type,
                                                          ACT_GELU_TANH if gelu else ACT_SILU))
 
+    # ---- FP8 linears: e4m3 weights with a scale for each 128 x 128, activations quantised in blocks of 128 of a row
+    def upload_lin_f8(self, name, q, s, n, k):
+        """q: e4m3 bits, uint8 [n][k]; s [ceil(n / 128)][ceil(k / 128)]: float32, float16, or uint16 (bf16 bits)."""
+        q, s = np.ascontiguousarray(q), np.ascontiguousarray(s)
+        types = {"float32": ffi.F32, "float16": ffi.F16, "uint16": ffi.BF16}
+        if q.dtype != np.uint8 or s.dtype.name not in types:
+            raise W4a16Error(ffi.ERR_ARG, "upload_lin_f8 %s: q %s, s %s (uint8, and float32, float16 or uint16)" % (name, q.dtype, s.dtype))
+        ffi.check(self.cc.lib.w4a16_upload_lin_f8(self.cc.h, name.encode(), _ptr(q), q.nbytes, _ptr(s), s.nbytes, n, k, types[s.dtype.name]))
+
+    def lin_f8_spec(self, name):
+        n, k = C.c_size_t(), C.c_size_t()
+        ffi.check(self.cc.lib.w4a16_lin_f8_info(self.cc.h, name.encode(), C.byref(n), C.byref(k)))
+        return {"n": n.value, "k": k.value}
+
+    def quant_rows_f8(self, x_dev, q_dev, s_dev, t, k, x_type=ffi.F16, ldx=0):
+        """q <- x in steps of a power of two for each 128 of a row, in tiles (q8_bytes(t, k) bytes; unpack_q8 reads their bits back), s [ceil(k / 128)][t]."""
+        ffi.check(self.cc.lib.w4a16_quant_rows_f8(self.cc.h, x_dev, x_type, ldx, t, k, q_dev, s_dev))
+
+    def norm_resid_f8(self, x_dev, nw_dev, ab_dev, q_dev, s_dev, t, hidden, w_off=0):
+        """norm_resid and quant_rows_f8 of its result in one launch: x <- x + ab; q, s <- the normalised rows."""
+        ffi.check(self.cc.lib.w4a16_norm_resid_f8(self.cc.h, x_dev, nw_dev, ab_dev, q_dev, s_dev, t, w_off, hidden))
+
+    def lin_forward_f8(self, name, x_dev, dst_dev, t, x_type=ffi.F16, ldx=0, xs_dev=0, y_type=ffi.F32):
+        """y [t][n]; x in rows of floats, quantised on the way, or x_type F8: what quant_rows_f8 or norm_resid_f8 wrote for t rows."""
+        ffi.check(self.cc.lib.w4a16_lin_forward_f8(self.cc.h, name.encode(), x_dev, x_type, ldx, xs_dev, t, dst_dev, y_type))
+
+    def lin_forward_f8_glu(self, name, x_dev, dst_dev, t, x_type=ffi.F16, ldx=0, xs_dev=0, y_type=ffi.F16, gelu=False):
+        """act(gate) * up of a fused gate|up linear (rows 0..n/2 gate), y [t][n/2]."""
+        ffi.check(self.cc.lib.w4a16_lin_forward_f8_glu(self.cc.h, name.encode(), x_dev, x_type, ldx, xs_dev, t, dst_dev, y_type,
+                                                       ACT_GELU_TANH if gelu else ACT_SILU))
+
     # ---- scoring of logits
     def token_logprobs(self, logits_dev, t, n_vocab, logits_type=ffi.F32, ld=0, targets_dev=0, logp_dev=0, entropy_dev=0, top_k=0,
                        top_idx_dev=0, top_logp_dev=0):
@@ -549,7 +587,7 @@ def q8_bytes(t, k):
 
 
 def unpack_q8(q, t, k):
-    """Rows int8 [t][k] from what quant_rows or norm_resid_q8 wrote (q: q8_bytes(t, k) bytes, on the host)."""
+    """Rows int8 [t][k] from what quant_rows or norm_resid_q8 wrote (q: q8_bytes(t, k) bytes, on the host); of e4m3 rows their bits."""
     r = 1 if t == 1 else 4 if t <= 4 else 16
     tiles = np.ascontiguousarray(q).reshape(-1).view(np.int8).reshape(-(-t // r), -(-k // 128) * 8, r, 16)
     return tiles.transpose(0, 2, 1, 3).reshape(-(-t // r) * r, -1)[:t, :k].copy()
