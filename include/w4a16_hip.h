@@ -595,6 +595,42 @@ int w4a16_plan_f8(size_t n, size_t k, size_t t, int cu_count, int glu, int y_typ
 int w4a16_token_logprobs(w4a16_ctx* ctx, uint64_t logits_dev, int logits_type, size_t ld, size_t t, size_t n_vocab, uint64_t targets_dev,
                          uint64_t logp_dev, uint64_t entropy_dev, size_t top_k, uint64_t top_idx_dev, uint64_t top_logp_dev);
 
+/* Verifies drafted tokens against a target's distributions, from given random numbers.  Sequence b has rows row0[b] .. row0[b + 1] - 1 (row0 int32 [seqs + 1], ascending,
+ * within 0..t; none, or one with no draft, are fine) of target logits [t][n_vocab] (f32, f16 or bf16, rows ld elements apart, 0 = n_vocab): its row i judges its drafted token i
+ * and the last row is what follows when all are accepted.  drafted int32 [t] and u f32 [t], numbers of [0, 1), lie by the same rows; draft_dev [t][n_vocab] (rows ld_draft
+ * apart, 0 = n_vocab), of the logits' type, holds the draft's own logits, 0: each drafted token was certain to its draft.  Of a sequence's last row the drafted token
+ * and the draft's logits are not used, and its u is the number that draws.
+ * With p and q the softmax of target and draft logits over temps[b] (f32 [seqs], 0: all 1), a drafted token x is accepted while u q(x) < p(x).  Behind the last one accepted
+ * comes one token more: the first whose running sum of max(0, p - q) where one was rejected (of p, where that is zero everywhere), of p behind the last draft, in the order of
+ * tokens, exceeds the sequence's last u times the whole sum.  A temperature that is not above 0: accepted is the most likely token (of equal ones the lowest), which also
+ * follows.  Powers and sums are of 64 bits.
+ *   tokens int32 [t]: of each sequence the accepted tokens, the one that follows, -1 for the rest of its rows (tokens may be drafted); accepted int32 [seqs]: how many were.
+ * Rows of no sequence are left as they are.  -infinity rules a token out.  A target's row that holds NaN or +infinity, or nothing but -infinity, has no distribution: its draft
+ * is rejected and -1 follows.  Where a draft's row has none, or a drafted token is none of the vocabulary, it is rejected and p (without that token, if it was certain) is drawn from. */
+int w4a16_verify_drafts(w4a16_ctx* ctx, uint64_t logits_dev, int logits_type, size_t ld, uint64_t draft_dev, size_t ld_draft, size_t t, size_t n_vocab,
+                        uint64_t row0_dev, size_t seqs, uint64_t drafted_dev, uint64_t u_dev, uint64_t temps_dev, uint64_t tokens_dev, uint64_t accepted_dev);
+
+/* ------------------------------------------------------------------------------------------------------------
+ * Queries and keys of a QKV projection: every head's norm and the rotation by position, in one launch
+ * ---------------------------------------------------------------------------------------------------------- */
+
+/* Frequencies of a rotation of rot_dim (even) elements, freqs f64 [rot_dim / 2] in radians per position, and the factor amp of cosines and sines, on the host; needs neither a
+ * context nor a GPU.  Plain: f_c = base^(-2 c / rot_dim).  For contexts longer than the `trained` one, by `factor`: LINEAR f / factor.  BANDS: f keeps a share of
+ * (trained * f / 2 pi - low) / (high - low), cut to 0..1, and has f / factor for the rest.  RAMP: the share falls from 1 to 0 over the pairs between the one that turns `high` times within
+ * the trained length (rounded down, 0 at least) and the one that turns `low` times (rounded up, rot_dim - 1 at most); amp = 0.1 ln(factor) + 1 for a factor above 1, else 1. */
+enum { W4A16_ROPE_PLAIN = 0, W4A16_ROPE_LINEAR = 1, W4A16_ROPE_BANDS = 2, W4A16_ROPE_RAMP = 3 };
+int w4a16_rope_freqs(size_t rot_dim, double base, int scaling, double factor, double trained, double low, double high, double* freqs, float* amp);
+
+/* x [t][...] (f32, f16 or bf16, rows ldx elements apart, 0 = (n_q + n_k) * head_dim): n_q heads of queries, n_k of keys (either may be 0), then whatever the row holds besides.
+ * Every head v [head_dim] (up to 1024): v / sqrt(mean v^2 + eps) * w, w f32 [head_dim] = qw for queries and kw for keys, where they are not 0; then the pairs (a, b) of its first rot_dim
+ * elements (even; 0: none) become (a cos - b sin, b cos + a sin), cosine and sine of pos[row] * freqs[pair] times amp: (c, c + rot_dim / 2), or (2 c, 2 c + 1) where interleaved != 0.
+ * pos int32 [t]; freqs f64 [rot_dim / 2]; angles are reduced in 64 bits.  f32 arithmetic, rounded once to y_type.
+ * Results: q [t][n_q][head_dim] with rows ldq apart, k likewise (0 = without gaps).  They may be x's own heads, in place (the same type and stride, q_dev = x_dev, k_dev behind the
+ * queries); otherwise they overlap neither x nor each other. */
+int w4a16_qk_norm_rope(w4a16_ctx* ctx, uint64_t x_dev, int x_type, size_t ldx, size_t t, size_t n_q, size_t n_k, size_t head_dim, uint64_t qw_dev, uint64_t kw_dev,
+                       float eps, uint64_t pos_dev, uint64_t freqs_dev, size_t rot_dim, float amp, int interleaved, uint64_t q_dev, size_t ldq, uint64_t k_dev, size_t ldk,
+                       int y_type);
+
 #ifdef __cplusplus
 }
 #endif

@@ -126,6 +126,10 @@ static const char* const kF8QuantSyms[] = {"w4a16_quant_rows_f8_f32", "w4a16_qua
 static const char* const kF8Syms[] = {W8_TT("w4a16_f8_skinny_r1", ""), W8_TT("w4a16_f8_skinny_r2", ""), W8_TT("w4a16_f8_skinny_r4", ""),
                                       W8_TT("w4a16_f8_skinny_r2", "_glu"), W8_TT("w4a16_f8_skinny_r4", "_glu"),
                                       F8_TILES("w4a16_f8_tiled"), F8_TILES("w4a16_f8_exact"), nullptr};
+#define ROPE_BUILDS(P) P "_v8", P "_v2", P "_v1", P "_v8_il", P "_v2_il", P "_v1_il"  // pairs to a lane; neighbours as pairs (kernels/rope.hip)
+static const char* const kRopeSyms[] = {ROPE_BUILDS("w4a16_qk_norm_rope_f32"), ROPE_BUILDS("w4a16_qk_norm_rope_f16"), ROPE_BUILDS("w4a16_qk_norm_rope_bf16"), nullptr};
+static const char* const kVerifySyms[] = {"w4a16_verify_rows_f32", "w4a16_verify_rows_f16", "w4a16_verify_rows_bf16", "w4a16_verify_pick_f32", "w4a16_verify_pick_f16",
+                                          "w4a16_verify_pick_bf16", nullptr};
 static const char* const kScoreSyms[] = {"w4a16_token_logprobs_f32", "w4a16_token_logprobs_f16", "w4a16_token_logprobs_bf16", nullptr};
 
 struct W4Asset {
@@ -147,6 +151,8 @@ static const W4Asset kAssets[] = {
     {"f8_quant", kF8QuantSyms},
     {"f8", kF8Syms},
     {"score", kScoreSyms},
+    {"rope", kRopeSyms},
+    {"verify", kVerifySyms},
 };
 static const size_t kAssetCount = sizeof kAssets / sizeof kAssets[0];
 

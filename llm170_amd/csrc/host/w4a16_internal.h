@@ -101,6 +101,8 @@ struct w4a16_ctx {
     size_t q8_cap = 0, q8_scales_cap = 0;
     uint64_t w8_part = 0, w8_tickets = 0;  // sums of the k slices of a W8A8 or FP8 launch, one ticket per workgroup of a slice
     size_t w8_part_cap = 0, w8_tickets_cap = 0;
+    uint64_t verify_ws = 0, verify_tickets = 0;  // verification of drafts: sums of the rows' segments, what is known of each row; a ticket per row and per sequence
+    size_t verify_ws_cap = 0, verify_tickets_cap = 0;
     uint64_t score_ws = 0, score_tickets = 0;  // records of the segments of a row of logits, one ticket per row
     size_t score_ws_cap = 0, score_tickets_cap = 0;
     W4MoeScratch moe;
@@ -151,6 +153,9 @@ constexpr int kW4Q8MaxK = 131071;           // Q8_MAX_K (q8_common.hpp)
 constexpr int kW4ScoreStageBytes = 4096;    // SCORE_STAGE_BYTES (score.hip): of a wave's stage, four waves to a workgroup
 constexpr int kW4ScoreMaxTop = 32;          // SCORE_MAX_TOP
 constexpr int kW4ScoreRecord = 272;         // SCORE_RECORD
+
+constexpr int kW4RopeMaxDim = 1024;         // ROPE_MAX_DIM (rope.hip)
+constexpr int kW4VerifyMaxSegment = 16384;  // VERIFY_MAX_SEGMENT (verify.hip)
 
 int w4_fail(int code, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
 int w4_hip(hipError_t e, const char* api);

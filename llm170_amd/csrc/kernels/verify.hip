@@ -1,0 +1,397 @@
+// Verification of drafted tokens against the target's distributions, from given random numbers.  A sequence has rows row0[b] .. row0[b + 1] - 1 of target logits: row i judges
+// drafted token i, the last one is what follows when all are accepted.  With p, q the softmax of target and draft logits over the temperature, token x of row i is
+// accepted while u_i q(x) < p(x); behind the last accepted one a token is drawn from max(0, p - q) at the first row that is not, from p at the last row: the first whose
+// running sum exceeds u_last times the whole sum.  Temperature 0: accepted is the most likely token, which also follows.
+//
+// Running sums over a vocabulary meet a border between two tokens about once in V / (relative error) draws, so powers and sums are of 64 bits: 2^x by a polynomial of
+// degree 8 (interpolation at Chebyshev nodes of [-1/2, 1/2], off by 1.1e-12), 17 instructions an element, which the stream of the logits about hides.
+//
+// Two launches.  Rows: a segment of a target's or a draft's row to a workgroup, with a running maximum in each thread; it leaves (sum, maximum) of its segment, and the last of
+// a row joins them and judges the row's token.  Pick: a sequence finds its first row that is not accepted.  What is drawn from p alone knows its segments' sums already,
+// finds the segment and goes over that; only max(0, p - q) takes a pass over both rows, a segment to a workgroup, the last of which finds the segment.  Within a segment a thread
+// sums a run of neighbours, and the run that holds the draw is gone over again, an element to a lane.
+#include "score_common.hpp"
+
+#define VERIFY_WAVES 4
+#define VERIFY_MAX_SEGMENT 16384  // elements: 64 to each thread that goes over it again
+
+typedef unsigned long long bits_t;
+
+struct VerifyRow {  // what is known of a row: sum 0 where it has no distribution
+    double s, sd;
+    float m, md;
+    int best, accepted;
+};
+struct VerifySum {  // of a segment: sum of powers relative to its maximum; or the key of its largest element; or the sum of max(0, p - q)
+    double s;
+    float m;
+    int pad;
+};
+
+// 2^x, x <= 0; a NaN counts as far below
+__device__ __forceinline__ double verify_exp2(double x) {
+    x = __builtin_fmax(x, -1100.0);
+    const double n = __builtin_rint(x), f = x - n;
+    double p = 1.3255224878668817e-06;
+    p = __builtin_fma(p, f, 1.5310079402249296e-05);
+    p = __builtin_fma(p, f, 0.00015403455852453838);
+    p = __builtin_fma(p, f, 0.0013333450568000645);
+    p = __builtin_fma(p, f, 0.009618129159402558);
+    p = __builtin_fma(p, f, 0.05550410941205933);
+    p = __builtin_fma(p, f, 0.2402265069581299);
+    p = __builtin_fma(p, f, 0.6931471805459335);
+    p = __builtin_fma(p, f, 1.0);
+    return __builtin_ldexp(p, (int)n);
+}
+// the power of logit v relative to the maximum m; c = log2 e / temperature
+__device__ __forceinline__ double verify_power(float v, float m, double c) { return verify_exp2(((double)v - (double)m) * c); }
+// a segment's sum relative to the maximum of its row
+__device__ __forceinline__ double verify_share(VerifySum a, float m, double c) { return a.s > 0.0 ? a.s * verify_power(a.m, m, c) : 0.0; }
+
+__device__ __forceinline__ double verify_factor(float temp) { return 1.4426950408889634074 / (double)temp; }
+
+__device__ __forceinline__ double verify_wave_sum(double v) {
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) v += __shfl_xor(v, d);
+    return v;
+}
+__device__ __forceinline__ double verify_wave_scan(double v) {  // of this lane and all below
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const double o = __shfl_up(v, d);
+        if (lane >= d) v += o;
+    }
+    return v;
+}
+
+__device__ __forceinline__ void verify_put(VerifySum* p, VerifySum v) {  // device scope: past this XCD's L2
+    bits_t* const b = reinterpret_cast<bits_t*>(p);
+    __hip_atomic_store(b, __builtin_bit_cast(bits_t, v.s), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __hip_atomic_store(b + 1, (bits_t)__builtin_bit_cast(unsigned, v.m), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ VerifySum verify_get(const VerifySum* p) {
+    const bits_t* const b = reinterpret_cast<const bits_t*>(p);
+    const bits_t s = __hip_atomic_load(b, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT), m = __hip_atomic_load(b + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    return {__builtin_bit_cast(double, s), q8_f32((unsigned)m), 0};
+}
+
+template <int T>
+__device__ __forceinline__ void verify_rows_body(const void* __restrict__ logits, size_t ld, const void* __restrict__ draft, size_t ldd, int vocab, int t, int row_first,
+                                                 const int* __restrict__ row0, int seqs, const int* __restrict__ drafted, const float* __restrict__ u,
+                                                 const float* __restrict__ temps, int segs, int seg_len, VerifySum* __restrict__ sums, VerifyRow* __restrict__ rows,
+                                                 int* __restrict__ tickets) {
+    __shared__ double red[VERIFY_WAVES];
+    __shared__ float redm[VERIFY_WAVES];
+    __shared__ int counts[VERIFY_WAVES];
+    __shared__ int last_one;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const unsigned streams = draft ? 2 : 1, per_row = (unsigned)segs * streams;
+    const int row = row_first + (int)(blockIdx.x / per_row);
+    const unsigned in_row = blockIdx.x % per_row;
+    const bool of_draft = in_row >= (unsigned)segs;
+    const int seg = (int)(of_draft ? in_row - segs : in_row);
+    constexpr int SIZE = ScoreChunk<T>::SIZE, E = ScoreChunk<T>::E;
+    constexpr unsigned STAGE = ScoreChunk<T>::STAGE, STEP = VERIFY_WAVES * STAGE;
+    const char* const z = static_cast<const char*>(of_draft ? draft : logits) + (size_t)row * (of_draft ? ldd : ld) * SIZE;
+    const unsigned lo = (unsigned)seg * (unsigned)seg_len, hi = min(lo + (unsigned)seg_len, (unsigned)vocab);
+    unsigned i = lo + wave * STAGE;
+    ScoreChunk<T> next;  // asked for ahead of what the row is
+    auto load = [&]() { next.load(z + (size_t)i * SIZE, hi > i ? hi - i : 0u, lane); };
+    load();
+    // The starts at or below the row, `below` of them: 256 probes at a time
+    int below = 0;
+    for (int n = seqs, step;; ) {
+        step = (n + 255) >> 8;
+        const int at = (int)threadIdx.x * step;
+        const int here = __popcll(__ballot(at < n && row0[below + min(at, n - 1)] <= row));
+        __syncthreads();
+        if (lane == 0) counts[wave] = here;
+        __syncthreads();
+        const int c = counts[0] + counts[1] + counts[2] + counts[3];
+        if (c == 0) return;  // ahead of the first sequence
+        below += (c - 1) * step;
+        n = min(step, n - (c - 1) * step);
+        if (step == 1) break;
+    }
+    below++;
+    const int end = min(row0[below], t);
+    if (row >= end) return;  // behind the last sequence
+    const bool last = row == end - 1;
+    const float temp = temps ? temps[below - 1] : 1.f;
+    const bool greedy = !(temp > 0.f), both = draft && !last && !greedy;
+    if (of_draft && !both) return;
+    const double c = greedy ? 0.0 : verify_factor(temp);
+
+    VerifySum mine = {0.0, -__builtin_inff(), 0};
+    unsigned best = 0;
+    for (;; i += STEP) {
+        const ScoreChunk<T> cur = next;
+        const unsigned here = i;
+        if (i + STEP < hi) next.load(z + (size_t)(i + STEP) * SIZE, hi - i - STEP, lane);
+        float most, least;
+        cur.extremes(most, least);
+        if (greedy) {
+            if (!(most <= mine.m)) {  // later elements of equal size come later; a NaN stays
+                mine.m = __builtin_elementwise_maximum(most, mine.m);
+                unsigned at = 0;
+#pragma unroll
+                for (int e = E - 1; e >= 0; e--)
+                    if (cur.value(e) == most) at = here + ScoreChunk<T>::at(lane, e);
+                best = at;
+            }
+        } else {
+            const float m = __builtin_elementwise_maximum(most, mine.m);
+            if (!(m == mine.m)) {
+                mine.s = mine.s > 0.0 ? mine.s * verify_power(mine.m, m, c) : 0.0;
+                mine.m = m;
+            }
+            const float mm = mine.m == -__builtin_inff() ? 0.f : mine.m;  // nothing so far: every element is -infinity
+#pragma unroll
+            for (int e = 0; e < E; e++) mine.s += verify_power(cur.value(e), mm, c);
+        }
+        if (i + STEP >= hi) break;
+    }
+    // the workgroup's sum; or the key of its largest, the lower index of equal ones
+    if (greedy) {
+        bits_t key = (bits_t)score_order(mine.m) << 32 | (0xffffffffu - best);
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) key = max(key, (bits_t)__shfl_xor((unsigned long long)key, d));
+        if (lane == 0) red[wave] = __builtin_bit_cast(double, key);
+    } else {
+        const float m = score_wave_max(mine.m);
+        const double s = verify_wave_sum(verify_share(mine, m, c));
+        if (lane == 0) {
+            red[wave] = s;
+            redm[wave] = m;
+        }
+    }
+    __syncthreads();
+    VerifySum* const of_row = sums + (size_t)row * per_row;
+    if (threadIdx.x == 0) {
+        VerifySum all = {red[0], redm[0], 0};
+        if (greedy) {
+            bits_t key = __builtin_bit_cast(bits_t, red[0]);
+            for (int w = 1; w < VERIFY_WAVES; w++) key = max(key, __builtin_bit_cast(bits_t, red[w]));
+            all = {__builtin_bit_cast(double, key), 0.f, 0};
+        } else {
+            for (int w = 1; w < VERIFY_WAVES; w++) all.m = __builtin_elementwise_maximum(all.m, redm[w]);
+            all.s = 0.0;
+            for (int w = 0; w < VERIFY_WAVES; w++) all.s += verify_share({red[w], redm[w], 0}, all.m, c);
+        }
+        verify_put(of_row + in_row, all);
+        // complete before the ticket is drawn; read behind the barrier that follows its return
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        last_one = __hip_atomic_fetch_add(tickets + row, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == segs * (both ? 2 : 1) - 1;
+    }
+    __syncthreads();
+    if (!last_one) return;
+    if (threadIdx.x == 0) __hip_atomic_store(tickets + row, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);  // for the next launch
+    if (wave != 0) return;
+    VerifyRow r = {0.0, 0.0, 0.f, 0.f, 0, 0};
+    const int x = last ? -1 : drafted[row];
+    const bool there = x >= 0 && x < vocab;
+    if (greedy) {
+        bits_t key = 0;
+        for (int s = lane; s < segs; s += 64) key = max(key, __builtin_bit_cast(bits_t, verify_get(of_row + s).s));
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) key = max(key, (bits_t)__shfl_xor((unsigned long long)key, d));
+        const unsigned order = (unsigned)(key >> 32);
+        r.best = (int)(0xffffffffu - (unsigned)key);
+        r.s = order > score_order(-__builtin_inff()) && order < score_order(__builtin_inff()) ? 1.0 : 0.0;
+        r.accepted = r.s > 0.0 && there && x == r.best;
+    } else {
+        auto join = [&](const VerifySum* of, float& m, double& s) {
+            VerifySum a = {0.0, -__builtin_inff(), 0};
+            for (int k = lane; k < segs; k += 64) {
+                const VerifySum v = verify_get(of + k);
+                const float both_m = __builtin_elementwise_maximum(a.m, v.m);
+                a.s = verify_share(a, both_m, c) + verify_share(v, both_m, c);
+                a.m = both_m;
+            }
+            m = score_wave_max(a.m);
+            s = verify_wave_sum(verify_share(a, m, c));
+            if (!(__builtin_fabsf(m) < __builtin_inff())) s = 0.0;  // nothing, infinity or NaN
+        };
+        join(of_row, r.m, r.s);
+        if (both) join(of_row + segs, r.md, r.sd);
+        if (there && r.s > 0.0) {
+            const double p = verify_power(q8_load1<T>(static_cast<const char*>(logits) + (size_t)row * ld * SIZE, (size_t)x), r.m, c) / r.s;
+            double q = 1.0;
+            if (both && r.sd > 0.0) q = verify_power(q8_load1<T>(static_cast<const char*>(draft) + (size_t)row * ldd * SIZE, (size_t)x), r.md, c) / r.sd;
+            r.accepted = (!both || r.sd > 0.0) && (double)u[row] * q < p;
+        }
+    }
+    if (lane == 0) rows[row] = r;
+}
+
+// The first of 256 values, one per thread, whose running sum from `before` on exceeds `aim`; else (`none`) the last one above zero; else -1.  `before` becomes the sum ahead of the first
+// kind; of every value it is in `starts`, and the waves' sums are in `red`.  All threads get the same.
+__device__ __forceinline__ int verify_find(double v, double aim, double& before, double* red, int* found, double* starts, bool& none) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const double run = verify_wave_scan(v);
+    __syncthreads();
+    if (lane == 63) red[wave] = run;
+    if (threadIdx.x < 2) found[threadIdx.x] = threadIdx.x == 0 ? 256 : -1;
+    __syncthreads();
+    double ahead = before;
+    for (int w = 0; w < wave; w++) ahead += red[w];
+    const bool over = ahead + run > aim && v > 0.0;
+    const unsigned long long those = __ballot(over), some = __ballot(v > 0.0);
+    if (lane == 0) {
+        if (those) atomicMin(&found[0], wave * 64 + __builtin_ctzll(those));
+        if (some) atomicMax(&found[1], wave * 64 + 63 - __builtin_clzll(some));
+    }
+    starts[threadIdx.x] = ahead + (run - v);
+    __syncthreads();
+    none = found[0] == 256;
+    const int at = none ? found[1] : found[0];
+    if (!none) before = starts[at];
+    return at;
+}
+
+template <int T>
+__device__ __forceinline__ void verify_pick_body(const void* __restrict__ logits, size_t ld, const void* __restrict__ draft, size_t ldd, int vocab, int t, int seq_first,
+                                                 const int* __restrict__ row0, const int* drafted, const float* __restrict__ u, const float* __restrict__ temps,
+                                                 int segs, int seg_len, const VerifySum* __restrict__ sums, const VerifyRow* __restrict__ rows,
+                                                 VerifySum* __restrict__ parts, int* __restrict__ tickets, int* tokens, int* __restrict__ accepted) {
+    __shared__ double red[VERIFY_WAVES], starts[256];
+    __shared__ int found[2];
+    __shared__ int last_one, chosen;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), tid = threadIdx.x;
+    const int b = seq_first + (int)(blockIdx.x / (unsigned)segs), seg = (int)(blockIdx.x % (unsigned)segs);
+    const int r0 = min(max(row0[b], 0), t), r1 = min(max(row0[b + 1], r0), t);
+    if (r0 >= r1) {
+        if (seg == 0 && tid == 0) accepted[b] = 0;
+        return;
+    }
+    int stop = r1 - 1;
+    for (int from = r0; from < r1 - 1; from += 64) {
+        const unsigned long long no = __ballot(from + lane < r1 - 1 && rows[min(from + lane, r1 - 1)].accepted == 0);
+        if (no) {
+            stop = from + __builtin_ctzll(no);
+            break;
+        }
+    }
+    const VerifyRow r = rows[stop];
+    const float temp = temps ? temps[b] : 1.f;
+    const bool greedy = !(temp > 0.f), last = stop == r1 - 1, residual = !greedy && r.s > 0.0 && draft && !last && r.sd > 0.0;
+    if (seg != 0 && !residual) return;
+    const double c = greedy ? 0.0 : verify_factor(temp);
+    int token = greedy && r.s > 0.0 ? r.best : -1;
+    if (!greedy && r.s > 0.0) {
+        constexpr int SIZE = T == Q8_F32 ? 4 : 2;
+        const char* const z = static_cast<const char*>(logits) + (size_t)stop * ld * SIZE;
+        const char* const zd = static_cast<const char*>(draft) + (size_t)stop * ldd * SIZE;
+        const unsigned streams = draft ? 2 : 1;
+        const VerifySum* const of_row = sums + (size_t)stop * segs * streams;
+        const double inv = 1.0 / r.s, inv_d = residual ? 1.0 / r.sd : 0.0;
+        // what is left out: the token that was certain to its draft
+        const int x = last || draft ? -1 : drafted[stop];
+        const int run = (seg_len + 4095) / 4096 * 16;  // neighbours to a thread
+        int out = x;
+        bool only_p = !residual;
+        auto weight = [&](float v, float d, int at) {
+            const double p = verify_power(v, r.m, c) * inv;
+            if (only_p) return at == out ? 0.0 : p;
+            return __builtin_fmax(p - verify_power(d, r.md, c) * inv_d, 0.0);
+        };
+        // the sum of this thread's run of segment s
+        auto of_run = [&](int s) {
+            const int from = s * seg_len + tid * run, to = min(min(from + run, (s + 1) * seg_len), vocab);
+            double sum = 0.0;
+            for (int at = from; at < to; at += 16) {
+                float v[16], d[16];
+                q8_load16<T>(z, (size_t)at, to - at, v);
+                if (!only_p) q8_load16<T>(zd, (size_t)at, to - at, d);
+#pragma unroll
+                for (int e = 0; e < 16; e++) {
+                    const double w = weight(v[e], only_p ? 0.f : d[e], at + e);
+                    sum += at + e < to ? w : 0.0;
+                }
+            }
+            return sum;
+        };
+        if (residual) {
+            const double mine = verify_wave_sum(of_run(seg));
+            if (lane == 0) red[wave] = mine;
+            __syncthreads();
+            if (tid == 0) {
+                verify_put(parts + (size_t)b * segs + seg, {red[0] + red[1] + red[2] + red[3], 0.f, 0});
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                last_one = __hip_atomic_fetch_add(tickets + b, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == segs - 1;
+            }
+            __syncthreads();
+            if (!last_one) return;
+            if (tid == 0) __hip_atomic_store(tickets + b, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);  // for the next launch
+        }
+        // a segment's sum
+        auto of_segment = [&](int s) {
+            if (s >= segs) return 0.0;
+            if (!only_p) return verify_get(parts + (size_t)b * segs + s).s;
+            double p = verify_share(of_row[s], r.m, c) * inv;
+            if (out >= 0 && out < vocab && out / seg_len == s) p = __builtin_fmax(p - verify_power(q8_load1<T>(z, (size_t)out), r.m, c) * inv, 0.0);
+            return p;
+        };
+        auto total = [&]() {
+            double sum = 0.0;
+            for (int s = tid; s < segs; s += 256) sum += of_segment(s);
+            sum = verify_wave_sum(sum);
+            __syncthreads();
+            if (lane == 0) red[wave] = sum;
+            __syncthreads();
+            return red[0] + red[1] + red[2] + red[3];
+        };
+        // Drawn from p where p is nowhere above q, or where what a rounding left over a segment's certain token is drawn
+        for (int attempt = 0; attempt < 2 && token < 0; attempt++) {
+            if (attempt == 1) only_p = true, out = -1;
+            const double all = total();
+            if (!(all > 0.0)) continue;
+            const double aim = (double)u[r1 - 1] * all;
+            double before = 0.0, from = 0.0;
+            int at = -1;
+            bool none = true;
+            for (int s = 0; s < segs && none; s += 256) {
+                double ahead = from;
+                const int f = verify_find(of_segment(s + tid), aim, ahead, red, found, starts, none);
+                if (f >= 0) {
+                    at = s + f;
+                    before = none ? starts[f] : ahead;
+                }
+                from += red[0] + red[1] + red[2] + red[3];
+            }
+            if (at < 0) continue;
+            if (tid == 0) chosen = -1;
+            const int f = verify_find(of_run(at), aim, before, red, found, starts, none);
+            if (f >= 0 && wave == 0) {
+                if (none) before = starts[f];
+                const int e = at * seg_len + f * run + lane;
+                const bool in = lane < run && e < min((at + 1) * seg_len, vocab);
+                const float v = in ? q8_load1<T>(z, (size_t)e) : 0.f, d = in && !only_p ? q8_load1<T>(zd, (size_t)e) : 0.f;
+                const double w = in ? weight(v, d, e) : 0.0, run_to = before + verify_wave_scan(w);  // by all lanes
+                const unsigned long long those = __ballot(w > 0.0 && run_to > aim), some = __ballot(w > 0.0);
+                if (lane == 0 && some) chosen = e + (those ? __builtin_ctzll(those) : 63 - __builtin_clzll(some));
+            }
+            __syncthreads();
+            token = chosen;
+        }
+    }
+    for (int i = r0 + tid; i < r1; i += 256) tokens[i] = i < stop ? drafted[i] : i == stop ? token : -1;
+    if (tid == 0) accepted[b] = stop - r0;
+}
+
+#define VERIFY_KERNELS(NAME, T)                                                                                                    \
+    extern "C" __global__ __launch_bounds__(256) void w4a16_verify_rows_##NAME(                                                    \
+        const void* logits, size_t ld, const void* draft, size_t ldd, int vocab, int t, int row_first, const int* row0, int seqs, const int* drafted, \
+        const float* u, const float* temps, int segs, int seg_len, VerifySum* sums, VerifyRow* rows, int* tickets) {               \
+        verify_rows_body<T>(logits, ld, draft, ldd, vocab, t, row_first, row0, seqs, drafted, u, temps, segs, seg_len, sums, rows, tickets); \
+    }                                                                                                                              \
+    extern "C" __global__ __launch_bounds__(256) void w4a16_verify_pick_##NAME(                                                    \
+        const void* logits, size_t ld, const void* draft, size_t ldd, int vocab, int t, int seq_first, const int* row0, const int* drafted, const float* u, \
+        const float* temps, int segs, int seg_len, const VerifySum* sums, const VerifyRow* rows, VerifySum* parts, int* tickets, int* tokens, \
+        int* accepted) {                                                                                                           \
+        verify_pick_body<T>(logits, ld, draft, ldd, vocab, t, seq_first, row0, drafted, u, temps, segs, seg_len, sums, rows, parts, tickets, tokens, accepted); \
+    }
+VERIFY_KERNELS(f32, Q8_F32)
+VERIFY_KERNELS(f16, Q8_F16)
+VERIFY_KERNELS(bf16, Q8_BF16)

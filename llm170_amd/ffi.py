@@ -11,6 +11,7 @@ ERR_SHAPE, ERR_SYMBOL, ERR_UNSUPPORTED, ERR_NOT_FOUND, ERR_ARG, ERR_ASSET, ERR_S
 PATH_AUTO, PATH_LANE, PATH_DECODE, PATH_PREFILL, PATH_STREAM = 0, 1, 2, 3, 4
 ACT_SILU, ACT_GELU_TANH = 0, 1
 F32, F16, BF16, Q8, F8 = 0, 1, 2, 3, 4
+ROPE_PLAIN, ROPE_LINEAR, ROPE_BANDS, ROPE_RAMP = 0, 1, 2, 3
 
 
 class W4a16Error(RuntimeError):
@@ -151,6 +152,10 @@ _SIGS = {
                                 C.POINTER(C.c_int), C.POINTER(C.c_int)]),
     "w4a16_token_logprobs": (C.c_int, [C.c_void_p, C.c_uint64, C.c_int, C.c_size_t, C.c_size_t, C.c_size_t, C.c_uint64, C.c_uint64,
                                        C.c_uint64, C.c_size_t, C.c_uint64, C.c_uint64]),
+    "w4a16_verify_drafts": (C.c_int, [C.c_void_p, C.c_uint64, C.c_int, C.c_size_t, C.c_uint64] + [C.c_size_t] * 3 + [C.c_uint64, C.c_size_t] + [C.c_uint64] * 5),
+    "w4a16_rope_freqs": (C.c_int, [C.c_size_t, C.c_double, C.c_int] + [C.c_double] * 4 + [C.c_void_p, C.POINTER(C.c_float)]),
+    "w4a16_qk_norm_rope": (C.c_int, [C.c_void_p, C.c_uint64, C.c_int] + [C.c_size_t] * 5 + [C.c_uint64, C.c_uint64, C.c_float, C.c_uint64, C.c_uint64, C.c_size_t,
+                                     C.c_float, C.c_int, C.c_uint64, C.c_size_t, C.c_uint64, C.c_size_t, C.c_int]),
     "w4a16_bench_moe": (C.c_int, [C.c_void_p, C.POINTER(C.c_char_p), C.c_size_t, C.c_uint64, C.c_uint64, C.c_uint64,
                                   C.c_size_t, C.c_size_t, C.c_uint64, C.c_size_t, C.c_size_t, C.POINTER(C.c_float),
                                   C.POINTER(C.c_double)]),

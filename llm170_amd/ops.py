@@ -519,6 +519,20 @@ class W4a16Dec:
         ffi.check(self.cc.lib.w4a16_token_logprobs(self.cc.h, logits_dev, logits_type, ld, t, n_vocab, targets_dev, logp_dev, entropy_dev,
                                                    top_k, top_idx_dev, top_logp_dev))
 
+    # ---- verification of drafted tokens
+    def verify_drafts(self, logits_dev, drafted_dev, row0_dev, u_dev, tokens_dev, accepted_dev, t, seqs, n_vocab, logits_type=ffi.F32, ld=0, draft_dev=0, ld_draft=0,
+                      temps_dev=0):
+        """Per sequence (rows row0[b] .. row0[b + 1] - 1 of t): the drafted tokens that the target accepts, the token that follows, then -1; how many were accepted."""
+        ffi.check(self.cc.lib.w4a16_verify_drafts(self.cc.h, logits_dev, logits_type, ld, draft_dev, ld_draft, t, n_vocab, row0_dev, seqs, drafted_dev, u_dev, temps_dev,
+                                                  tokens_dev, accepted_dev))
+
+    # ---- queries and keys
+    def qk_norm_rope(self, x_dev, q_dev, k_dev, pos_dev, freqs_dev, t, n_q, n_k, head_dim, rot_dim, x_type=ffi.F16, ldx=0, y_type=ffi.F16, ldq=0, ldk=0, qw_dev=0, kw_dev=0,
+                     eps=1e-6, amp=1.0, interleaved=False):
+        """Heads of queries and keys of a QKV projection's rows: their norm (where weights are given) and the rotation of their first rot_dim elements."""
+        ffi.check(self.cc.lib.w4a16_qk_norm_rope(self.cc.h, x_dev, x_type, ldx, t, n_q, n_k, head_dim, qw_dev, kw_dev, eps, pos_dev, freqs_dev, rot_dim, amp,
+                                                 int(bool(interleaved)), q_dev, ldq, k_dev, ldk, y_type))
+
     # ---- layer chain
     CHAIN_ROLES = ("attn_qkv", "attn_output", "ffn_gate_up", "ffn_down")
 
@@ -579,6 +593,13 @@ class W4a16Dec:
         ffi.check(self.cc.lib.w4a16_bench_chain(self.cc.h, prefix.encode(), n_layers, x_dev, t, y_dev, warmup, reps,
                                                 int(use_graph), int(fused), C.byref(ms), C.byref(wall)))
         return ms.value, wall.value
+
+
+def rope_freqs(rot_dim, base, scaling=ffi.ROPE_PLAIN, factor=1.0, trained=0.0, low=0.0, high=0.0):
+    """(frequencies f64 [rot_dim / 2] in radians per position, amp) of a rotation (no context, no GPU)."""
+    freqs, amp = np.empty(max(rot_dim // 2, 1)), C.c_float()
+    ffi.check(ffi.load().w4a16_rope_freqs(rot_dim, base, scaling, factor, trained, low, high, _ptr(freqs), C.byref(amp)))
+    return freqs, amp.value
 
 
 def q8_bytes(t, k):
