@@ -155,7 +155,6 @@ constexpr int kW4ScoreMaxTop = 32;          // SCORE_MAX_TOP
 constexpr int kW4ScoreRecord = 272;         // SCORE_RECORD
 
 constexpr int kW4RopeMaxDim = 1024;         // ROPE_MAX_DIM (rope.hip)
-constexpr int kW4VerifyMaxSegment = 16384;  // VERIFY_MAX_SEGMENT (verify.hip)
 
 int w4_fail(int code, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
 int w4_hip(hipError_t e, const char* api);

@@ -3,17 +3,17 @@
 // accepted while u_i q(x) < p(x); behind the last accepted one a token is drawn from max(0, p - q) at the first row that is not, from p at the last row: the first whose
 // running sum exceeds u_last times the whole sum.  Temperature 0: accepted is the most likely token, which also follows.
 //
-// Running sums over a vocabulary meet a border between two tokens about once in V / (relative error) draws, so powers and sums are of 64 bits: 2^x by a polynomial of
-// degree 8 (interpolation at Chebyshev nodes of [-1/2, 1/2], off by 1.1e-12), 17 instructions an element, which the stream of the logits about hides.
-//
-// Two launches.  Rows: a segment of a target's or a draft's row to a workgroup, with a running maximum in each thread; it leaves (sum, maximum) of its segment, and the last of
-// a row joins them and judges the row's token.  Pick: a sequence finds its first row that is not accepted.  What is drawn from p alone knows its segments' sums already,
-// finds the segment and goes over that; only max(0, p - q) takes a pass over both rows, a segment to a workgroup, the last of which finds the segment.  Within a segment a thread
-// sums a run of neighbours, and the run that holds the draw is gone over again, an element to a lane.
+// Two launches.  Rows: a segment of a target's or a draft's row to a workgroup, with a running maximum in each thread; it leaves (sum, maximum) of its segment, and the last
+// of a row joins them and judges the row's token.  A decision wants its sum to some 10^-7, so powers are of 32 bits here and the stream of the logits is what takes the time.
+// Pick: of the first row that is not accepted alone, a segment to a workgroup.  Running sums over a vocabulary meet a border between two tokens about once in V / (relative error)
+// draws, so powers and sums are of 64 bits: 2^x by a polynomial of degree 8 (interpolation at Chebyshev nodes of [-1/2, 1/2], off by 1.1e-12), some 17 instructions of four
+// cycles.  A segment leaves sum p, sum q and, over the tokens where p is above q by the first launch's sums, sum p and sum q again: what is known of the whole sums then makes sum max(0, p - q) of
+// them.  Tokens that the first launch's 10^-7 puts on the wrong side have no more than that share of themselves to give; where that is over 10^-9 of the whole, target and draft being
+// nearly alike, the sums are made again with what is known now.  The last workgroup of a sequence finds the segment that holds the draw, a thread of it sums a run of neighbours, and the run
+// that holds it is gone over again, an element to a lane.
 #include "score_common.hpp"
 
 #define VERIFY_WAVES 4
-#define VERIFY_MAX_SEGMENT 16384  // elements: 64 to each thread that goes over it again
 
 typedef unsigned long long bits_t;
 
@@ -22,11 +22,20 @@ struct VerifyRow {  // what is known of a row: sum 0 where it has no distributio
     float m, md;
     int best, accepted;
 };
-struct VerifySum {  // of a segment: sum of powers relative to its maximum; or the key of its largest element; or the sum of max(0, p - q)
+struct VerifySum {  // of a segment: sum of powers relative to its maximum; or the key of its largest element
     double s;
     float m;
     int pad;
 };
+struct VerifyPart {  // of a segment of a row that is drawn from: sums of the powers of target and draft, all and where p > q; of the target's where p is nearly q
+    double v[5];
+};
+#define VERIFY_E 0
+#define VERIFY_D 1
+#define VERIFY_E_OVER 2
+#define VERIFY_D_OVER 3
+#define VERIFY_E_NEAR 4
+#define VERIFY_NEAR 1e-6
 
 // 2^x, x <= 0; a NaN counts as far below
 __device__ __forceinline__ double verify_exp2(double x) {
@@ -122,6 +131,7 @@ __device__ __forceinline__ void verify_rows_body(const void* __restrict__ logits
     const bool greedy = !(temp > 0.f), both = draft && !last && !greedy;
     if (of_draft && !both) return;
     const double c = greedy ? 0.0 : verify_factor(temp);
+    const float c_hi = (float)__builtin_fmin(c, 1e37), c_lo = (float)(__builtin_fmin(c, 1e37) - (double)c_hi);  // as 32-bit numbers: its own rounding would be on every power
 
     VerifySum mine = {0.0, -__builtin_inff(), 0};
     unsigned best = 0;
@@ -148,7 +158,15 @@ __device__ __forceinline__ void verify_rows_body(const void* __restrict__ logits
             }
             const float mm = mine.m == -__builtin_inff() ? 0.f : mine.m;  // nothing so far: every element is -infinity
 #pragma unroll
-            for (int e = 0; e < E; e++) mine.s += verify_power(cur.value(e), mm, c);
+            for (int e = 0; e < E; e += 4) {
+                float p[4];
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const float v = cur.value(e + k), d = __builtin_fmaxf(v - mm, -3.402823466e38f), x = __builtin_fmaf(d, c_hi, d * c_lo);
+                    p[k] = __builtin_amdgcn_exp2f(v == -__builtin_inff() ? v : x);
+                }
+                mine.s += (double)((p[0] + p[1]) + (p[2] + p[3]));
+            }
         }
         if (i + STEP >= hi) break;
     }
@@ -253,9 +271,9 @@ __device__ __forceinline__ int verify_find(double v, double aim, double& before,
 template <int T>
 __device__ __forceinline__ void verify_pick_body(const void* __restrict__ logits, size_t ld, const void* __restrict__ draft, size_t ldd, int vocab, int t, int seq_first,
                                                  const int* __restrict__ row0, const int* drafted, const float* __restrict__ u, const float* __restrict__ temps,
-                                                 int segs, int seg_len, const VerifySum* __restrict__ sums, const VerifyRow* __restrict__ rows,
-                                                 VerifySum* __restrict__ parts, int* __restrict__ tickets, int* tokens, int* __restrict__ accepted) {
-    __shared__ double red[VERIFY_WAVES], starts[256];
+                                                 int segs, int seg_len, const VerifyRow* __restrict__ rows, VerifyPart* __restrict__ parts, int* __restrict__ tickets,
+                                                 int* tokens, int* __restrict__ accepted) {
+    __shared__ double red[VERIFY_WAVES], sums[5][VERIFY_WAVES], starts[256];
     __shared__ int found[2];
     __shared__ int last_one, chosen;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), tid = threadIdx.x;
@@ -275,49 +293,66 @@ __device__ __forceinline__ void verify_pick_body(const void* __restrict__ logits
     }
     const VerifyRow r = rows[stop];
     const float temp = temps ? temps[b] : 1.f;
-    const bool greedy = !(temp > 0.f), last = stop == r1 - 1, residual = !greedy && r.s > 0.0 && draft && !last && r.sd > 0.0;
-    if (seg != 0 && !residual) return;
-    const double c = greedy ? 0.0 : verify_factor(temp);
+    const bool greedy = !(temp > 0.f), last = stop == r1 - 1, both = draft && !last && r.sd > 0.0;
     int token = greedy && r.s > 0.0 ? r.best : -1;
-    if (!greedy && r.s > 0.0) {
-        constexpr int SIZE = T == Q8_F32 ? 4 : 2;
+    if (greedy || !(r.s > 0.0)) {
+        if (seg != 0) return;
+    } else {
+        constexpr int SIZE = ScoreChunk<T>::SIZE, E = ScoreChunk<T>::E;
+        constexpr unsigned STAGE = ScoreChunk<T>::STAGE, STEP = VERIFY_WAVES * STAGE;
         const char* const z = static_cast<const char*>(logits) + (size_t)stop * ld * SIZE;
         const char* const zd = static_cast<const char*>(draft) + (size_t)stop * ldd * SIZE;
-        const unsigned streams = draft ? 2 : 1;
-        const VerifySum* const of_row = sums + (size_t)stop * segs * streams;
-        const double inv = 1.0 / r.s, inv_d = residual ? 1.0 / r.sd : 0.0;
-        // what is left out: the token that was certain to its draft
-        const int x = last || draft ? -1 : drafted[stop];
-        const int run = (seg_len + 4095) / 4096 * 16;  // neighbours to a thread
-        int out = x;
-        bool only_p = !residual;
-        auto weight = [&](float v, float d, int at) {
-            const double p = verify_power(v, r.m, c) * inv;
-            if (only_p) return at == out ? 0.0 : p;
-            return __builtin_fmax(p - verify_power(d, r.md, c) * inv_d, 0.0);
-        };
-        // the sum of this thread's run of segment s
-        auto of_run = [&](int s) {
-            const int from = s * seg_len + tid * run, to = min(min(from + run, (s + 1) * seg_len), vocab);
-            double sum = 0.0;
-            for (int at = from; at < to; at += 16) {
-                float v[16], d[16];
-                q8_load16<T>(z, (size_t)at, to - at, v);
-                if (!only_p) q8_load16<T>(zd, (size_t)at, to - at, d);
+        const double c = verify_factor(temp);
+        const float draw = u[r1 - 1];
+        const int x = last || draft ? -1 : drafted[stop];  // left out: the token that was certain to its draft
+        const unsigned lo = (unsigned)seg * (unsigned)seg_len, hi = min(lo + (unsigned)seg_len, (unsigned)vocab);
+        double sum[5] = {0.0, 0.0, 0.0, 0.0, 0.0};
+        const double rough = both ? r.s / r.sd : 0.0;  // p > q: e > d S / S_draft
+        for (unsigned i = lo + wave * STAGE; i < hi; i += STEP) {
+            ScoreChunk<T> v, d;
+            v.load(z + (size_t)i * SIZE, hi - i, lane);
+            if (both) {
+                d.load(zd + (size_t)i * SIZE, hi - i, lane);
 #pragma unroll
-                for (int e = 0; e < 16; e++) {
-                    const double w = weight(v[e], only_p ? 0.f : d[e], at + e);
-                    sum += at + e < to ? w : 0.0;
+                for (int e = 0; e < E; e++) {
+                    const double p = verify_power(v.value(e), r.m, c), q = verify_power(d.value(e), r.md, c), more = p - q * rough;
+                    const bool over = more > 0.0, near = __builtin_fabs(more) <= VERIFY_NEAR * p;
+                    sum[VERIFY_E] += p;
+                    sum[VERIFY_D] += q;
+                    sum[VERIFY_E_OVER] += over ? p : 0.0;
+                    sum[VERIFY_D_OVER] += over ? q : 0.0;
+                    sum[VERIFY_E_NEAR] += near ? p : 0.0;
+                }
+            } else {
+                const int out = x - (int)i - ScoreChunk<T>::at(lane, 0);
+#pragma unroll
+                for (int e = 0; e < E; e++) {
+                    const double p = verify_power(v.value(e), r.m, c);
+                    sum[VERIFY_E] += out == ScoreChunk<T>::at(0, e) ? 0.0 : p;
                 }
             }
-            return sum;
-        };
-        if (residual) {
-            const double mine = verify_wave_sum(of_run(seg));
-            if (lane == 0) red[wave] = mine;
+        }
+        // five sums over the workgroup at once, or the first alone; all threads get them
+        auto of_all = [&](double (&v)[5]) {
             __syncthreads();
+#pragma unroll
+            for (int k = 0; k < 5; k++) {
+                if (k > 0 && !both) break;
+                const double w = verify_wave_sum(v[k]);
+                if (lane == 0) sums[k][wave] = w;
+            }
+            __syncthreads();
+#pragma unroll
+            for (int k = 0; k < 5; k++) v[k] = k == 0 || both ? (sums[k][0] + sums[k][1]) + (sums[k][2] + sums[k][3]) : 0.0;
+        };
+        of_all(sum);
+        VerifyPart* const of_seq = parts + (size_t)b * segs;
+        if (segs > 1) {
             if (tid == 0) {
-                verify_put(parts + (size_t)b * segs + seg, {red[0] + red[1] + red[2] + red[3], 0.f, 0});
+#pragma unroll
+                for (int k = 0; k < 5; k++)
+                    if (k == 0 || both) __hip_atomic_store(reinterpret_cast<bits_t*>(of_seq[seg].v + k), __builtin_bit_cast(bits_t, sum[k]), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                // complete before the ticket is drawn; read behind the barrier that follows its return
                 asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
                 last_one = __hip_atomic_fetch_add(tickets + b, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == segs - 1;
             }
@@ -325,35 +360,95 @@ __device__ __forceinline__ void verify_pick_body(const void* __restrict__ logits
             if (!last_one) return;
             if (tid == 0) __hip_atomic_store(tickets + b, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);  // for the next launch
         }
-        // a segment's sum
-        auto of_segment = [&](int s) {
-            if (s >= segs) return 0.0;
-            if (!only_p) return verify_get(parts + (size_t)b * segs + s).s;
-            double p = verify_share(of_row[s], r.m, c) * inv;
-            if (out >= 0 && out < vocab && out / seg_len == s) p = __builtin_fmax(p - verify_power(q8_load1<T>(z, (size_t)out), r.m, c) * inv, 0.0);
-            return p;
+        // Segments tid, tid + 256, ..: the first is kept in registers
+        auto fetch = [&](int s, double (&v)[5]) {
+#pragma unroll
+            for (int k = 0; k < 5; k++) {
+                v[k] = 0.0;
+                if (s < segs && (k == 0 || both))
+                    v[k] = segs == 1 ? sum[k] : __builtin_bit_cast(double, __hip_atomic_load(reinterpret_cast<const bits_t*>(of_seq[s].v + k), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+            }
         };
+        double first[5], all[5];
+        fetch(tid, first);
+#pragma unroll
+        for (int k = 0; k < 5; k++) all[k] = first[k];
+        for (int s = tid + 256; s < segs; s += 256) {
+            double v[5];
+            fetch(s, v);
+#pragma unroll
+            for (int k = 0; k < 5; k++) all[k] += v[k];
+        }
+        of_all(all);
+        const double inv = 1.0 / all[VERIFY_E], inv_d = both ? 1.0 / all[VERIFY_D] : 0.0;
+        bool only_p = !both, again = false;
+        auto weight = [&](float v, float d, int at) {
+            const double p = verify_power(v, r.m, c) * inv;
+            if (only_p) return at == x ? 0.0 : p;
+            return __builtin_fmax(p - verify_power(d, r.md, c) * inv_d, 0.0);
+        };
+        const int run = (seg_len + 255) / 256;  // neighbours to a thread: 16, or 32 of 16-bit logits
+        // the sum of this thread's run of segment s
+        auto of_run = [&](int s) {
+            const int from = s * seg_len + tid * run, to = min(min(from + run, (s + 1) * seg_len), vocab);
+            double w_sum = 0.0;
+            for (int at = from; at < to; at += 16) {
+                float v[16], d[16];
+                q8_load16<T>(z, (size_t)at, to - at, v);
+                if (!only_p) q8_load16<T>(zd, (size_t)at, to - at, d);
+#pragma unroll
+                for (int e = 0; e < 16; e++) {
+                    const double w = weight(v[e], only_p ? 0.f : d[e], at + e);
+                    w_sum += at + e < to ? w : 0.0;
+                }
+            }
+            return w_sum;
+        };
+        auto share = [&](const double (&v)[5]) { return only_p ? v[VERIFY_E] * inv : again ? v[VERIFY_E_OVER] : __builtin_fmax(v[VERIFY_E_OVER] * inv - v[VERIFY_D_OVER] * inv_d, 0.0); };
+        // what the segments have to give
         auto total = [&]() {
-            double sum = 0.0;
-            for (int s = tid; s < segs; s += 256) sum += of_segment(s);
-            sum = verify_wave_sum(sum);
-            __syncthreads();
-            if (lane == 0) red[wave] = sum;
-            __syncthreads();
-            return red[0] + red[1] + red[2] + red[3];
+            double v[5] = {share(first), 0.0, 0.0, 0.0, 0.0};
+            for (int s = tid + 256; s < segs; s += 256) {
+                double w[5];
+                fetch(s, w);
+                v[0] += share(w);
+            }
+            of_all(v);
+            return v[0];
         };
-        // Drawn from p where p is nowhere above q, or where what a rounding left over a segment's certain token is drawn
+        double whole = only_p ? (all[VERIFY_E] > 0.0 ? 1.0 : 0.0) : total();
+        if (both) {
+            const double off = __builtin_fabs(rough * all[VERIFY_D] * inv - 1.0);
+            again = !(off < VERIFY_NEAR) || off * all[VERIFY_E_NEAR] * inv > 1e-9 * whole;
+            if (again) {
+                for (int s = 0; s < segs; s++) {
+                    double v[5] = {of_run(s), 0.0, 0.0, 0.0, 0.0};
+                    of_all(v);
+                    if (s == tid) first[VERIFY_E_OVER] = v[0];
+                    if (segs > 256 && tid == 0)
+                        __hip_atomic_store(reinterpret_cast<bits_t*>(of_seq[s].v + VERIFY_E_OVER), __builtin_bit_cast(bits_t, v[0]), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                }
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                __syncthreads();
+                whole = total();
+            }
+        }
+        // Drawn from p where p is nowhere above q, or where no token of the segment that the draw falls into is left at the second look
         for (int attempt = 0; attempt < 2 && token < 0; attempt++) {
-            if (attempt == 1) only_p = true, out = -1;
-            const double all = total();
-            if (!(all > 0.0)) continue;
-            const double aim = (double)u[r1 - 1] * all;
+            if (attempt == 1) {
+                if (only_p) break;
+                only_p = true;
+                whole = 1.0;
+            }
+            if (!(whole > 0.0)) continue;
+            const double aim = (double)draw * whole;
             double before = 0.0, from = 0.0;
             int at = -1;
             bool none = true;
             for (int s = 0; s < segs && none; s += 256) {
-                double ahead = from;
-                const int f = verify_find(of_segment(s + tid), aim, ahead, red, found, starts, none);
+                double ahead = from, v[5];
+                if (s > 0) fetch(s + tid, v);
+                const int f = verify_find(s > 0 ? share(v) : share(first), aim, ahead, red, found, starts, none);
                 if (f >= 0) {
                     at = s + f;
                     before = none ? starts[f] : ahead;
@@ -375,6 +470,7 @@ __device__ __forceinline__ void verify_pick_body(const void* __restrict__ logits
             __syncthreads();
             token = chosen;
         }
+        if (token < 0) token = x;  // all of p is on the token that was left out
     }
     for (int i = r0 + tid; i < r1; i += 256) tokens[i] = i < stop ? drafted[i] : i == stop ? token : -1;
     if (tid == 0) accepted[b] = stop - r0;
@@ -388,9 +484,8 @@ __device__ __forceinline__ void verify_pick_body(const void* __restrict__ logits
     }                                                                                                                              \
     extern "C" __global__ __launch_bounds__(256) void w4a16_verify_pick_##NAME(                                                    \
         const void* logits, size_t ld, const void* draft, size_t ldd, int vocab, int t, int seq_first, const int* row0, const int* drafted, const float* u, \
-        const float* temps, int segs, int seg_len, const VerifySum* sums, const VerifyRow* rows, VerifySum* parts, int* tickets, int* tokens, \
-        int* accepted) {                                                                                                           \
-        verify_pick_body<T>(logits, ld, draft, ldd, vocab, t, seq_first, row0, drafted, u, temps, segs, seg_len, sums, rows, parts, tickets, tokens, accepted); \
+        const float* temps, int segs, int seg_len, const VerifyRow* rows, VerifyPart* parts, int* tickets, int* tokens, int* accepted) {  \
+        verify_pick_body<T>(logits, ld, draft, ldd, vocab, t, seq_first, row0, drafted, u, temps, segs, seg_len, rows, parts, tickets, tokens, accepted); \
     }
 VERIFY_KERNELS(f32, Q8_F32)
 VERIFY_KERNELS(f16, Q8_F16)
