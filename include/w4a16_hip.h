@@ -555,7 +555,7 @@ int w4a16_plan_w8a8(size_t n, size_t k, size_t t, int cu_count, int glu, char* k
  * A block of a row x is quantised with the least power of two s >= 2^-126 that brings its largest magnitude to 448 or below; q = x / s to the nearest e4m3
  * number (halves to the even one), exactly: powers of two make the quotients exact and cost no relative precision.  A block of zeros has s = 0, one that holds infinity or
  * NaN s = NaN (and so has every output of its row) and q = 0.
- * Sums are held in f32, a block's products summed first; the result is rounded once more to y's type.  f32 results, and any of up to 64 rows, are sums of 32 bits.
+ * Sums are held in f32, a block's products summed first; the result is rounded once more to y's type.  f32 results, and any of up to 1024 rows, are sums of 32 bits.
  * For f16 and bf16 results of more rows the products of a block may be summed by the e4m3 matrix instruction, which drops of a product what lies more than 2^-13 below the
  * largest of its group: 1.6e-5 of the results' size on normal numbers, 1 / 17 of an f16 result's own rounding.  The same call gives the same bits every time.
  * Streams, captures, scratch and the number of rows: as for the W8A8 linears above.
@@ -582,8 +582,9 @@ int w4a16_lin_forward_f8(w4a16_ctx* ctx, const char* name, uint64_t x_dev, int x
  * to y's type.  act: W4A16_ACT_SILU or W4A16_ACT_GELU_TANH. */
 int w4a16_lin_forward_f8_glu(w4a16_ctx* ctx, const char* name, uint64_t x_dev, int x_type, size_t ldx, uint64_t xs_dev, size_t t, uint64_t y_dev,
                              int y_type, int act);
-/* The launch that t rows through an FP8 linear with results of y_type go to, as w4a16_plan_w8a8. */
-int w4a16_plan_f8(size_t n, size_t k, size_t t, int cu_count, int glu, int y_type, char* kernel, size_t cap, size_t* workgroups, int* waves, int* k_slices);
+/* The launch that t rows of x_type through an FP8 linear with results of y_type go to, as w4a16_plan_w8a8. */
+int w4a16_plan_f8(size_t n, size_t k, size_t t, int cu_count, int glu, int x_type, int y_type, char* kernel, size_t cap, size_t* workgroups, int* waves,
+                  int* k_slices);
 
 /* Scores rows of logits z [t][n_vocab] (f32, f16 or bf16, rows ld elements apart, 0 = n_vocab); results of no interest are 0.
  *   targets int32 [t], logp f32 [t]: log softmax(z)[target]; 0 for a negative target (none is asked for), NaN for one >= n_vocab;

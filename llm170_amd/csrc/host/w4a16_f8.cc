@@ -201,18 +201,22 @@ struct F8Launch {
     char kernel[64] = "";
     size_t grid_x = 0, grid_y = 1, tickets = 0, part_bytes = 0;
     int block = 256, nks = 1, band = 0;  // band: tile rows of a band, 0 = the kernel for groups of up to 64 rows
+    bool floats = false;                 // the kernel takes rows of floats
 };
 
-static int plan_f8(const char* what, size_t n, size_t k, size_t t, size_t cus, bool glu, int y_type, F8Launch* out) {
+static int plan_f8(const char* what, size_t n, size_t k, size_t t, size_t cus, bool glu, int x_type, int y_type, F8Launch* out) {
     F8Launch& P = *out;
-    const bool exact = y_type == W4A16_F32;
+    const bool exact = y_type == W4A16_F32 || t <= 1024;
     const F8Skinny few = plan_skinny(n, k, t, cus, glu);
     const F8Tiled tiles = t <= 64 ? F8Tiled() : plan_tiled(n, k, t, cus, exact);
     if (t <= 64 || (t <= 1024 && few.price < tiles.price)) {
         const size_t groups = (t + 63) / 64;  // of as many rows each as can be
         const int tt = (int)((t + 16 * groups - 1) / (16 * groups));
         const size_t blocks16 = (n + 15) / 16;
-        snprintf(P.kernel, sizeof P.kernel, "w4a16_f8_skinny_r%d_t%d%s", few.rb, tt, glu ? "_glu" : "");
+        P.floats = t <= 16 && x_type != W4A16_F8;  // quantised by the kernel itself
+        char rows[8];
+        snprintf(rows, sizeof rows, "t%d", tt);
+        snprintf(P.kernel, sizeof P.kernel, "w4a16_f8_skinny_r%d_%s%s", few.rb, P.floats ? w4_type_name(x_type) : rows, glu ? "_glu" : "");
         P.nks = few.nks;
         P.grid_x = glu ? (blocks16 / 2 + few.rb / 2 - 1) / (few.rb / 2) : (blocks16 + few.rb - 1) / few.rb;
         P.grid_y = few.nks * groups;
@@ -231,16 +235,17 @@ static int plan_f8(const char* what, size_t n, size_t k, size_t t, size_t cus, b
     return 0;
 }
 
-extern "C" int w4a16_plan_f8(size_t n, size_t k, size_t t, int cu_count, int glu, int y_type, char* kernel, size_t cap, size_t* workgroups, int* waves,
-                             int* k_slices) {
+extern "C" int w4a16_plan_f8(size_t n, size_t k, size_t t, int cu_count, int glu, int x_type, int y_type, char* kernel, size_t cap, size_t* workgroups,
+                             int* waves, int* k_slices) {
     if (cu_count <= 0 || (kernel && cap < sizeof(F8Launch::kernel)))
         return w4_fail(W4A16_ERR_ARG, "plan_f8: cus=%d, %zu bytes for a name of up to %zu", cu_count, cap, sizeof(F8Launch::kernel));
+    if (x_type != W4A16_F8 && !w4_float_type(x_type)) return w4_fail(W4A16_ERR_ARG, "plan_f8: x type %d (0 = f32, 1 = f16, 2 = bf16, 4 = rows quantised to e4m3)", x_type);
     if (!w4_float_type(y_type)) return w4_fail(W4A16_ERR_ARG, "plan_f8: y type %d (0 = f32, 1 = f16, 2 = bf16)", y_type);
     W4_TRY(w4_q8_check_rows("plan_f8", t, k));
     if (n == 0 || n > 0x7fffff00u || (glu && n % 256 != 0))
         return w4_fail(W4A16_ERR_SHAPE, "plan_f8: n=%zu outside 1..2^31-256, or gated and no multiple of 256", n);
     F8Launch P;
-    W4_TRY(plan_f8("plan_f8", n, k, t, (size_t)cu_count, glu != 0, y_type, &P));
+    W4_TRY(plan_f8("plan_f8", n, k, t, (size_t)cu_count, glu != 0, x_type, y_type, &P));
     if (kernel) memcpy(kernel, P.kernel, sizeof P.kernel);
     if (workgroups) *workgroups = P.grid_x * P.grid_y;
     if (waves) *waves = P.block / 64;
@@ -248,13 +253,14 @@ extern "C" int w4a16_plan_f8(size_t n, size_t k, size_t t, int cu_count, int glu
     return 0;
 }
 
-static int launch_f8(w4a16_ctx* ctx, const F8Lin& L, const F8Launch& P, uint64_t q, uint64_t s, size_t t, uint64_t y, int y_type, int act) {
+static int launch_f8(w4a16_ctx* ctx, const F8Lin& L, const F8Launch& P, uint64_t q, uint64_t s, size_t ldx, size_t t, uint64_t y, int y_type, int act) {
     if (P.nks > 1) W4_TRY(w4_split_workspace(ctx, P.part_bytes, P.tickets));
     uint64_t wt = L.q, ws = L.s, part = ctx->w8_part, tickets = ctx->w8_tickets;
-    int ni = (int)L.n, kb = (int)w4_q8_blocks(L.k), ti = (int)t, r = (int)w4_q8_tile_rows(t), wi = P.block / 64, ksi = P.nks, band = P.band;
+    int ni = (int)L.n, ki = (int)L.k, kb = (int)w4_q8_blocks(L.k), ti = (int)t, r = (int)w4_q8_tile_rows(t), wi = P.block / 64, ksi = P.nks, band = P.band;
     void* few[] = {&wt, &ws, &q, &s, &y, &ni, &kb, &ti, &r, &y_type, &act, &wi, &ksi, &part, &tickets};
+    void* floats[] = {&wt, &ws, &q, &ldx, &ki, &y, &ni, &kb, &ti, &y_type, &act, &wi, &ksi, &part, &tickets};
     void* tiles[] = {&wt, &ws, &q, &s, &y, &ni, &kb, &ti, &y_type, &act, &ksi, &band, &part, &tickets};
-    return w4_launch(ctx, P.kernel, (unsigned)P.grid_x, (unsigned)P.grid_y, (unsigned)P.block, 0, P.band ? tiles : few);
+    return w4_launch(ctx, P.kernel, (unsigned)P.grid_x, (unsigned)P.grid_y, (unsigned)P.block, 0, P.band ? tiles : P.floats ? floats : few);
 }
 
 static int forward_f8(w4a16_ctx* ctx, const char* api, const char* name, uint64_t x, int x_type, size_t ldx, uint64_t xs, size_t t, uint64_t y,
@@ -277,16 +283,16 @@ static int forward_f8(w4a16_ctx* ctx, const char* api, const char* name, uint64_
     if (y % w4_type_bytes(y_type) || x % (x_type == W4A16_F8 ? 16 : w4_type_bytes(x_type)) || xs % 4)
         return w4_fail(W4A16_ERR_ARG, "%s %s: operands must be aligned to their elements, quantised rows to 16 bytes", api, name);
     F8Launch P;
-    W4_TRY(plan_f8(api, L->n, L->k, t, (size_t)std::max(ctx->cu_count, 1), act >= 0, y_type, &P));
+    W4_TRY(plan_f8(api, L->n, L->k, t, (size_t)std::max(ctx->cu_count, 1), act >= 0, x_type, y_type, &P));
     W4_TRY(w4_hip(hipSetDevice(ctx->device), "hipSetDevice"));
-    if (x_type != W4A16_F8) {
+    if (x_type != W4A16_F8 && !P.floats) {
         W4_TRY(w4_ensure(ctx, &ctx->q8, &ctx->q8_cap, w4a16_q8_bytes(t, L->k)));
         W4_TRY(w4_ensure(ctx, &ctx->q8_scales, &ctx->q8_scales_cap, std::max<size_t>(t * w4_q8_blocks(L->k) * 4, 256)));
         W4_TRY(quant_rows(ctx, x, x_type, ldx, t, L->k, ctx->q8, ctx->q8_scales));
         x = ctx->q8;
         xs = ctx->q8_scales;
     }
-    return launch_f8(ctx, *L, P, x, xs, t, y, y_type, act);
+    return launch_f8(ctx, *L, P, x, xs, ldx, t, y, y_type, act);
 }
 
 extern "C" int w4a16_lin_forward_f8(w4a16_ctx* ctx, const char* name, uint64_t x_dev, int x_type, size_t ldx, uint64_t xs_dev, size_t t, uint64_t y_dev,

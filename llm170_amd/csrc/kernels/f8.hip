@@ -6,7 +6,7 @@
 // numbers 1.6e-5 of the results' size, 4.2 PFLOP/s alone (16x16x128; 32x32x64 3.8), 3.5 with the scaling.  As f16, which holds every e4m3 number, the same
 // sums are those of 32 bits (1e-8), at the f16 instruction's 1.6.  So: up to 64 rows, where the weight stream is what takes the time, and for f32 results, f16; for 16-bit
 // results of more rows, whose own rounding is 30 times as large and whose rows' quantisation 1000 times, e4m3.
-#include "q8_common.hpp"
+#include "f8_common.hpp"
 
 typedef int i8_t __attribute__((ext_vector_type(8)));
 
@@ -23,11 +23,53 @@ __device__ __forceinline__ float f8_lane(float v, int lane) { return q8_f32((uns
 // As the int8 kernel for few rows (w8a8.hip): a workgroup's waves take consecutive runs of a k slice of the same RB row blocks (16 outputs each), weights as whole
 // tiles straight in registers, DEPTH blocks of them in flight, TT tiles of 16 activation rows from the L2.  The waves' sums are added in the order of
 // the waves in LDS and the k slices' in their order by the last workgroup: the same bits every time.  The weights' scales of a run lie one to a lane.
-template <int RB, int TT, bool GLU>
+//
+// Up to 16 rows of floats (XT: their type) are quantised on the way: a wave takes of its run of k what it needs, once, behind its first weights; that is 16 conversions of eight
+// cycles a lane and block, and saves the launch that would do it.
+template <int XT>
+struct F8Rows {  // a lane's share of a block of 16 activation rows, row lane % 16: chunks kg and kg + 4 of eight
+    F8Run<XT> run[2];
+    const char* row;
+    int k, kg;
+    __device__ __forceinline__ void at(const void* x, size_t ldx, int k_, int t) {
+        row = static_cast<const char*>(x) + (size_t)min((int)(threadIdx.x & 15), t - 1) * ldx * (XT == Q8_F32 ? 4 : 2);
+        k = k_;
+        kg = (threadIdx.x & 63) >> 4;
+    }
+    __device__ __forceinline__ void load(int block) {
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const int from = block * 128 + h * 64 + kg * 16;
+            run[h].load(row, from, block * 128 + 128 <= k ? 16 : k - from);  // whole blocks without a branch
+        }
+    }
+    // its e4m3 numbers as f16, and their scale
+    __device__ __forceinline__ void get(h8_t (&x)[4], float& s) const {
+        unsigned m = run[1].most(run[0].most(0));
+        const auto a = __builtin_amdgcn_permlane32_swap(m, m, false, false);
+        m = max(a[0], a[1]);
+        const auto b = __builtin_amdgcn_permlane16_swap(m, m, false, false);
+        m = max(b[0], b[1]);
+        float by;
+        s = f8_step(m, by);
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const u4_t q = run[h].pack(by, !(s > 0.f));
+            x[2 * h] = f8_to_f16(q[0], q[1]);
+            x[2 * h + 1] = f8_to_f16(q[2], q[3]);
+        }
+    }
+};
+template <>
+struct F8Rows<F8_ROWS> {};
+
+template <int RB, int TT, bool GLU, int XT>
 __device__ __forceinline__ void f8_skinny_body(const char* __restrict__ wt, const float* __restrict__ ws, const char* __restrict__ xq,
-                                               const float* __restrict__ xs, void* __restrict__ y, int n, int kb, int t, int R, int y_type, int act,
-                                               int W, int nks, w8_pair_t* __restrict__ part, int* __restrict__ tickets) {
-    constexpr int TILES = RB * TT, DEPTH = TILES == 1 ? 4 : TILES <= 8 ? 2 : 1, SLOTS = TILES <= 4 ? 8 : 4;
+                                               const float* __restrict__ xs, size_t ldx, int k_in, void* __restrict__ y, int n, int kb, int t, int R, int y_type,
+                                               int act, int W, int nks, w8_pair_t* __restrict__ part, int* __restrict__ tickets) {
+    constexpr bool FLOATS = XT != F8_ROWS;
+    static_assert(!FLOATS || TT == 1, "floats: up to 16 rows");
+    constexpr int TILES = RB * TT, DEPTH = TILES == 1 ? (XT == Q8_F32 ? 3 : 4) : TILES <= 8 ? 2 : 1, SLOTS = TILES <= 4 ? 8 : 4, XD = FLOATS ? 1 : DEPTH;
     __shared__ float sums[SLOTS][TILES][4][64];
     __shared__ int last_one;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -40,6 +82,11 @@ __device__ __forceinline__ void f8_skinny_body(const char* __restrict__ wt, cons
     const int runs = nks * W, run = ks * W + wave;
     const int m0 = group * TT * 16, x_last = (t - 1) >> 4;  // rows of the group, and the last tile of 16 that there is
     const int lo = (int)((long long)kb * run / runs), hi = (int)((long long)kb * (run + 1) / runs);
+    F8Rows<XT> rows;
+    if constexpr (FLOATS) {
+        rows.at(xq, ldx, k_in, t);
+        if (lo < hi) rows.load(lo);
+    }
     const char* wp[RB];
     const float* wsp[RB];
     float wsv[RB];
@@ -53,25 +100,30 @@ __device__ __forceinline__ void f8_skinny_body(const char* __restrict__ wt, cons
         wsv[i] = wsp[i][min(lo + lane, kb - 1)];
     }
     // activations: tiles of R rows, [k tile][kg][R] chunks
-    const char* const xp = xq + ((size_t)kg * R + tok % R) * 16;
+    const char* const xp = FLOATS ? nullptr : xq + ((size_t)kg * R + tok % R) * 16;
     const size_t x_tile = (size_t)R * 64, x_block = x_tile * 2 * kb;
     f4_t acc[RB][TT];
 #pragma unroll
     for (int i = 0; i < RB; i++)
 #pragma unroll
         for (int j = 0; j < TT; j++) acc[i][j] = (f4_t){0.f, 0.f, 0.f, 0.f};
-    u4_t wv[DEPTH][RB][2], xv[DEPTH][TT][2];
-    float xsv[DEPTH][TT];
+    u4_t wv[DEPTH][RB][2], xv[XD][TT][2];
+    float xsv[XD][TT];
     auto load_w = [&](int d, int i, int k) {
+        // Non-temporal weights: 34816 x 5120 gated int8 at t = 1 31.3 us, else 35.2
 #pragma unroll
         for (int h = 0; h < 2; h++) wv[d][i][h] = __builtin_nontemporal_load(reinterpret_cast<const u4_t*>(wp[i] + (size_t)k * 2048 + h * 1024));
     };
     auto load_x = [&](int d, int k) {
+        if constexpr (FLOATS) {
+            rows.load(k);
+        } else {
 #pragma unroll
-        for (int j = 0; j < TT; j++) {
+            for (int j = 0; j < TT; j++) {
 #pragma unroll
-            for (int h = 0; h < 2; h++) xv[d][j][h] = *reinterpret_cast<const u4_t*>(xp + min((m0 >> 4) + j, x_last) * x_block + (2 * k + h) * x_tile);
-            xsv[d][j] = xs[(size_t)k * t + min(m0 + j * 16 + tok, t - 1)];
+                for (int h = 0; h < 2; h++) xv[d][j][h] = *reinterpret_cast<const u4_t*>(xp + min((m0 >> 4) + j, x_last) * x_block + (2 * k + h) * x_tile);
+                xsv[d][j] = xs[(size_t)k * t + min(m0 + j * 16 + tok, t - 1)];
+            }
         }
     };
 #pragma unroll
@@ -79,7 +131,7 @@ __device__ __forceinline__ void f8_skinny_body(const char* __restrict__ wt, cons
         if (lo + d >= hi) continue;
 #pragma unroll
         for (int i = 0; i < RB; i++) load_w(d, i, lo + d);
-        load_x(d, lo + d);
+        if (!FLOATS) load_x(d, lo + d);
     }
     int base = lo;  // of the 64 blocks whose scales are in the lanes
     for (int k = lo; k < hi; k += DEPTH) {
@@ -94,13 +146,18 @@ __device__ __forceinline__ void f8_skinny_body(const char* __restrict__ wt, cons
                 const int next = k + d + DEPTH;
                 h8_t x[TT][4];
                 float sx[TT];
+                if constexpr (FLOATS) {
+                    rows.get(x[0], sx[0]);
+                    if (k + d + 1 < hi) load_x(0, k + d + 1);
+                } else {
 #pragma unroll
-                for (int j = 0; j < TT; j++) {
-                    sx[j] = xsv[d][j];
+                    for (int j = 0; j < TT; j++) {
+                        sx[j] = xsv[d][j];
 #pragma unroll
-                    for (int c = 0; c < 4; c++) x[j][c] = f8_to_f16(xv[d][j][c / 2][c % 2 * 2], xv[d][j][c / 2][c % 2 * 2 + 1]);
+                        for (int c = 0; c < 4; c++) x[j][c] = f8_to_f16(xv[d][j][c / 2][c % 2 * 2], xv[d][j][c / 2][c % 2 * 2 + 1]);
+                    }
+                    if (next < hi) load_x(d, next);
                 }
-                if (next < hi) load_x(d, next);
 #pragma unroll
                 for (int i = 0; i < RB; i++) {
                     const float sw = f8_lane(wsv[i], k + d - base);
@@ -210,13 +267,22 @@ __device__ __forceinline__ void f8_skinny_body(const char* __restrict__ wt, cons
     extern "C" __global__ __launch_bounds__(512) void NAME(const char* wt, const float* ws, const char* xq, const float* xs, void* y, int n, \
                                                            int kb, int t, int R, int y_type, int act, int waves, int nks, w8_pair_t* part,    \
                                                            int* tickets) {                                                        \
-        f8_skinny_body<RB, TT, GLU>(wt, ws, xq, xs, y, n, kb, t, R, y_type, act, waves, nks, part, tickets);                      \
+        f8_skinny_body<RB, TT, GLU, F8_ROWS>(wt, ws, xq, xs, 0, 0, y, n, kb, t, R, y_type, act, waves, nks, part, tickets);       \
     }
-#define F8_SKINNY_T(NAME, RB, GLU, SUFFIX)        \
-    F8_SKINNY(NAME##_t1##SUFFIX, RB, 1, GLU)      \
-    F8_SKINNY(NAME##_t2##SUFFIX, RB, 2, GLU)      \
-    F8_SKINNY(NAME##_t3##SUFFIX, RB, 3, GLU)      \
-    F8_SKINNY(NAME##_t4##SUFFIX, RB, 4, GLU)
+#define F8_SKINNY_X(NAME, RB, GLU, XT)                                                                                            \
+    extern "C" __global__ __launch_bounds__(512) void NAME(const char* wt, const float* ws, const char* x, size_t ldx, int k, void* y, int n, \
+                                                           int kb, int t, int y_type, int act, int waves, int nks, w8_pair_t* part,          \
+                                                           int* tickets) {                                                        \
+        f8_skinny_body<RB, 1, GLU, XT>(wt, ws, x, nullptr, ldx, k, y, n, kb, t, 16, y_type, act, waves, nks, part, tickets);      \
+    }
+#define F8_SKINNY_T(NAME, RB, GLU, SUFFIX)                           \
+    F8_SKINNY(NAME##_t1##SUFFIX, RB, 1, GLU)                         \
+    F8_SKINNY(NAME##_t2##SUFFIX, RB, 2, GLU)                         \
+    F8_SKINNY(NAME##_t3##SUFFIX, RB, 3, GLU)                         \
+    F8_SKINNY(NAME##_t4##SUFFIX, RB, 4, GLU)                         \
+    F8_SKINNY_X(NAME##_f32##SUFFIX, RB, GLU, Q8_F32)                 \
+    F8_SKINNY_X(NAME##_f16##SUFFIX, RB, GLU, Q8_F16)                 \
+    F8_SKINNY_X(NAME##_bf16##SUFFIX, RB, GLU, Q8_BF16)
 F8_SKINNY_T(w4a16_f8_skinny_r1, 1, false, )
 F8_SKINNY_T(w4a16_f8_skinny_r2, 2, false, )
 F8_SKINNY_T(w4a16_f8_skinny_r4, 4, false, )
@@ -420,7 +486,7 @@ summed:
         }
     };
     // One type's code is run, and read for the first time: branches inside hold up the launch's end
-    if (EXACT) store(w8_type<Q8_F32>{});
+    if (y_type == Q8_F32) store(w8_type<Q8_F32>{});
     else if (y_type == Q8_F16) store(w8_type<Q8_F16>{});
     else store(w8_type<Q8_BF16>{});
 }

@@ -1,23 +1,7 @@
 // Quantisation of activation rows to e4m3 with a scale for each block of 128 k.  The scale is a power of two, the least that brings the block's largest
 // magnitude to 448 or below: every quotient is then exact and the conversion its only rounding (to nearest, halves to even), and since the numbers float, a
 // step up to twice as large loses nothing but the last of 18 binary orders below the largest.
-#include "q8_common.hpp"
-
-// The scale of a block from the bits of its largest magnitude, and its reciprocal.  448 is 1.75 * 2^8.  Zeros have the scale 0; infinity and NaN the scale NaN; both
-// have the reciprocal 0.
-__device__ __forceinline__ float f8_step(unsigned mag, float& r) {
-    const int e = max((int)(mag >> 23) - 8 + ((mag & 0x7fffffu) > 0x600000u ? 1 : 0), 1);  // biased; 1 is 2^-126
-    const bool some = mag != 0 && mag < 0x7f800000u;
-    r = some ? q8_f32((unsigned)(254 - e) << 23) : 0.f;
-    return some ? q8_f32((unsigned)e << 23) : mag == 0 ? 0.f : __builtin_nanf("");
-}
-
-// Four values as e4m3, byte e of the result is value e's; r = 0: zeros, whatever the values are
-__device__ __forceinline__ unsigned f8_pack(float a, float b, float c, float d, float r) {
-    int o = __builtin_amdgcn_cvt_pk_fp8_f32(a * r, b * r, 0, false);
-    o = __builtin_amdgcn_cvt_pk_fp8_f32(c * r, d * r, o, true);
-    return r == 0.f ? 0u : (unsigned)o;
-}
+#include "f8_common.hpp"
 
 // Largest of the eight lanes that share a block: neighbours, pairs, fours
 __device__ __forceinline__ unsigned f8_block_max(unsigned v) {
@@ -37,16 +21,11 @@ __device__ __forceinline__ void f8_quant_body(const void* __restrict__ x, size_t
     const int row = group * lr + (lane >> 3) % lr, b = ((int)blockIdx.y * stride + ahead) * per + (lane >> 3) / lr, c = b * 8 + (lane & 7);
     if (row >= t || b >= kb) return;  // whole runs of eight lanes
     const char* const xr = static_cast<const char*>(x) + (size_t)row * ldx * (T == Q8_F32 ? 4 : 2);
-    float v[16];
-    q8_load16<T>(xr, (size_t)c * 16, k - c * 16, v);
-    unsigned m = 0;
-#pragma unroll
-    for (int e = 0; e < 16; e++) m = max(m, q8_mag(v[e]));
-    float r;
-    const float step = f8_step(f8_block_max(m), r);
-    u4_t o;
-#pragma unroll
-    for (int i = 0; i < 4; i++) o[i] = f8_pack(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3], r);
+    F8Run<T> v;
+    v.load(xr, c * 16, k - c * 16);
+    float by;
+    const float step = f8_step(f8_block_max(v.most(0)), by);
+    const u4_t o = v.pack(by, !(step > 0.f));
     *reinterpret_cast<u4_t*>(q + q8_chunk_at(row, c, 2 * kb, R)) = o;
     if ((lane & 7) == 0) s[(size_t)b * s_ld + row] = step;
 }
@@ -102,9 +81,9 @@ extern "C" __global__ __launch_bounds__(1024) void w4a16_norm_resid_f8(float* __
     for (int j = 0; j < 8; j++) {
         if (j * 1024 >= hidden) continue;
         const int c = j * 1024 + tid;
-        float rs;
-        const float step = f8_step(max(redm[j][wave & ~1], redm[j][wave | 1]), rs);
-        line[c] = (char)f8_pack(c < hidden ? y[j] : 0.f, 0.f, 0.f, 0.f, rs);
+        float by;
+        const float step = f8_step(max(redm[j][wave & ~1], redm[j][wave | 1]), by);
+        line[c] = (char)f8_pack4(c < hidden ? y[j] : 0.f, 0.f, 0.f, 0.f, by, !(step > 0.f));
         if ((tid & 127) == 0 && c < hidden) s[(size_t)(c >> 7) * s_ld + row] = step;
     }
     __syncthreads();

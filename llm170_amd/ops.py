@@ -69,10 +69,10 @@ def plan_w8a8(t, n, k, cu_count=256, glu=False):
     return {"kernel": name.value.decode(), "workgroups": wgs.value, "waves": waves.value, "k_slices": nks.value}
 
 
-def plan_f8(t, n, k, cu_count=256, glu=False, y_type=ffi.F16):
-    """Launch of t rows through an FP8 linear with results of y_type (no context, no GPU): dict of kernel, workgroups, waves, k_slices."""
+def plan_f8(t, n, k, cu_count=256, glu=False, x_type=ffi.F8, y_type=ffi.F16):
+    """Launch of t rows of x_type through an FP8 linear with results of y_type (no context, no GPU): dict of kernel, workgroups, waves, k_slices."""
     name, wgs, waves, nks = C.create_string_buffer(64), C.c_size_t(), C.c_int(), C.c_int()
-    ffi.check(ffi.load().w4a16_plan_f8(n, k, t, cu_count, int(bool(glu)), y_type, name, 64, C.byref(wgs), C.byref(waves), C.byref(nks)))
+    ffi.check(ffi.load().w4a16_plan_f8(n, k, t, cu_count, int(bool(glu)), x_type, y_type, name, 64, C.byref(wgs), C.byref(waves), C.byref(nks)))
     return {"kernel": name.value.decode(), "workgroups": wgs.value, "waves": waves.value, "k_slices": nks.value}
 
 

@@ -139,25 +139,29 @@ def test_both_ways_to_quantised_rows_write_the_same_bytes(dec, t, hidden):
 @pytest.mark.parametrize("key", sorted(shapes()), ids=lambda k: k[0][10:] + ("_slices" if k[1] else ""))
 def test_every_build(dec, key):
     """Bit for bit on whole numbers whose sums are exact; within their room on normal numbers."""
-    t, n, k, glu, y_type = shapes()[key]
+    t, n, k, glu, x_type, y_type = shapes()[key]
     kernel, cc = key[0], dec.cc
-    say("build", key, t, n, k, glu, y_type)
+    say("build", key, t, n, k, glu, x_type, y_type)
     for whole in (True, False):
         if whole:
             q, s, w, sv = ref.small_whole(n + k, t, n, k)
             sb = sv
+            x = (ref.E4M3[q] * np.repeat(s.T, 128, 1)[:, :k]).astype(np.float32)  # floats that quantise to what they are
+            floats = x if x_type == ffi.F8 else w8.narrow(x, x_type)[0]
         else:
-            q, s = ref.quantised(np.random.default_rng(t).standard_normal((t, k)).astype(np.float32))
+            floats, x = w8.narrow(np.random.default_rng(t).standard_normal((t, k)).astype(np.float32), ffi.F32 if x_type == ffi.F8 else x_type)
+            q, s = ref.quantised(x)
             w, sb, sv = ref.weights(n * 5 + k, n, k)
         dec.upload_lin_f8("b", w, sb, n, k)
         assert dec.lin_f8_spec("b") == {"n": n, "k": k}
         want, a, most = ref.product(q, s, w, sv)
         size = 4 if y_type == ffi.F32 else 2
         with w8.Buffers(cc) as b:
-            dq, ds, y = b.put(ref.pack(q, t, k)), b.put(s), b.filled(t * n * size + 64)
+            dq, ds = (b.put(ref.pack(q, t, k)), b.put(s)) if x_type == ffi.F8 else (b.put(floats, floats.itemsize), 0)
+            y = b.filled(t * n * size + 64)
             for again in range(2):  # a second time over the same tickets
                 if not glu:
-                    dec.lin_forward_f8("b", dq, y, t, x_type=ffi.F8, xs_dev=ds, y_type=y_type)
+                    dec.lin_forward_f8("b", dq, y, t, x_type=x_type, xs_dev=ds, y_type=y_type)
                     out, ran = n, cc.last_launch_symbol()
                     got = cc.d2h(y, (t, n), w8.bits_type(y_type))
                     if whole:
@@ -167,7 +171,7 @@ def test_every_build(dec, key):
                         ref.near(ref.value(got, y_type), want, space, y_type)
                         assert ref.rel_norm(ref.value(got, y_type), want) <= (1.1e-3 if "tiled" in ran else 2e-6) + ref.half_step(y_type)
                 else:
-                    dec.lin_forward_f8_glu("b", dq, y, t, x_type=ffi.F8, xs_dev=ds, y_type=y_type, gelu=bool(again))
+                    dec.lin_forward_f8_glu("b", dq, y, t, x_type=x_type, xs_dev=ds, y_type=y_type, gelu=bool(again))
                     out, ran = n // 2, cc.last_launch_symbol()
                     got = cc.d2h(y, (t, out), w8.bits_type(y_type))
                     if whole and y_type == ffi.F16:  # the separate kernel's activation of the same f32 sums
