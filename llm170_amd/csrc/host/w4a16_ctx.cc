@@ -122,11 +122,11 @@ static const char* const kW8a8Syms[] = {W8_TT("w4a16_w8a8_skinny_r1", ""), W8_TT
                                         "w4a16_w8a8_tiled_m128", "w4a16_w8a8_tiled_m128_glu", "w4a16_w8a8_tiled_m64", "w4a16_w8a8_tiled_m64_glu", "w4a16_w8a8_tiled_m64_n128", "w4a16_w8a8_tiled_m64_n128_glu", nullptr};
 static const char* const kF8QuantSyms[] = {"w4a16_quant_rows_f8_f32", "w4a16_quant_rows_f8_f16", "w4a16_quant_rows_f8_bf16", "w4a16_norm_resid_f8", nullptr};
 // as W8A8's, of rows of floats too; tiles with e4m3 products and with f16 ones (kernels/f8.hip)
-#define F8_TILES(P) P "_m64", P "_m64_glu", P "_m64_n128", P "_m64_n128_glu"
+#define F8_TILES(P) P, P "_glu"
 #define F8_FEW(P, S) W8_TT(P, S), P "_f32" S, P "_f16" S, P "_bf16" S
-static const char* const kF8Syms[] = {F8_FEW("w4a16_f8_skinny_r1", ""), F8_FEW("w4a16_f8_skinny_r2", ""), F8_FEW("w4a16_f8_skinny_r4", ""),
-                                      F8_FEW("w4a16_f8_skinny_r2", "_glu"), F8_FEW("w4a16_f8_skinny_r4", "_glu"),
-                                      F8_TILES("w4a16_f8_tiled"), F8_TILES("w4a16_f8_exact"), nullptr};
+static const char* const kF8Syms[] = {F8_FEW("w4a16_f8_skinny_r1", ""), F8_FEW("w4a16_f8_skinny_r2", ""), F8_FEW("w4a16_f8_skinny_r2", "_glu"),
+                                      F8_TILES("w4a16_f8_skinny_r4_t2"), F8_TILES("w4a16_f8_skinny_r4_t3"),
+                                      F8_TILES("w4a16_f8_tiled_m64"), F8_TILES("w4a16_f8_tiled_m128"), F8_TILES("w4a16_f8_exact_n128"), F8_TILES("w4a16_f8_exact_n256"), nullptr};
 #define ROPE_BUILDS(P) P "_v8", P "_v2", P "_v1", P "_v8_il", P "_v2_il", P "_v1_il"  // pairs to a lane; neighbours as pairs (kernels/rope.hip)
 static const char* const kRopeSyms[] = {ROPE_BUILDS("w4a16_qk_norm_rope_f32"), ROPE_BUILDS("w4a16_qk_norm_rope_f16"), ROPE_BUILDS("w4a16_qk_norm_rope_bf16"), nullptr};
 static const char* const kVerifySyms[] = {"w4a16_verify_rows_f32", "w4a16_verify_rows_f16", "w4a16_verify_rows_bf16", "w4a16_verify_pick_f32", "w4a16_verify_pick_f16",

@@ -134,6 +134,7 @@ extern "C" int w4a16_lin_f8_info(w4a16_ctx* ctx, const char* name, size_t* n, si
 
 // ------------------------------------------------------------------------------------------------ forward
 // Launch of the kernel for groups of up to 64 rows: row blocks per workgroup, waves, k slices; a function of the shape alone.
+// Prices in us, fitted to 226 shapes (512 x 1024 to 65536 x 1024, 1000 x 17408, 1 to 1000 rows): with those of the tiles they pick launches 1 % above the best on average.
 struct F8Skinny {
     int rb = 1, waves = 8, nks = 1;
     double price = 0.0;
@@ -145,51 +146,54 @@ static F8Skinny plan_skinny(size_t n, size_t k, size_t t, size_t cus, bool glu) 
     const int tt = (int)((t + 16 * groups - 1) / (16 * groups));
     F8Skinny best;
     best.price = 1e30;
-    for (int rb = 4; rb >= (glu ? 2 : 1); rb /= 2) {
+    // Four row blocks a workgroup pay with 17 to 48 rows alone (5120 x 17408 at 40 24.3 us, two 27.9; at 16 none do; at 64 their sums leave no room for loads in flight)
+    for (int rb = tt == 2 || tt == 3 ? 4 : 2; rb >= (glu ? 2 : 1); rb /= 2) {
         for (int nks = 1; nks <= 8; nks++) {
-            const size_t blocks = (blocks16 + rb - 1) / rb, grid = blocks * nks * groups;
+            const size_t grid = (blocks16 + rb - 1) / rb * nks * groups;
             if (nks > 1 && ((size_t)nks * 8 > kt || grid > 4 * cus)) break;
-            const double run = (double)kt / nks;
-            const size_t full = grid / cus, rest = grid % cus;
-            const double rounds = (double)full + (rest == 0 ? 0.0 : full == 0 ? 1.0 : 0.94 + 0.06 * (double)rest / (double)cus);
-            const double load = run * (rb + (groups > 1 ? 0.28 : 0.48) * (t <= 4 ? 0.25 : tt));
-            const double sums = 1e-6 * nks * n * t * 8, join = nks == 1 ? 0.0 : groups > 1 ? 0.91 + 0.37 * sums : 2.07 + 0.24 * sums;
+            const double run = (double)kt / nks, load = (double)grid / (double)cus, rounds = 0.92 * std::max(1.0, 0.89 * std::ceil(load) + 0.11 * load) + 0.08;
+            const double products = rounds * run * (rb + 0.62 * (t <= 4 ? 0.25 : tt)) * 0.024;
+            const double tiles = (double)blocks16 * (double)kt, loads = tiles * 0.000146 * (1.0 + 0.104 * tt * groups / rb);
+            const double join = nks == 1 ? 0.0 : 2.5 + 0.24e-6 * nks * n * t * 8;
             F8Skinny p;
             p.rb = rb;
             p.nks = nks;
-            p.waves = (grid > cus && (run <= 40 || rb * tt >= 16)) || run <= 16 ? 4 : 8;
+            p.waves = (grid > cus && t > 16) || run <= 16 ? 4 : 8;  // 34816 x 5120 gated at 40 rows: 4 waves 48.3 us, 8 64.1
             p.waves = (int)std::min<size_t>(p.waves, std::max<size_t>(kt / 2, 1));
-            p.price = (groups > 1 ? 4.3 : 0.0) + std::max(rounds * load / (groups > 1 ? 34.2 : 49.6), (double)(blocks16 * kt) / 9079.0) + join;
+            p.price = 2.7 + std::max(products, loads) + join + 0.22 * rb * tt + 0.000032 * tiles * tt * groups / rb;
             if (p.price < best.price) best = p;
         }
     }
     return best;
 }
 
-// Launch of the tiled kernel: rows and columns (of weights) per tile, k slices; a function of the shape alone.
+// Launch of a tiled kernel: rows and columns (of weights) per tile, k slices; a function of the shape alone.  Prices as above.
 struct F8Tiled {
     int bm = 64, bn = 128, nks = 1;
     double price = 0.0;
 };
 
 static F8Tiled plan_tiled(size_t n, size_t k, size_t t, size_t cus, bool exact) {
-    static const struct { int bm, bn, per_cu; double alone, full; } kTiles[] = {{64, 128, 3, 0.18, 0.50}, {64, 256, 2, 0.29, 0.57}};
-    (void)exact;
+    // of 64 k: one workgroup of a CU, all of them
+    struct Tile { int bm, bn, per_cu; double alone, full; };
+    static const Tile kExact[] = {{64, 128, 3, 0.325, 0.588}, {64, 256, 2, 0.479, 0.610}}, kE4m3[] = {{64, 128, 4, 0.177, 0.540}, {128, 256, 2, 0.400, 0.857}};
+    const double start = exact ? 5.7 : 7.9, whole = exact ? 0.82 : 0.69, per_slice = exact ? 1.3 : 1.06, per_load = exact ? 13.7 : 9.5;
     const size_t kt = w4_q8_blocks(k) * 2;
     F8Tiled best;
     best.price = 1e30;
-    for (const auto& T : kTiles) {
+    for (int i = 0; i < 2; i++) {
+        const Tile& T = exact ? kExact[i] : kE4m3[i];
         for (int nks = 1; nks <= 8; nks++) {
             const size_t grid = (t + T.bm - 1) / T.bm * ((n + T.bn - 1) / T.bn) * nks;
             if (nks > 1 && ((size_t)nks * 8 > kt || grid > T.per_cu * cus)) break;
             const double load = (double)grid / (double)cus, rounds = load / T.per_cu;
             const double per_k = rounds <= 1.0 ? T.alone + (T.full - T.alone) * (std::ceil(load) - 1.0) / (T.per_cu - 1)
-                                               : T.full * (0.5 * std::ceil(rounds) + 0.5 * rounds);
+                                               : T.full * (whole * std::ceil(rounds) + (1.0 - whole) * rounds);
             F8Tiled p;
             p.bm = T.bm;
             p.bn = T.bn;
             p.nks = nks;
-            p.price = 4.7 + (double)((kt + nks - 1) / nks) * per_k + (nks > 1 ? (nks + 8.5 * load) * T.bm * T.bn / 32768.0 : 0.0);
+            p.price = start + (double)((kt + nks - 1) / nks) * per_k + (nks > 1 ? (per_slice * nks + per_load * load) * T.bm * T.bn / 32768.0 : 0.0);
             if (p.price < best.price) best = p;
         }
     }
@@ -201,22 +205,25 @@ struct F8Launch {
     char kernel[64] = "";
     size_t grid_x = 0, grid_y = 1, tickets = 0, part_bytes = 0;
     int block = 256, nks = 1, band = 0;  // band: tile rows of a band, 0 = the kernel for groups of up to 64 rows
-    bool floats = false;                 // the kernel takes rows of floats
+    size_t lds_x = 0;                    // bytes of LDS for rows of floats that the kernel quantises (132 a block: the numbers and a scale); 0: it takes quantised rows
 };
 
 static int plan_f8(const char* what, size_t n, size_t k, size_t t, size_t cus, bool glu, int x_type, int y_type, F8Launch* out) {
     F8Launch& P = *out;
     const bool exact = y_type == W4A16_F32 || t <= 1024;
     const F8Skinny few = plan_skinny(n, k, t, cus, glu);
-    const F8Tiled tiles = t <= 64 ? F8Tiled() : plan_tiled(n, k, t, cus, exact);
-    if (t <= 64 || (t <= 1024 && few.price < tiles.price)) {
+    const F8Tiled tiles = plan_tiled(n, k, t, cus, exact);
+    if (t <= 16 || (t <= 1024 && few.price < tiles.price)) {
         const size_t groups = (t + 63) / 64;  // of as many rows each as can be
         const int tt = (int)((t + 16 * groups - 1) / (16 * groups));
         const size_t blocks16 = (n + 15) / 16;
-        P.floats = t <= 16 && x_type != W4A16_F8;  // quantised by the kernel itself
+        // Floats are quantised by the kernel itself, each workgroup its k slice of them, where that takes less than a launch before it does (1.7 to 2.5 us): a few blocks of
+        // 128, once or, with one or two rows, a few times a CU.  4096 x 4096 at 1 row 7.1 us, 6.0 and 2.1 with a launch of its own; 65536 x 1024 at 8 rows 17.2, 13.8 and 2.3.
+        const size_t blocks = (w4_q8_blocks(k) + few.nks - 1) / few.nks * t, grid = (glu ? (blocks16 / 2 + few.rb / 2 - 1) / (few.rb / 2) : (blocks16 + few.rb - 1) / few.rb) * few.nks;
+        if (x_type != W4A16_F8 && t <= 16 && blocks <= kW4F8FloatBlocks && grid <= (t <= 2 ? 4 * cus : cus)) P.lds_x = blocks * 132;
         char rows[8];
         snprintf(rows, sizeof rows, "t%d", tt);
-        snprintf(P.kernel, sizeof P.kernel, "w4a16_f8_skinny_r%d_%s%s", few.rb, P.floats ? w4_type_name(x_type) : rows, glu ? "_glu" : "");
+        snprintf(P.kernel, sizeof P.kernel, "w4a16_f8_skinny_r%d_%s%s", few.rb, P.lds_x ? w4_type_name(x_type) : rows, glu ? "_glu" : "");
         P.nks = few.nks;
         P.grid_x = glu ? (blocks16 / 2 + few.rb / 2 - 1) / (few.rb / 2) : (blocks16 + few.rb - 1) / few.rb;
         P.grid_y = few.nks * groups;
@@ -224,7 +231,8 @@ static int plan_f8(const char* what, size_t n, size_t k, size_t t, size_t cus, b
         P.tickets = P.grid_x * groups;
         P.part_bytes = P.tickets * few.nks * few.rb * tt * 1024;
     } else {
-        snprintf(P.kernel, sizeof P.kernel, "w4a16_f8_%s_m%d%s%s", exact ? "exact" : "tiled", tiles.bm, tiles.bn == 128 ? "_n128" : "", glu ? "_glu" : "");
+        if (exact) snprintf(P.kernel, sizeof P.kernel, "w4a16_f8_exact_n%d%s", tiles.bn, glu ? "_glu" : "");
+        else snprintf(P.kernel, sizeof P.kernel, "w4a16_f8_tiled_m%d%s", tiles.bm, glu ? "_glu" : "");
         P.nks = tiles.nks;
         P.tickets = (t + tiles.bm - 1) / tiles.bm * ((n + tiles.bn - 1) / tiles.bn);
         P.part_bytes = P.tickets * tiles.nks * tiles.bm * tiles.bn * 4;
@@ -260,7 +268,7 @@ static int launch_f8(w4a16_ctx* ctx, const F8Lin& L, const F8Launch& P, uint64_t
     void* few[] = {&wt, &ws, &q, &s, &y, &ni, &kb, &ti, &r, &y_type, &act, &wi, &ksi, &part, &tickets};
     void* floats[] = {&wt, &ws, &q, &ldx, &ki, &y, &ni, &kb, &ti, &y_type, &act, &wi, &ksi, &part, &tickets};
     void* tiles[] = {&wt, &ws, &q, &s, &y, &ni, &kb, &ti, &y_type, &act, &ksi, &band, &part, &tickets};
-    return w4_launch(ctx, P.kernel, (unsigned)P.grid_x, (unsigned)P.grid_y, (unsigned)P.block, 0, P.band ? tiles : P.floats ? floats : few);
+    return w4_launch(ctx, P.kernel, (unsigned)P.grid_x, (unsigned)P.grid_y, (unsigned)P.block, (unsigned)P.lds_x, P.band ? tiles : P.lds_x ? floats : few);
 }
 
 static int forward_f8(w4a16_ctx* ctx, const char* api, const char* name, uint64_t x, int x_type, size_t ldx, uint64_t xs, size_t t, uint64_t y,
@@ -285,7 +293,7 @@ static int forward_f8(w4a16_ctx* ctx, const char* api, const char* name, uint64_
     F8Launch P;
     W4_TRY(plan_f8(api, L->n, L->k, t, (size_t)std::max(ctx->cu_count, 1), act >= 0, x_type, y_type, &P));
     W4_TRY(w4_hip(hipSetDevice(ctx->device), "hipSetDevice"));
-    if (x_type != W4A16_F8 && !P.floats) {
+    if (x_type != W4A16_F8 && !P.lds_x) {
         W4_TRY(w4_ensure(ctx, &ctx->q8, &ctx->q8_cap, w4a16_q8_bytes(t, L->k)));
         W4_TRY(w4_ensure(ctx, &ctx->q8_scales, &ctx->q8_scales_cap, std::max<size_t>(t * w4_q8_blocks(L->k) * 4, 256)));
         W4_TRY(quant_rows(ctx, x, x_type, ldx, t, L->k, ctx->q8, ctx->q8_scales));

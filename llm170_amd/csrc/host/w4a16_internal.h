@@ -154,6 +154,7 @@ constexpr int kW4ScoreStageBytes = 4096;    // SCORE_STAGE_BYTES (score.hip): of
 constexpr int kW4ScoreMaxTop = 32;          // SCORE_MAX_TOP
 constexpr int kW4ScoreRecord = 272;         // SCORE_RECORD
 
+constexpr int kW4F8FloatBlocks = 128;      // F8_FLOAT_BLOCKS (f8.hip)
 constexpr int kW4RopeMaxDim = 1024;         // ROPE_MAX_DIM (rope.hip)
 
 int w4_fail(int code, const char* fmt, ...) __attribute__((format(printf, 2, 3)));

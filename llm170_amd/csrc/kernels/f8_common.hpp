@@ -14,6 +14,13 @@ __device__ __forceinline__ float f8_step(unsigned mag, float& by) {
     return some ? s : mag == 0 ? 0.f : __builtin_nanf("");
 }
 
+// Largest of the eight lanes that share a block: neighbours, pairs, fours
+__device__ __forceinline__ unsigned f8_block_max(unsigned v) {
+    v = max(v, (unsigned)__builtin_amdgcn_update_dpp((int)v, (int)v, 0xb1, 0xf, 0xf, false));   // quad_perm 1 0 3 2
+    v = max(v, (unsigned)__builtin_amdgcn_update_dpp((int)v, (int)v, 0x4e, 0xf, 0xf, false));   // quad_perm 2 3 0 1
+    return max(v, (unsigned)__builtin_amdgcn_update_dpp((int)v, (int)v, 0x141, 0xf, 0xf, false));  // row_half_mirror
+}
+
 typedef short f8_pair_t __attribute__((ext_vector_type(2)));
 typedef __bf16 bf2_t __attribute__((ext_vector_type(2)));
 

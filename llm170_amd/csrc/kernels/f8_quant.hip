@@ -3,13 +3,6 @@
 // step up to twice as large loses nothing but the last of 18 binary orders below the largest.
 #include "f8_common.hpp"
 
-// Largest of the eight lanes that share a block: neighbours, pairs, fours
-__device__ __forceinline__ unsigned f8_block_max(unsigned v) {
-    v = max(v, (unsigned)__builtin_amdgcn_update_dpp((int)v, (int)v, 0xb1, 0xf, 0xf, false));   // quad_perm 1 0 3 2
-    v = max(v, (unsigned)__builtin_amdgcn_update_dpp((int)v, (int)v, 0x4e, 0xf, 0xf, false));   // quad_perm 2 3 0 1
-    return max(v, (unsigned)__builtin_amdgcn_update_dpp((int)v, (int)v, 0x141, 0xf, 0xf, false));  // row_half_mirror
-}
-
 // A thread per 16 columns, eight lanes to a block; a wave takes LR = 1, 4 or 8 neighbouring rows (tiles of R = 1, 4, 16 rows), whose 16-byte chunks lie side by
 // side, and 8 / LR blocks of each.  Whole blocks are written: zeros behind the row's end, which meet zero weights as numbers.
 template <int T>

@@ -40,15 +40,15 @@ def test_pack_is_what_unpack_reads():
 @functools.lru_cache(None)
 def shapes():
     """(t, n, k, gated, row type, result type) of every build, found by the plans themselves: the first of a fixed walk that goes to it."""
-    r = np.random.default_rng(11)
+    r = np.random.default_rng(13)
     found = {}
     want = set(itertools.product(manifest("f8"), (False, True)))
     for _ in range(200000):
         t = int(np.exp(r.uniform(0, np.log(2600))))
-        n, k = int(np.exp(r.uniform(np.log(20), np.log(14000)))), int(np.exp(r.uniform(np.log(140), np.log(9000))))
+        n, k = int(np.exp(r.uniform(np.log(20), np.log(14000)))), int(np.exp(r.uniform(np.log(140), np.log(17408))))
         glu, y_type, x_type = bool(r.integers(2)), int(r.integers(3)), int(r.choice([0, 1, 2, 4, 4, 4]))
         n = max(256, n // 256 * 256) if glu else n
-        if float(t) * n * k > 4e9:
+        if float(t) * n * k > 6e10:
             continue
         p = ops.plan_f8(t, n, k, glu=glu, x_type=x_type, y_type=y_type)
         found.setdefault((p["kernel"], p["k_slices"] > 1), (t, n, k, glu, x_type, y_type))
@@ -63,24 +63,26 @@ def test_every_build_has_a_shape_with_whole_k_and_in_slices():
 
 def test_plans_hold_what_the_kernels_count_on():
     """At most eight waves and eight k slices, a block of 128 at least for every wave of every slice, groups of up to 64 rows that cover all of them;
-    grids of fewer than 2^32 threads; 32-bit sums for f32 results and up to 1024 rows; up to 16 rows of floats without a launch to quantise them."""
+    grids of fewer than 2^32 threads; 32-bit sums for f32 results and up to 1024 rows; few rows of floats without a launch to quantise them."""
     r = np.random.default_rng(6)
     for _ in range(20000):
         t, n, k = (int(np.exp(r.uniform(0, np.log(top)))) for top in (5000, 300000, 131071))
         glu, y_type, x_type = bool(r.integers(2)), int(r.integers(3)), int(r.choice([0, 1, 2, 4]))
         n = max(256, n // 256 * 256) if glu else n
-        p = ops.plan_f8(t, n, k, cu_count=int(r.integers(1, 305)), glu=glu, x_type=x_type, y_type=y_type)
+        cus = int(r.integers(1, 305))
+        p = ops.plan_f8(t, n, k, cu_count=cus, glu=glu, x_type=x_type, y_type=y_type)
         kb = (k + 127) // 128
         assert 1 <= p["k_slices"] <= 8 and p["workgroups"] * p["waves"] * 64 < 2**32 and ("_glu" in p["kernel"]) == glu
         if "skinny" in p["kernel"]:
             rows = p["kernel"].split("_")[4]
-            assert rows == (["f32", "f16", "bf16"][x_type] if t <= 16 and x_type != ffi.F8 else rows) and (rows[0] == "t") == (t > 16 or x_type == ffi.F8)
+            itself = t <= 16 and x_type != ffi.F8 and -(-kb // p["k_slices"]) * t <= 128 and p["workgroups"] <= (4 * cus if t <= 2 else cus)  # quantised by the kernel
+            assert rows == ["f32", "f16", "bf16", "", ""][x_type] if itself else rows[0] == "t"
             rb, tt = int(p["kernel"].split("_")[3][1:]), int(rows[1:]) if rows[0] == "t" else 1
             groups, columns = -(-t // 64), -(-(n // 2 if glu else n) // 16)
             assert 1 <= p["waves"] <= 8 and p["waves"] * p["k_slices"] <= kb and 16 * tt * groups >= t > 16 * tt * (groups - 1)
             assert p["workgroups"] == -(-columns // (rb // 2 if glu else rb)) * p["k_slices"] * groups
         else:
-            assert p["waves"] == 4 and p["k_slices"] <= kb and t > 64 and ("exact" in p["kernel"]) == (y_type == ffi.F32 or t <= 1024)
+            assert p["waves"] == 4 and p["k_slices"] <= kb and t > 16 and ("exact" in p["kernel"]) == (y_type == ffi.F32 or t <= 1024)
 
 
 def test_plan_refusals():
