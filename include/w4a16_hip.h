@@ -555,9 +555,9 @@ int w4a16_plan_w8a8(size_t n, size_t k, size_t t, int cu_count, int glu, char* k
  * A block of a row x is quantised with the least power of two s >= 2^-126 that brings its largest magnitude to 448 or below; q = x / s to the nearest e4m3
  * number (halves to the even one), exactly: powers of two make the quotients exact and cost no relative precision.  A block of zeros has s = 0, one that holds infinity or
  * NaN s = NaN (and so has every output of its row) and q = 0.
- * Sums are held in f32, a block's products summed first; the result is rounded once more to y's type.  f32 results, and any of up to 1024 rows, are sums of 32 bits.
- * For f16 and bf16 results of more rows the products of a block may be summed by the e4m3 matrix instruction, which drops of a product what lies more than 2^-13 below the
- * largest of its group: 1.6e-5 of the results' size on normal numbers, 1 / 17 of an f16 result's own rounding.  The same call gives the same bits every time.
+ * Sums are held in f32, a block's products summed first; the result is rounded once more to y's type.  f32 results, those of up to 64 rows and gated ones of up to 1024 are
+ * sums of 32 bits.  For other f16 and bf16 results the products of a block may be summed by the e4m3 matrix instruction, which drops of a product what lies more than 2^-13 below
+ * the largest of its group: 1.6e-5 of the results' size on normal numbers, 1 / 17 of an f16 result's own rounding.  The same call gives the same bits every time.
  * Streams, captures, scratch and the number of rows: as for the W8A8 linears above.
  * ---------------------------------------------------------------------------------------------------------- */
 

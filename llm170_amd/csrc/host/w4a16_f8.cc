@@ -176,8 +176,8 @@ struct F8Tiled {
 static F8Tiled plan_tiled(size_t n, size_t k, size_t t, size_t cus, bool exact) {
     // of 64 k: one workgroup of a CU, all of them
     struct Tile { int bm, bn, per_cu; double alone, full; };
-    static const Tile kExact[] = {{64, 128, 3, 0.325, 0.588}, {64, 256, 2, 0.479, 0.610}}, kE4m3[] = {{64, 128, 4, 0.177, 0.540}, {128, 256, 2, 0.400, 0.857}};
-    const double start = exact ? 5.7 : 7.9, whole = exact ? 0.82 : 0.69, per_slice = exact ? 1.3 : 1.06, per_load = exact ? 13.7 : 9.5;
+    static const Tile kExact[] = {{64, 128, 3, 0.325, 0.588}, {64, 256, 2, 0.479, 0.610}}, kE4m3[] = {{64, 128, 4, 0.213, 0.549}, {128, 256, 2, 0.437, 0.857}};
+    const double start = exact ? 5.7 : 6.7, whole = exact ? 0.82 : 0.77, per_slice = exact ? 1.3 : 1.23, per_load = exact ? 13.7 : 9.7;
     const size_t kt = w4_q8_blocks(k) * 2;
     F8Tiled best;
     best.price = 1e30;
@@ -210,7 +210,7 @@ struct F8Launch {
 
 static int plan_f8(const char* what, size_t n, size_t k, size_t t, size_t cus, bool glu, int x_type, int y_type, F8Launch* out) {
     F8Launch& P = *out;
-    const bool exact = y_type == W4A16_F32 || t <= 1024;
+    const bool exact = y_type == W4A16_F32 || t <= 64 || (glu && t <= 1024);  // the products' own precision: kernels/f8.hip
     const F8Skinny few = plan_skinny(n, k, t, cus, glu);
     const F8Tiled tiles = plan_tiled(n, k, t, cus, exact);
     if (t <= 16 || (t <= 1024 && few.price < tiles.price)) {
