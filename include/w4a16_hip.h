@@ -604,7 +604,7 @@ int w4a16_token_logprobs(w4a16_ctx* ctx, uint64_t logits_dev, int logits_type, s
  * With p and q the softmax of target and draft logits over temps[b] (f32 [seqs], 0: all 1), a drafted token x is accepted while u q(x) < p(x).  Behind the last one accepted
  * comes one token more: the first whose running sum of max(0, p - q) where one was rejected (of p, where that is zero everywhere), of p behind the last draft, in the order of
  * tokens, exceeds the sequence's last u times the whole sum.  A temperature that is not above 0: accepted is the most likely token (of equal ones the lowest), which also
- * follows.  Powers and sums are of 64 bits.
+ * follows.  Sums that decide are of 32-bit powers (some 10^-7 of p and q), those that draw of 64-bit ones.
  *   tokens int32 [t]: of each sequence the accepted tokens, the one that follows, -1 for the rest of its rows (tokens may be drafted); accepted int32 [seqs]: how many were.
  * Rows of no sequence are left as they are.  -infinity rules a token out.  A target's row that holds NaN or +infinity, or nothing but -infinity, has no distribution: its draft
  * is rejected and -1 follows.  Where a draft's row has none, or a drafted token is none of the vocabulary, it is rejected and p (without that token, if it was certain) is drawn from. */

@@ -17,15 +17,15 @@ extern "C" int w4a16_verify_drafts(w4a16_ctx* ctx, uint64_t logits_dev, int logi
     if ((logits_dev | draft_dev) % w4_type_bytes(logits_type) || (row0_dev | drafted_dev | u_dev | temps_dev | tokens_dev | accepted_dev) % 4)
         return w4_fail(W4A16_ERR_ARG, "%s: operands must be aligned to their elements", api);
     W4_TRY(w4_hip(hipSetDevice(ctx->device), "hipSetDevice"));
-    // Elements of a segment, of whole stages of a workgroup's four waves.  Rows: as many segments as make twelve workgroups to a CU; us with 1 / 4 / 8 / 12 / 16 / 40 of them: 193 rows
-    // of 131072 bf16 with drafts 30.6 / 25.8 / 26.5 / 25.9 / 28.3 / 38.6; 400 of 100003 f16 45.5 / 44.9 / 46.0 / 43.2 / 40.0 / 42.6.  Pick: one stage (28 and 62 us; two 35 and 71).
+    // Elements of a segment, of whole stages of a workgroup's four waves.  Rows: as many segments as make twelve workgroups to a CU; us with 1 / 4 / 8 / 12 / 16 / 24 / 40 of them: 193 rows
+    // of 131072 bf16 with drafts 24.0 / 21.3 / 22.9 / 22.4 / 25.2 / 25.7 / 37.5; 400 of 100003 f16 41.0 / 40.8 / 40.7 / 32.4 / 31.1 / 33.3 / 33.5.  Pick: one stage.
     const size_t stage = 4 * 4096 / w4_type_bytes(logits_type), streams = draft_dev ? 2 : 1, cus = (size_t)std::max(ctx->cu_count, 1);
     const size_t stages = (n_vocab + stage - 1) / stage, want = std::min(stages, std::max<size_t>(1, 12 * cus / (t * streams)));
     const size_t seg = (stages + want - 1) / want * stage, segs = (n_vocab + seg - 1) / seg;
-    const size_t pick_seg = stage, pick_segs = stages;
+    const size_t pick_segs = stages;
     if (pick_segs > 0xffffffu / streams || t * streams > 0xffffffffffu / segs || seqs > 0xffffffffffu / pick_segs)
         return w4_fail(W4A16_ERR_SHAPE, "%s: t=%zu seqs=%zu n_vocab=%zu exceed the scratch", api, t, seqs, n_vocab);
-    const size_t rows_at = t * streams * segs * 16, parts_at = rows_at + t * 32, bytes = parts_at + seqs * pick_segs * 40;
+    const size_t rows_at = t * streams * segs * 16, parts_at = rows_at + t * 32, bytes = parts_at + seqs * pick_segs * 4 * 40;  // a part of a row to each wave
     W4_TRY(w4_ensure(ctx, &ctx->verify_ws, &ctx->verify_ws_cap, bytes));
     if ((t + seqs) * 4 > ctx->verify_tickets_cap) {
         W4_TRY(w4_ensure(ctx, &ctx->verify_tickets, &ctx->verify_tickets_cap, std::max<size_t>((t + seqs) * 4, 8192)));
@@ -34,7 +34,7 @@ extern "C" int w4a16_verify_drafts(w4a16_ctx* ctx, uint64_t logits_dev, int logi
         W4_TRY(rc);
     }
     uint64_t sums = ctx->verify_ws, rows = sums + rows_at, parts = sums + parts_at, row_tickets = ctx->verify_tickets, seq_tickets = row_tickets + t * 4;
-    int v = (int)n_vocab, ti = (int)t, nb = (int)seqs, sg = (int)segs, sl = (int)std::min<size_t>(seg, 0x7fffffff), psg = (int)pick_segs, psl = (int)pick_seg, first = 0;
+    int v = (int)n_vocab, ti = (int)t, nb = (int)seqs, sg = (int)segs, sl = (int)std::min<size_t>(seg, 0x7fffffff), psg = (int)pick_segs, first = 0;
     char sym[64];
     // HIP takes fewer than 2^32 threads in a launch: more rows or sequences go in several
     snprintf(sym, sizeof sym, "w4a16_verify_rows_%s", w4_type_name(logits_type));
@@ -47,7 +47,7 @@ extern "C" int w4a16_verify_drafts(w4a16_ctx* ctx, uint64_t logits_dev, int logi
     snprintf(sym, sizeof sym, "w4a16_verify_pick_%s", w4_type_name(logits_type));
     for (size_t at = 0; at < seqs; at += most_seqs) {
         first = (int)at;
-        void* params[] = {&logits_dev, &ld, &draft_dev, &ld_draft, &v, &ti, &first, &row0_dev, &drafted_dev, &u_dev, &temps_dev, &psg, &psl, &rows, &parts, &seq_tickets,
+        void* params[] = {&logits_dev, &ld, &draft_dev, &ld_draft, &v, &ti, &first, &row0_dev, &drafted_dev, &u_dev, &temps_dev, &psg, &rows, &parts, &seq_tickets,
                           &tokens_dev, &accepted_dev};
         W4_TRY(w4_launch(ctx, sym, (unsigned)(std::min(most_seqs, seqs - at) * pick_segs), 1, 256, 0, params));
     }

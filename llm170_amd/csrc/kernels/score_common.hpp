@@ -91,6 +91,15 @@ struct ScoreChunk {
         else asm("v_fma_mix_f32 %0, %1, %2, -%3 op_sel_hi:[1,0,0]" : "=v"(d) : "v"(h), "s"(l), "v"(r));
         return d;
     }
+    // value(e) - m; an f16 enters the subtraction as it is
+    __device__ __forceinline__ float minus(int e, float m) const {
+        if (T != Q8_F16) return value(e) - m;
+        float d;
+        const unsigned h = w[e / PER][e % PER / 2];
+        if (e & 1) asm("v_fma_mix_f32 %0, %1, 1.0, -%2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(d) : "v"(h), "v"(m));
+        else asm("v_fma_mix_f32 %0, %1, 1.0, -%2 op_sel_hi:[1,0,0]" : "=v"(d) : "v"(h), "v"(m));
+        return d;
+    }
     // the largest and the smallest (NaN if there is one); f16 two at a time
     __device__ __forceinline__ void extremes(float& most, float& least) const {
         if (T == Q8_F16) {

@@ -4,13 +4,15 @@
 // running sum exceeds u_last times the whole sum.  Temperature 0: accepted is the most likely token, which also follows.
 //
 // Two launches.  Rows: a segment of a target's or a draft's row to a workgroup, with a running maximum in each thread; it leaves (sum, maximum) of its segment, and the last
-// of a row joins them and judges the row's token.  A decision wants its sum to some 10^-7, so powers are of 32 bits here and the stream of the logits is what takes the time.
-// Pick: of the first row that is not accepted alone, a segment to a workgroup.  Running sums over a vocabulary meet a border between two tokens about once in V / (relative error)
+// of a row joins them and judges the row's token.  A decision wants its sum to some 10^-7, so powers are of 32 bits here, some 7 instructions an element, and the stream of the logits
+// takes most of the time: 193 rows of 131072 bf16 with 129 drafts' 22.4 us (84 MB, 3.8 TB/s), 400 of 100003 f16 with 200 drafts' 31.9 (120 MB).
+// Pick: of the first row that is not accepted alone, a stage of 64 lanes to a wave.  Running sums over a vocabulary meet a border between two tokens about once in V / (relative error)
 // draws, so powers and sums are of 64 bits: 2^x by a polynomial of degree 8 (interpolation at Chebyshev nodes of [-1/2, 1/2], off by 1.1e-12), some 17 instructions of four
-// cycles.  A segment leaves sum p, sum q and, over the tokens where p is above q by the first launch's sums, sum p and sum q again: what is known of the whole sums then makes sum max(0, p - q) of
-// them.  Tokens that the first launch's 10^-7 puts on the wrong side have no more than that share of themselves to give; where that is over 10^-9 of the whole, target and draft being
-// nearly alike, the sums are made again with what is known now.  The last workgroup of a sequence finds the segment that holds the draw, a thread of it sums a run of neighbours, and the run
-// that holds it is gone over again, an element to a lane.
+// cycles, which are what takes the time where there are many sequences: 64 of them 21.8 us (7 of arithmetic; launch, loads that depend on each other and the last workgroup's work the rest), 200 48.5 (28).
+// A wave leaves sum p, sum q and, by the first launch's sums (`rough` of the draft's power is one of the target's), sum max(0, p - q) and the sum of q where p is above q: what is
+// known of the whole sums then changes it by their difference times the last.  Tokens that the first launch's 10^-7 puts on the wrong side have no more than that share of themselves to
+// give; where that is over 10^-9 of the whole, target and draft being nearly alike, the sums are made again with what is known now.  The last workgroup of a sequence finds the
+// wave's stage that holds the draw, a thread of it sums a few neighbours, and the few that hold it are gone over again, an element to a lane.
 #include "score_common.hpp"
 
 #define VERIFY_WAVES 4
@@ -27,14 +29,14 @@ struct VerifySum {  // of a segment: sum of powers relative to its maximum; or t
     float m;
     int pad;
 };
-struct VerifyPart {  // of a segment of a row that is drawn from: sums of the powers of target and draft, all and where p > q; of the target's where p is nearly q
-    double v[5];
+struct VerifyPart {  // of a wave's stage of a row that is drawn from: sums of the powers of target and draft; of max(0, target - rough draft); of the draft's where that is above 0, and where it is
+    double v[5];     // nearly 0 (the last two of 32 bits)
 };
 #define VERIFY_E 0
 #define VERIFY_D 1
-#define VERIFY_E_OVER 2
+#define VERIFY_MORE 2
 #define VERIFY_D_OVER 3
-#define VERIFY_E_NEAR 4
+#define VERIFY_D_NEAR 4
 #define VERIFY_NEAR 1e-6
 
 // 2^x, x <= 0; a NaN counts as far below
@@ -72,6 +74,12 @@ __device__ __forceinline__ double verify_wave_scan(double v) {  // of this lane 
         if (lane >= d) v += o;
     }
     return v;
+}
+
+__device__ __forceinline__ double verify_of_lane(double v, int lane) {
+    const bits_t b = __builtin_bit_cast(bits_t, v);
+    const unsigned lo = (unsigned)__builtin_amdgcn_readlane((int)b, lane), hi = (unsigned)__builtin_amdgcn_readlane((int)(b >> 32), lane);
+    return __builtin_bit_cast(double, (bits_t)hi << 32 | lo);
 }
 
 __device__ __forceinline__ void verify_put(VerifySum* p, VerifySum v) {  // device scope: past this XCD's L2
@@ -130,8 +138,9 @@ __device__ __forceinline__ void verify_rows_body(const void* __restrict__ logits
     const float temp = temps ? temps[below - 1] : 1.f;
     const bool greedy = !(temp > 0.f), both = draft && !last && !greedy;
     if (of_draft && !both) return;
-    const double c = greedy ? 0.0 : verify_factor(temp);
-    const float c_hi = (float)__builtin_fmin(c, 1e37), c_lo = (float)(__builtin_fmin(c, 1e37) - (double)c_hi);  // as 32-bit numbers: its own rounding would be on every power
+    // The factor as a 32-bit number, here for all of the row: decisions are those of a temperature 2^-25 off at most.  Never 0, which would make a number of -infinity's power.
+    const float factor = greedy ? 0.f : (float)__builtin_fmin(__builtin_fmax(verify_factor(temp), 1e-30), 1e37);
+    const double c = factor;
 
     VerifySum mine = {0.0, -__builtin_inff(), 0};
     unsigned best = 0;
@@ -162,8 +171,7 @@ __device__ __forceinline__ void verify_rows_body(const void* __restrict__ logits
                 float p[4];
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
-                    const float v = cur.value(e + k), d = __builtin_fmaxf(v - mm, -3.402823466e38f), x = __builtin_fmaf(d, c_hi, d * c_lo);
-                    p[k] = __builtin_amdgcn_exp2f(v == -__builtin_inff() ? v : x);
+                    p[k] = __builtin_amdgcn_exp2f(cur.minus(e + k, mm) * factor);
                 }
                 mine.s += (double)((p[0] + p[1]) + (p[2] + p[3]));
             }
@@ -271,7 +279,7 @@ __device__ __forceinline__ int verify_find(double v, double aim, double& before,
 template <int T>
 __device__ __forceinline__ void verify_pick_body(const void* __restrict__ logits, size_t ld, const void* __restrict__ draft, size_t ldd, int vocab, int t, int seq_first,
                                                  const int* __restrict__ row0, const int* drafted, const float* __restrict__ u, const float* __restrict__ temps,
-                                                 int segs, int seg_len, const VerifyRow* __restrict__ rows, VerifyPart* __restrict__ parts, int* __restrict__ tickets,
+                                                 int segs, const VerifyRow* __restrict__ rows, VerifyPart* __restrict__ parts, int* __restrict__ tickets,
                                                  int* tokens, int* __restrict__ accepted) {
     __shared__ double red[VERIFY_WAVES], sums[5][VERIFY_WAVES], starts[256];
     __shared__ int found[2];
@@ -283,156 +291,184 @@ __device__ __forceinline__ void verify_pick_body(const void* __restrict__ logits
         if (seg == 0 && tid == 0) accepted[b] = 0;
         return;
     }
+    const float temp = temps ? temps[b] : 1.f, draw = u[r1 - 1];
     int stop = r1 - 1;
-    for (int from = r0; from < r1 - 1; from += 64) {
-        const unsigned long long no = __ballot(from + lane < r1 - 1 && rows[min(from + lane, r1 - 1)].accepted == 0);
-        if (no) {
-            stop = from + __builtin_ctzll(no);
-            break;
-        }
+    VerifyRow r;
+    for (int from = r0;; from += 64) {  // what is known of 64 rows, one to a lane
+        const VerifyRow mine = rows[min(from + lane, r1 - 1)];
+        const unsigned long long no = __ballot(from + lane < r1 - 1 && mine.accepted == 0);
+        if (!no && from + 64 < r1) continue;
+        const int of = no ? __builtin_ctzll(no) : r1 - 1 - from;
+        stop = from + of;
+        r.s = verify_of_lane(mine.s, of);
+        r.sd = verify_of_lane(mine.sd, of);
+        r.m = q8_f32((unsigned)__builtin_amdgcn_readlane(__builtin_bit_cast(int, mine.m), of));
+        r.md = q8_f32((unsigned)__builtin_amdgcn_readlane(__builtin_bit_cast(int, mine.md), of));
+        r.best = __builtin_amdgcn_readlane(mine.best, of);
+        break;
     }
-    const VerifyRow r = rows[stop];
-    const float temp = temps ? temps[b] : 1.f;
     const bool greedy = !(temp > 0.f), last = stop == r1 - 1, both = draft && !last && r.sd > 0.0;
     int token = greedy && r.s > 0.0 ? r.best : -1;
     if (greedy || !(r.s > 0.0)) {
         if (seg != 0) return;
     } else {
-        constexpr int SIZE = ScoreChunk<T>::SIZE, E = ScoreChunk<T>::E;
-        constexpr unsigned STAGE = ScoreChunk<T>::STAGE, STEP = VERIFY_WAVES * STAGE;
+        constexpr int SIZE = ScoreChunk<T>::SIZE, E = ScoreChunk<T>::E, PER = ScoreChunk<T>::PER;
+        constexpr int STAGE = ScoreChunk<T>::STAGE;
         const char* const z = static_cast<const char*>(logits) + (size_t)stop * ld * SIZE;
         const char* const zd = static_cast<const char*>(draft) + (size_t)stop * ldd * SIZE;
         const double c = verify_factor(temp);
-        const float draw = u[r1 - 1];
         const int x = last || draft ? -1 : drafted[stop];  // left out: the token that was certain to its draft
-        const unsigned lo = (unsigned)seg * (unsigned)seg_len, hi = min(lo + (unsigned)seg_len, (unsigned)vocab);
-        double sum[5] = {0.0, 0.0, 0.0, 0.0, 0.0};
         const double rough = both ? r.s / r.sd : 0.0;  // p > q: e > d S / S_draft
-        for (unsigned i = lo + wave * STAGE; i < hi; i += STEP) {
+        const int parts_n = segs * VERIFY_WAVES;
+        VerifyPart* const of_seq = parts + (size_t)b * parts_n;
+        auto load = [&](ScoreChunk<T>& to, const char* from, int part) {
+            const int i = part * STAGE;
+            to.load(from + (size_t)i * SIZE, i < vocab ? (unsigned)(vocab - i) : 0u, lane);
+        };
+        auto put = [&](int part, int k, double v) { __hip_atomic_store(reinterpret_cast<bits_t*>(of_seq[part].v + k), __builtin_bit_cast(bits_t, v), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
+        {
+            const int part = seg * VERIFY_WAVES + wave;
+            double sum[5] = {0.0, 0.0, 0.0, 0.0, 0.0};
             ScoreChunk<T> v, d;
-            v.load(z + (size_t)i * SIZE, hi - i, lane);
+            load(v, z, part);
             if (both) {
-                d.load(zd + (size_t)i * SIZE, hi - i, lane);
+                load(d, zd, part);
+                float over = 0.f, near = 0.f;
 #pragma unroll
                 for (int e = 0; e < E; e++) {
-                    const double p = verify_power(v.value(e), r.m, c), q = verify_power(d.value(e), r.md, c), more = p - q * rough;
-                    const bool over = more > 0.0, near = __builtin_fabs(more) <= VERIFY_NEAR * p;
+                    const double p = verify_power(v.value(e), r.m, c), q = verify_power(d.value(e), r.md, c), more = __builtin_fma(-q, rough, p);
+                    const float qf = (float)q;
                     sum[VERIFY_E] += p;
                     sum[VERIFY_D] += q;
-                    sum[VERIFY_E_OVER] += over ? p : 0.0;
-                    sum[VERIFY_D_OVER] += over ? q : 0.0;
-                    sum[VERIFY_E_NEAR] += near ? p : 0.0;
+                    sum[VERIFY_MORE] += __builtin_fmax(more, 0.0);
+                    over += more > 0.0 ? qf : 0.f;
+                    near += __builtin_fabs(more) <= VERIFY_NEAR * p ? qf : 0.f;
+                    // 2 powers of each under way at once: more take the registers of whole waves
+                    if (e % 2 == 1) asm volatile("" : "+v"(sum[VERIFY_E]), "+v"(sum[VERIFY_D]), "+v"(sum[VERIFY_MORE]), "+v"(over), "+v"(near));
+                }
+                sum[VERIFY_D_OVER] = over;
+                sum[VERIFY_D_NEAR] = near;
+#pragma unroll
+                for (int k = 0; k < 5; k++) {
+                    sum[k] = verify_wave_sum(sum[k]);
+                    if (lane == k) put(part, k, sum[k]);
                 }
             } else {
-                const int out = x - (int)i - ScoreChunk<T>::at(lane, 0);
+                const int out = x - part * STAGE - ScoreChunk<T>::at(lane, 0);
 #pragma unroll
                 for (int e = 0; e < E; e++) {
                     const double p = verify_power(v.value(e), r.m, c);
                     sum[VERIFY_E] += out == ScoreChunk<T>::at(0, e) ? 0.0 : p;
+                    if (e % 2 == 1) asm volatile("" : "+v"(sum[VERIFY_E]));
                 }
+                sum[VERIFY_E] = verify_wave_sum(sum[VERIFY_E]);
+                if (lane == 0) put(part, VERIFY_E, sum[VERIFY_E]);
             }
         }
-        // five sums over the workgroup at once, or the first alone; all threads get them
-        auto of_all = [&](double (&v)[5]) {
+        // complete before the ticket is drawn; read behind the barrier that follows its return
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        if (segs > 1) {
+            if (tid == 0) last_one = __hip_atomic_fetch_add(tickets + b, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == segs - 1;
+            __syncthreads();
+            if (!last_one) return;
+            if (tid == 0) __hip_atomic_store(tickets + b, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);  // for the next launch
+        }
+        // sums over the workgroup, or the first alone; all threads get them
+        auto of_all = [&](double (&v)[5], int count) {
             __syncthreads();
 #pragma unroll
             for (int k = 0; k < 5; k++) {
-                if (k > 0 && !both) break;
+                if (k >= count) break;
                 const double w = verify_wave_sum(v[k]);
                 if (lane == 0) sums[k][wave] = w;
             }
             __syncthreads();
 #pragma unroll
-            for (int k = 0; k < 5; k++) v[k] = k == 0 || both ? (sums[k][0] + sums[k][1]) + (sums[k][2] + sums[k][3]) : 0.0;
+            for (int k = 0; k < 5; k++) v[k] = k < count ? (sums[k][0] + sums[k][1]) + (sums[k][2] + sums[k][3]) : 0.0;
         };
-        of_all(sum);
-        VerifyPart* const of_seq = parts + (size_t)b * segs;
-        if (segs > 1) {
-            if (tid == 0) {
-#pragma unroll
-                for (int k = 0; k < 5; k++)
-                    if (k == 0 || both) __hip_atomic_store(reinterpret_cast<bits_t*>(of_seq[seg].v + k), __builtin_bit_cast(bits_t, sum[k]), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                // complete before the ticket is drawn; read behind the barrier that follows its return
-                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-                last_one = __hip_atomic_fetch_add(tickets + b, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == segs - 1;
-            }
-            __syncthreads();
-            if (!last_one) return;
-            if (tid == 0) __hip_atomic_store(tickets + b, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);  // for the next launch
-        }
-        // Segments tid, tid + 256, ..: the first is kept in registers
-        auto fetch = [&](int s, double (&v)[5]) {
+        // Parts tid, tid + 256, ..: the first is kept in registers
+        auto fetch = [&](int part, double (&v)[5]) {
 #pragma unroll
             for (int k = 0; k < 5; k++) {
                 v[k] = 0.0;
-                if (s < segs && (k == 0 || both))
-                    v[k] = segs == 1 ? sum[k] : __builtin_bit_cast(double, __hip_atomic_load(reinterpret_cast<const bits_t*>(of_seq[s].v + k), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+                if (part < parts_n && (k == 0 || both))
+                    v[k] = __builtin_bit_cast(double, __hip_atomic_load(reinterpret_cast<const bits_t*>(of_seq[part].v + k), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
             }
         };
         double first[5], all[5];
         fetch(tid, first);
 #pragma unroll
         for (int k = 0; k < 5; k++) all[k] = first[k];
-        for (int s = tid + 256; s < segs; s += 256) {
+        for (int part = tid + 256; part < parts_n; part += 256) {
             double v[5];
-            fetch(s, v);
+            fetch(part, v);
 #pragma unroll
             for (int k = 0; k < 5; k++) all[k] += v[k];
         }
-        of_all(all);
+        of_all(all, both ? 5 : 1);
         const double inv = 1.0 / all[VERIFY_E], inv_d = both ? 1.0 / all[VERIFY_D] : 0.0;
+        const double left = both ? rough - all[VERIFY_E] * inv_d : 0.0;  // max(0, p - q) by what is known now: that of the rough factor, and this much of the draft's
         bool only_p = !both, again = false;
         auto weight = [&](float v, float d, int at) {
             const double p = verify_power(v, r.m, c) * inv;
             if (only_p) return at == x ? 0.0 : p;
             return __builtin_fmax(p - verify_power(d, r.md, c) * inv_d, 0.0);
         };
-        const int run = (seg_len + 255) / 256;  // neighbours to a thread: 16, or 32 of 16-bit logits
-        // the sum of this thread's run of segment s
-        auto of_run = [&](int s) {
-            const int from = s * seg_len + tid * run, to = min(min(from + run, (s + 1) * seg_len), vocab);
-            double w_sum = 0.0;
-            for (int at = from; at < to; at += 16) {
-                float v[16], d[16];
-                q8_load16<T>(z, (size_t)at, to - at, v);
-                if (!only_p) q8_load16<T>(zd, (size_t)at, to - at, d);
-#pragma unroll
-                for (int e = 0; e < 16; e++) {
-                    const double w = weight(v[e], only_p ? 0.f : d[e], at + e);
-                    w_sum += at + e < to ? w : 0.0;
-                }
-            }
-            return w_sum;
+        auto share = [&](const double (&v)[5]) {
+            return only_p ? v[VERIFY_E] * inv : again ? v[VERIFY_MORE] : __builtin_fmax(__builtin_fma(left, v[VERIFY_D_OVER], v[VERIFY_MORE]) * inv, 0.0);
         };
-        auto share = [&](const double (&v)[5]) { return only_p ? v[VERIFY_E] * inv : again ? v[VERIFY_E_OVER] : __builtin_fmax(v[VERIFY_E_OVER] * inv - v[VERIFY_D_OVER] * inv_d, 0.0); };
-        // what the segments have to give
+        // what the parts have to give
         auto total = [&]() {
             double v[5] = {share(first), 0.0, 0.0, 0.0, 0.0};
-            for (int s = tid + 256; s < segs; s += 256) {
+            for (int part = tid + 256; part < parts_n; part += 256) {
                 double w[5];
-                fetch(s, w);
+                fetch(part, w);
                 v[0] += share(w);
             }
-            of_all(v);
+            of_all(v, 1);
             return v[0];
         };
         double whole = only_p ? (all[VERIFY_E] > 0.0 ? 1.0 : 0.0) : total();
         if (both) {
             const double off = __builtin_fabs(rough * all[VERIFY_D] * inv - 1.0);
-            again = !(off < VERIFY_NEAR) || off * all[VERIFY_E_NEAR] * inv > 1e-9 * whole;
+            again = !(off < VERIFY_NEAR) || off * rough * all[VERIFY_D_NEAR] * inv > 1e-9 * whole;
             if (again) {
-                for (int s = 0; s < segs; s++) {
-                    double v[5] = {of_run(s), 0.0, 0.0, 0.0, 0.0};
-                    of_all(v);
-                    if (s == tid) first[VERIFY_E_OVER] = v[0];
-                    if (segs > 256 && tid == 0)
-                        __hip_atomic_store(reinterpret_cast<bits_t*>(of_seq[s].v + VERIFY_E_OVER), __builtin_bit_cast(bits_t, v[0]), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                for (int part = wave; part < parts_n; part += VERIFY_WAVES) {
+                    ScoreChunk<T> v, d;
+                    load(v, z, part);
+                    load(d, zd, part);
+                    double w = 0.0;
+#pragma unroll
+                    for (int e = 0; e < E; e++) {
+                        w += weight(v.value(e), d.value(e), -1);
+                        if (e % 2 == 1) asm volatile("" : "+v"(w));
+                    }
+                    w = verify_wave_sum(w);
+                    if (lane == 0) put(part, VERIFY_MORE, w);
                 }
                 asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
                 __syncthreads();
+                fetch(tid, first);
                 whole = total();
             }
         }
+        // Of a part, thread i has the PER neighbours from i PER on
+        auto of_run = [&](int part) {
+            const int from = part * STAGE + tid * PER, to = min(from + PER, vocab);
+            double w = 0.0;
+            if (from + PER <= vocab) {
+                const u4_t a = *reinterpret_cast<const u4_any_t*>(z + (size_t)from * SIZE), g = only_p ? a : (u4_t)*reinterpret_cast<const u4_any_t*>(zd + (size_t)from * SIZE);
+                ScoreChunk<T> v, d;
+                v.w[0] = a;
+                d.w[0] = g;
+#pragma unroll
+                for (int e = 0; e < PER; e++) w += weight(v.value(e), d.value(e), from + e);
+            } else {
+                for (int at = from; at < to; at++) w += weight(q8_load1<T>(z, (size_t)at), only_p ? 0.f : q8_load1<T>(zd, (size_t)at), at);
+            }
+            return w;
+        };
         // Drawn from p where p is nowhere above q, or where no token of the segment that the draw falls into is left at the second look
         for (int attempt = 0; attempt < 2 && token < 0; attempt++) {
             if (attempt == 1) {
@@ -445,12 +481,12 @@ __device__ __forceinline__ void verify_pick_body(const void* __restrict__ logits
             double before = 0.0, from = 0.0;
             int at = -1;
             bool none = true;
-            for (int s = 0; s < segs && none; s += 256) {
+            for (int part = 0; part < parts_n && none; part += 256) {
                 double ahead = from, v[5];
-                if (s > 0) fetch(s + tid, v);
-                const int f = verify_find(s > 0 ? share(v) : share(first), aim, ahead, red, found, starts, none);
+                if (part > 0) fetch(part + tid, v);
+                const int f = verify_find(part > 0 ? share(v) : share(first), aim, ahead, red, found, starts, none);
                 if (f >= 0) {
-                    at = s + f;
+                    at = part + f;
                     before = none ? starts[f] : ahead;
                 }
                 from += red[0] + red[1] + red[2] + red[3];
@@ -460,8 +496,8 @@ __device__ __forceinline__ void verify_pick_body(const void* __restrict__ logits
             const int f = verify_find(of_run(at), aim, before, red, found, starts, none);
             if (f >= 0 && wave == 0) {
                 if (none) before = starts[f];
-                const int e = at * seg_len + f * run + lane;
-                const bool in = lane < run && e < min((at + 1) * seg_len, vocab);
+                const int e = at * STAGE + f * PER + lane;
+                const bool in = lane < PER && e < vocab;
                 const float v = in ? q8_load1<T>(z, (size_t)e) : 0.f, d = in && !only_p ? q8_load1<T>(zd, (size_t)e) : 0.f;
                 const double w = in ? weight(v, d, e) : 0.0, run_to = before + verify_wave_scan(w);  // by all lanes
                 const unsigned long long those = __ballot(w > 0.0 && run_to > aim), some = __ballot(w > 0.0);
@@ -484,8 +520,8 @@ __device__ __forceinline__ void verify_pick_body(const void* __restrict__ logits
     }                                                                                                                              \
     extern "C" __global__ __launch_bounds__(256) void w4a16_verify_pick_##NAME(                                                    \
         const void* logits, size_t ld, const void* draft, size_t ldd, int vocab, int t, int seq_first, const int* row0, const int* drafted, const float* u, \
-        const float* temps, int segs, int seg_len, const VerifyRow* rows, VerifyPart* parts, int* tickets, int* tokens, int* accepted) {  \
-        verify_pick_body<T>(logits, ld, draft, ldd, vocab, t, seq_first, row0, drafted, u, temps, segs, seg_len, rows, parts, tickets, tokens, accepted); \
+        const float* temps, int segs, const VerifyRow* rows, VerifyPart* parts, int* tickets, int* tokens, int* accepted) {  \
+        verify_pick_body<T>(logits, ld, draft, ldd, vocab, t, seq_first, row0, drafted, u, temps, segs, rows, parts, tickets, tokens, accepted); \
     }
 VERIFY_KERNELS(f32, Q8_F32)
 VERIFY_KERNELS(f16, Q8_F16)
