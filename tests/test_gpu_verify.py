@@ -1,5 +1,6 @@
-"""Verification of drafted tokens on the GPU against the definition in 64 bits.  Both sides hold powers and sums to 10^-11 and better, so that of the some 10^5 draws here the
-chance that one lies between their borders is V * 10^-11 each, 10^-1 in 10^3 runs of all: tokens and counts are equal."""
+"""Verification of drafted tokens on the GPU against the definition in 64 bits.  Both sides hold what draws to 10^-11 and better, so that of the some 10^5 draws here the
+chance that one lies between their borders is V * 10^-11 each, 10^-1 in 10^3 runs of all; decisions to 10^-6, of some 10^4 here.  Their inputs are fixed, as are the results of both sides:
+tokens and counts are equal."""
 import numpy as np
 import pytest
 
@@ -195,6 +196,20 @@ def test_strides_and_alignment(dec, kind, v, ld, ldd, off):
         got = call(dec, b, flat[0], flat[1], row0, drafted, u, temps, kind, v, ld=ld, ldd=ldd, off=off)
     want = ref.verified(z, d, row0, drafted, u, temps, np.full(t, -1, np.int32))
     assert np.array_equal(got[0], want[0]) and np.array_equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("kind", TYPES)
+def test_temperatures_of_any_size(dec, kind):
+    """Above all logits' sizes every token that is not ruled out is as likely; far below them the largest is certain."""
+    bits, z, dbits, d, row0, drafted, u, _ = problem(9, [3] * 12, 700, kind)
+    for rows in (z, d):
+        rows[:, 100:400] = -np.inf
+    (bits, z), (dbits, d) = w8.narrow(z, kind), w8.narrow(d, kind)
+    drafted = np.where((drafted >= 100) & (drafted < 400), 5, drafted)
+    for temp in (np.inf, 3e38, 1e30, 1e-6, 1e-30, 1e-38):
+        temps = np.full(12, temp, np.float32)
+        check(dec, bits, z, dbits, d, row0, drafted, u, temps, kind)
+        check(dec, bits, z, None, None, row0, drafted, u, temps, kind)
 
 
 def test_rows_of_no_sequence_stay_as_they_are(dec):
