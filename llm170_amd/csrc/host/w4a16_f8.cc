@@ -50,13 +50,13 @@ extern "C" int w4a16_norm_resid_f8(w4a16_ctx* ctx, uint64_t x_dev, uint64_t nw_d
     W4_TRY(w4_hip(hipSetDevice(ctx->device), "hipSetDevice"));
     int wo = (int)w_off, h = (int)hidden, kb = (int)w4_q8_blocks(hidden), r = (int)w4_q8_tile_rows(t);
     size_t s_ld = t;
-    const size_t most = w4_rows_per_launch(1024);
+    const size_t most = w4_rows_per_launch(256);
     for (size_t at = 0; at < t; at += most) {
         const size_t rows = std::min(most, t - at);
         uint64_t x_at = x_dev + at * hidden * 4, ab_at = ab_dev + at * hidden * 4, q_at = q_dev + at * kb * 128, s_at = s_dev + at * 4;
         int ti = (int)rows;
         void* params[] = {&x_at, &nw_dev, &ab_at, &q_at, &s_at, &wo, &h, &kb, &r, &ti, &s_ld};
-        W4_TRY(w4_launch(ctx, "w4a16_norm_resid_f8", r == 16 ? ceil_div(rows, 128) * 128 : (unsigned)rows, 1, 1024, 0, params));
+        W4_TRY(w4_launch(ctx, "w4a16_norm_resid_f8", r == 16 ? ceil_div(rows, 128) * 128 : (unsigned)rows, 1, 256, 0, params));
     }
     return 0;
 }

@@ -21,6 +21,14 @@ __device__ __forceinline__ unsigned f8_block_max(unsigned v) {
     return max(v, (unsigned)__builtin_amdgcn_update_dpp((int)v, (int)v, 0x141, 0xf, 0xf, false));  // row_half_mirror
 }
 
+// Largest of 32 lanes
+__device__ __forceinline__ unsigned f8_half_wave_max(unsigned v) {
+    v = f8_block_max(v);
+    v = max(v, (unsigned)__builtin_amdgcn_update_dpp((int)v, (int)v, 0x140, 0xf, 0xf, false));  // row_mirror
+    const auto rows = __builtin_amdgcn_permlane16_swap(v, v, false, false);  // the even one's and the odd one's of each two rows of 16
+    return max((unsigned)rows[0], (unsigned)rows[1]);
+}
+
 typedef short f8_pair_t __attribute__((ext_vector_type(2)));
 typedef __bf16 bf2_t __attribute__((ext_vector_type(2)));
 

@@ -147,10 +147,15 @@ __device__ __forceinline__ unsigned q8_wave_max(unsigned v) {
 
 // The sum of one value per thread of 1024, the same bits as in w4a16_norm_resid (pairwise at strides 512 .. 1) with one barrier: strides 512 .. 64 pair
 // waves, so every lane adds the sixteen waves' partials of its own lane in that order; strides 32 .. 1 pair lanes, and lane 0 has the sum.
+__device__ __forceinline__ float q8_norm_total(const float* red);
 __device__ __forceinline__ float q8_norm_sum(float ss, float* red) {
-    const int tid = threadIdx.x;
-    red[tid] = ss;
+    red[threadIdx.x] = ss;
     __syncthreads();
+    return q8_norm_total(red);
+}
+// of the 1024 values in red, behind a barrier; by any wave
+__device__ __forceinline__ float q8_norm_total(const float* red) {
+    const int tid = threadIdx.x;
     float w[16];
 #pragma unroll
     for (int i = 0; i < 16; i++) w[i] = red[i * 64 + (tid & 63)];
