@@ -317,6 +317,21 @@ def test_results_at_any_element_alignment(dec):
                 assert np.array_equal(dec.cc.d2h(y, (t, n), w8.bits_type(y_type)), w8.as_type(want, y_type))
 
 
+@pytest.mark.parametrize("k,tiles", [(300, False), (1024, True)])
+@pytest.mark.parametrize("t", [17, 33, 64])
+def test_wide_linears_of_few_rows(dec, t, k, tiles):
+    """17 to 64 rows go to tiles, most of whose rows are not there, where k is long enough for them."""
+    n, cc = 65536 + 40, dec.cc
+    q, s, w, sv = ref.small_whole(t, t, n, k)
+    dec.upload_lin_f8("wide", w, sv, n, k)
+    want = ref.product(q, s, w, sv)[0].astype(np.float32)
+    with w8.Buffers(cc) as b:
+        y = b.filled(t * n * 2 + 64)
+        dec.lin_forward_f8("wide", b.put(ref.pack(q, t, k)), y, t, x_type=ffi.F8, xs_dev=b.put(s), y_type=ffi.F16)
+        assert not tiles or "exact" in cc.last_launch_symbol()
+        assert np.array_equal(cc.d2h(y, (t, n), np.uint16), w8.as_type(want, ffi.F16)) and (cc.d2h(y + t * n * 2, (64,), np.uint8) == 0xA5).all()
+
+
 def refused(code, words, call):
     with pytest.raises(ops.W4a16Error) as e:
         call()
