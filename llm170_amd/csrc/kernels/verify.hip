@@ -8,11 +8,11 @@
 // takes most of the time: 193 rows of 131072 bf16 with 129 drafts' 22.4 us (84 MB, 3.8 TB/s), 400 of 100003 f16 with 200 drafts' 31.9 (120 MB).
 // Pick: of the first row that is not accepted alone, a stage of 64 lanes to a wave.  Running sums over a vocabulary meet a border between two tokens about once in V / (relative error)
 // draws, so powers and sums are of 64 bits: 2^x by a polynomial of degree 8 (interpolation at Chebyshev nodes of [-1/2, 1/2], off by 1.1e-12), some 17 instructions of four
-// cycles, which are what takes the time where there are many sequences: 64 of them 21.8 us (7 of arithmetic; launch, loads that depend on each other and the last workgroup's work the rest), 200 48.5 (28).
+// cycles, which are what takes the time where there are many sequences: 64 of them 20.6 us (7 of arithmetic; launch, loads that depend on each other and the last workgroup's work the rest), 200 45.5 (28).
 // A wave leaves sum p, sum q and, by the first launch's sums (`rough` of the draft's power is one of the target's), sum max(0, p - q) and the sum of q where p is above q: what is
 // known of the whole sums then changes it by their difference times the last.  Tokens that the first launch's 10^-7 puts on the wrong side have no more than that share of themselves to
 // give; where that is over 10^-9 of the whole, target and draft being nearly alike, the sums are made again with what is known now.  The last workgroup of a sequence finds the
-// wave's stage that holds the draw, a thread of it sums a few neighbours, and the few that hold it are gone over again, an element to a lane.
+// wave's stage that holds the draw, and the thread in it whose few neighbours do.
 #include "score_common.hpp"
 
 #define VERIFY_WAVES 4
@@ -416,20 +416,9 @@ __device__ __forceinline__ void verify_pick_body(const void* __restrict__ logits
             return __builtin_fmax(p - verify_power(d, r.md, c) * inv_d, 0.0);
         };
         auto share = [&](const double (&v)[5]) {
-            return only_p ? v[VERIFY_E] * inv : again ? v[VERIFY_MORE] : __builtin_fmax(__builtin_fma(left, v[VERIFY_D_OVER], v[VERIFY_MORE]) * inv, 0.0);
+            return only_p ? v[VERIFY_E] * inv : again ? v[VERIFY_MORE] : __builtin_fma(left, v[VERIFY_D_OVER], v[VERIFY_MORE]) * inv;  // below 0 where tokens are nearly alike
         };
-        // what the parts have to give
-        auto total = [&]() {
-            double v[5] = {share(first), 0.0, 0.0, 0.0, 0.0};
-            for (int part = tid + 256; part < parts_n; part += 256) {
-                double w[5];
-                fetch(part, w);
-                v[0] += share(w);
-            }
-            of_all(v, 1);
-            return v[0];
-        };
-        double whole = only_p ? (all[VERIFY_E] > 0.0 ? 1.0 : 0.0) : total();
+        double whole = only_p ? (all[VERIFY_E] > 0.0 ? 1.0 : 0.0) : share(all);
         if (both) {
             const double off = __builtin_fabs(rough * all[VERIFY_D] * inv - 1.0);
             again = !(off < VERIFY_NEAR) || off * rough * all[VERIFY_D_NEAR] * inv > 1e-9 * whole;
@@ -450,24 +439,34 @@ __device__ __forceinline__ void verify_pick_body(const void* __restrict__ logits
                 asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
                 __syncthreads();
                 fetch(tid, first);
-                whole = total();
+                double v[5] = {first[VERIFY_MORE], 0.0, 0.0, 0.0, 0.0};
+                for (int part = tid + 256; part < parts_n; part += 256) {
+                    double w[5];
+                    fetch(part, w);
+                    v[0] += w[VERIFY_MORE];
+                }
+                of_all(v, 1);
+                whole = v[0];
             }
         }
-        // Of a part, thread i has the PER neighbours from i PER on
+        // Of a part, thread i has the PER neighbours from i PER on: their weights, and the sum of them
+        double weights[PER];
         auto of_run = [&](int part) {
-            const int from = part * STAGE + tid * PER, to = min(from + PER, vocab);
-            double w = 0.0;
+            const int from = part * STAGE + tid * PER;
+            ScoreChunk<T> v, d;
             if (from + PER <= vocab) {
-                const u4_t a = *reinterpret_cast<const u4_any_t*>(z + (size_t)from * SIZE), g = only_p ? a : (u4_t)*reinterpret_cast<const u4_any_t*>(zd + (size_t)from * SIZE);
-                ScoreChunk<T> v, d;
-                v.w[0] = a;
-                d.w[0] = g;
+                v.w[0] = *reinterpret_cast<const u4_any_t*>(z + (size_t)from * SIZE);
+                if (!only_p) d.w[0] = *reinterpret_cast<const u4_any_t*>(zd + (size_t)from * SIZE);
 #pragma unroll
-                for (int e = 0; e < PER; e++) w += weight(v.value(e), d.value(e), from + e);
+                for (int e = 0; e < PER; e++) weights[e] = weight(v.value(e), only_p ? 0.f : d.value(e), from + e);
             } else {
-                for (int at = from; at < to; at++) w += weight(q8_load1<T>(z, (size_t)at), only_p ? 0.f : q8_load1<T>(zd, (size_t)at), at);
+#pragma unroll
+                for (int e = 0; e < PER; e++) weights[e] = from + e < vocab ? weight(q8_load1<T>(z, (size_t)(from + e)), only_p ? 0.f : q8_load1<T>(zd, (size_t)(from + e)), from + e) : 0.0;
             }
-            return w;
+            double sum = 0.0;
+#pragma unroll
+            for (int e = 0; e < PER; e++) sum += weights[e];
+            return sum;
         };
         // Drawn from p where p is nowhere above q, or where no token of the segment that the draw falls into is left at the second look
         for (int attempt = 0; attempt < 2 && token < 0; attempt++) {
@@ -494,14 +493,16 @@ __device__ __forceinline__ void verify_pick_body(const void* __restrict__ logits
             if (at < 0) continue;
             if (tid == 0) chosen = -1;
             const int f = verify_find(of_run(at), aim, before, red, found, starts, none);
-            if (f >= 0 && wave == 0) {
-                if (none) before = starts[f];
-                const int e = at * STAGE + f * PER + lane;
-                const bool in = lane < PER && e < vocab;
-                const float v = in ? q8_load1<T>(z, (size_t)e) : 0.f, d = in && !only_p ? q8_load1<T>(zd, (size_t)e) : 0.f;
-                const double w = in ? weight(v, d, e) : 0.0, run_to = before + verify_wave_scan(w);  // by all lanes
-                const unsigned long long those = __ballot(w > 0.0 && run_to > aim), some = __ballot(w > 0.0);
-                if (lane == 0 && some) chosen = e + (those ? __builtin_ctzll(those) : 63 - __builtin_clzll(some));
+            if (tid == f) {
+                double run = starts[f];
+                int over = -1, some = -1;
+#pragma unroll
+                for (int e = 0; e < PER; e++) {
+                    run += weights[e];
+                    some = weights[e] > 0.0 ? e : some;
+                    over = over < 0 && weights[e] > 0.0 && run > aim ? e : over;
+                }
+                if (some >= 0) chosen = at * STAGE + f * PER + (over >= 0 ? over : some);
             }
             __syncthreads();
             token = chosen;
