@@ -153,3 +153,51 @@ def test_a_step_stage_by_stage_and_replayed(dec, lens):
             assert all(np.array_equal(a, c) for a, c in zip(st.results(), eager[seed])), seed
             dec.quant_rows_f8(st.p["ab"], st.p["q"], st.p["s"], t, HIDDEN, x_type=ffi.F32)  # eager work between them
         graph.destroy()
+
+
+def test_two_contexts_and_two_graphs_at_once(dec):
+    """Launches of two contexts without a wait between them, and two graphs over one scratch: the results of one after the other."""
+    other = ops.W4a16Dec()
+    try:
+        with w8.Buffers(dec.cc) as b0, w8.Buffers(other.cc) as b1:
+            steps = [Step(dec, b0, [5, 2]), Step(other, b1, [3] * 9)]
+            want = []
+            for st in steps:
+                per = []
+                for seed in (11, 12):
+                    st.start(seed)
+                    for _, go in st.stages():
+                        go()
+                    per.append(st.results())
+                want.append(per)
+            for at, seed in enumerate((11, 12)):
+                for st in steps:
+                    st.start(seed)
+                for (_, a), (_, c) in zip(steps[0].stages(), steps[1].stages()):  # in turns
+                    a()
+                    c()
+                for st, per in zip(steps, want):
+                    st.cc.sync()
+                    assert all(np.array_equal(x, y) for x, y in zip(st.results(), per[at]))
+            more = Step(dec, b0, [4, 4, 1])
+            more.start(13)
+            for _, go in more.stages():
+                go()
+            alone = more.results()
+            graphs = []
+            for st in (steps[0], more):
+                st.cc.capture_begin()
+                for _, go in st.stages():
+                    go()
+                graphs.append(st.cc.capture_end())
+            for _ in range(3):
+                steps[0].start(12)
+                more.start(13)
+                for g in graphs:
+                    g.launch()
+                dec.cc.sync()
+                assert all(np.array_equal(x, y) for x, y in zip(steps[0].results(), want[0][1])) and all(np.array_equal(x, y) for x, y in zip(more.results(), alone))
+            for g in graphs:
+                g.destroy()
+    finally:
+        other.cc.close()
