@@ -6,7 +6,7 @@
 // numbers 1.6e-5 of the results' size, 4.2 PFLOP/s alone (16x16x128; 32x32x64 3.8), 3.5 with the scaling.  As f16, which holds every e4m3 number, the same
 // sums are those of 32 bits (1e-8), at the f16 instruction's 1.6.  So f16 for f32 results, up to 64 rows, where
 // the weight stream is what takes the time, and for gated results of up to 1024 rows: the next linear quantises those, and a number that falls to the other side of one of its
-// roundings shows 4000 times what was dropped (two linears at 300 rows: 1.4e-3 of their result's size, with f16 products 2e-4).  e4m3 for the other 16-bit results, whose own rounding
+// roundings shows 4000 times what was dropped (two linears at 300 rows: 1.4e-3 of their result's size, with f16 products 2e-4 to 5e-4).  e4m3 for the other 16-bit results, whose own rounding
 // is ten times as large and more: 5120 x 17408 at 300 rows 53.5 us, with f16 products 70.8.
 #include "f8_common.hpp"
 
